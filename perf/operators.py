@@ -165,7 +165,7 @@ def _make(case, seed):
             kc[i], ks[i] = _quantise(_vectors((h, cap, d), g, dev, False), case["fmt"])
             vc[i], vs[i] = _quantise(_vectors((h, cap, d), g, dev, True), case["fmt"])
         s = dict(q=(2 * torch.randn((b, n, case["heads"], d), generator=g, device=dev)).to(dt), kc=kc, vc=vc, ks=ks, vs=vs,
-                 lengths=torch.tensor(lengths, dtype=torch.int32, device=dev), tree=None, sees=None, gate=None)
+                 start=torch.tensor([m - n for m in lengths], dtype=torch.int32, device=dev), tree=None, sees=None, gate=None)
         if case["mask"] == "tree":
             sees = np.stack([_tree(n, rng) for _ in range(b)])
             s["sees"] = torch.tensor(sees, device=dev)
@@ -219,7 +219,7 @@ def _run_own(s):
         kv_append(s["cache"], s["k"], s["v"], s["start"])
         return kv_read(s["cache"], s["start"], case["tokens"], dtype=TYPES[case["dtype"]])
     if case["op"] == "attend":
-        return cached_attention(s["q"], s["cache"], s["lengths"], tree=s["tree"], gate=s["gate"])
+        return cached_attention(s["q"], s["cache"], s["start"], tree=s["tree"], gate=s["gate"])
     return adjust_logits(s["logits"], history=s["history"], repetition=s["repetition"], frequency=s["frequency"],
                          presence=s["presence"], bias_ids=s["bias_ids"], bias_values=s["bias_values"], allowed=s["allowed"])
 
@@ -246,7 +246,7 @@ def _plain_cache(s):
 def _sees(s, n, cap):
     """[B, n, cap]: which cached positions each new token sees."""
     pos = torch.arange(cap, device=s["q"].device)
-    base = s["lengths"].long() - n
+    base = s["start"].long()  # where the new tokens begin
     if s["sees"] is None:
         return pos[None, None, :] <= (base[:, None] + torch.arange(n, device=pos.device))[:, :, None]
     off = pos[None, :] - base[:, None]  # [B, cap]
