@@ -181,7 +181,8 @@ GSQ_API int gsq_qmm_gather_mc(int qtype, const void* x, int x_dtype, const uint8
 
 /* Synchronises `stream`, then returns and clears the device error word the
  * kernels of the current device write (0 = none; 1 = a bounded wait expired;
- * 2 = an embedding id was out of range).  On 1 it also synchronises the
+ * 2 = an embedding id was out of range; 3 = a key or value was appended
+ * outside its cache).  On 1 it also synchronises the
  * device and zero-fills gsq_qmv_noalloc's fixed scratch array; workspaces
  * that the caller passed to gsq_qmv / gsq_qmm / the gathers must be
  * zero-filled again by the caller.  No reference counterpart: the

@@ -123,6 +123,110 @@ GSQ_API int gsq_attn_decode_batch(const float* qkv, int64_t nq, int64_t nkv, con
                                   float* v_cache, int64_t max_len, const int32_t* pos, void* out, int out_dtype,
                                   int64_t batch, gsq_stream_t stream);
 
+/* ---- Quantised key/value cache ------------------------------------------
+ * No reference counterpart (the reference keeps mlx_lm's fp16 cache).  The
+ * cache of one attention layer is four plain tensors:
+ *
+ *   codes   [batch, heads, cap, dim] one byte a value, for keys and values:
+ *           two's-complement int8 (GSQ_KV_INT8) or e4m3 (GSQ_KV_FP8)
+ *   scale   [batch, heads, cap] fp32, for keys and values
+ *
+ * and a stored vector is code * scale.  With a = max|x| over the vector and
+ * m = 127 (int8) or 448 (e4m3), scale = a * (1/m) and code = the nearest (ties
+ * to even) of x / scale, with 1/m, scale and the quotient each rounded to fp32
+ * (scale downwards where m * scale would pass fp32's range).  A zero vector has scale 0; a vector with an Inf
+ * or NaN has scale NaN and reads back as NaN.
+ * dim is 128 or 256; the codes are 16-byte aligned.
+ *
+ * Sequence b's new tokens begin at position start[b * start_stride] (device
+ * int32; stride 0: one position for all, such as the decode position of a
+ * captured graph).  counts (device int32 [batch], or NULL): sequence b has
+ * only counts[b] new tokens, the rest of its rows is padding. */
+typedef enum { GSQ_KV_INT8 = 0, GSQ_KV_FP8 = 1 } gsq_kv_format;
+
+/* Quantises k and v [batch, tokens, heads, dim] (dtype fp32, fp16 or bf16;
+ * strides in elements of the first three dimensions, the last contiguous)
+ * into positions start .. start + tokens - 1.  Padding is skipped.  A
+ * position outside [0, cap) is not written and sets 3 in gsq_device_status. */
+GSQ_API int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_t tokens, int64_t heads,
+                          int64_t dim, const int64_t* k_strides, const int64_t* v_strides, const int32_t* start,
+                          int64_t start_stride, const int32_t* counts, int fmt, void* k_codes, void* v_codes,
+                          float* k_scale, float* v_scale, int64_t cap, gsq_stream_t stream);
+
+/* Reads positions start .. start + tokens - 1 back as k and v [batch, tokens,
+ * heads, dim] of dtype (code * scale in fp32, rounded once; 16-byte aligned).
+ * Padding and positions outside [0, cap) read as zeros. */
+GSQ_API int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* k_scale, const float* v_scale,
+                        int64_t batch, int64_t heads, int64_t cap, int64_t dim, const int32_t* start,
+                        int64_t start_stride, const int32_t* counts, int64_t tokens, void* k, void* v, int dtype,
+                        gsq_stream_t stream);
+
+/* Attention of n new tokens of each sequence, whose keys and values are in
+ * the cache already (gsq_kv_append with the same start and counts):
+ *
+ *   out[b,i,h] = sum_p softmax_p(scale * q[b,i,h] . k[b,p,h']) v[b,p,h']
+ *                [* sigmoid(gate[b,i,h])],   h' = h / (heads / kv_heads)
+ *
+ * over the positions p < cap that row i sees: p <= start + i (a single
+ * token, or a chunk of a prompt), or with `tree` the cached text p < start
+ * and those new tokens p = start + j, j < counts[b], whose bit j is set in
+ * row i of the tree (int32 words [n, ceil(n / 32)] of sequence b at
+ * tree + b * tree_stride, bit j % 32 of word j / 32; n <= 1024; stride 0: one
+ * tree for all).  A row that sees nothing, and padding, gives zeros.
+ *   q     [batch, n, heads, dim] fp16 or bf16, strides in elements of the
+ *         first three dimensions; rows 16-byte aligned
+ *   gate  fp32 of the same shape with strides of its own, or NULL
+ *   out   [batch, n, heads, dim] of q's type, contiguous, 16-byte aligned
+ * workspace: gsq_cached_attention_workspace_size() bytes, 256-byte aligned,
+ * of any content, for this call alone until it has completed. */
+GSQ_API size_t gsq_cached_attention_workspace_size(int64_t batch, int64_t n, int64_t heads, int64_t kv_heads,
+                                                   int64_t dim, int64_t cap);
+GSQ_API int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int64_t batch, int64_t n,
+                                 int64_t heads, int64_t kv_heads, int64_t dim, int fmt, const void* k_codes,
+                                 const void* v_codes, const float* k_scale, const float* v_scale, int64_t cap,
+                                 const int32_t* start, int64_t start_stride, const int32_t* counts,
+                                 const int32_t* tree, int64_t tree_stride, const float* gate,
+                                 const int64_t* gate_strides, float scale, void* out, void* workspace,
+                                 size_t workspace_bytes, gsq_stream_t stream);
+
+/* ---- Logits --------------------------------------------------------------
+ * The history of row r: seen, int32 words [rows, ceil(vocab / 32)] with bit
+ * v % 32 of word v / 32 set for every token v of its prompt or output, and
+ * counts, int32 [rows, vocab], how often its output holds v (zero wherever
+ * the bit is not set).
+ *
+ * gsq_adjust_logits, per row and token v, each step rounded to fp32:
+ *   seen:      z = z > 0 ? z / repetition : z * repetition
+ *   counts>0:  z = z - frequency * counts;  z = z - presence
+ *   z = z + the sum, in list order, of the row's biases of token v
+ *   not allowed: z = -inf
+ * out [rows, vocab] fp32 takes z (it may be the logits themselves when they
+ * are fp32 with row_stride == vocab); next[r] the token of the row's largest
+ * z, the lowest of equal ones (NaN counts as the largest).  With `record`
+ * the history learns next[r] as output.
+ *   logits      fp32, fp16 or bf16, rows row_stride elements apart
+ *   repetition, frequency, presence  device fp32 [rows], or NULL (1, 0, 0);
+ *               they need a history
+ *   bias_ids, bias_values  [rows, biases], at most 65536; ids outside
+ *               [0, vocab) are skipped (padding)
+ *   allowed     words like seen's, row r's at r * allowed_stride (0: one mask
+ *               for all), bit set = allowed; or NULL
+ * workspace: gsq_adjust_logits_workspace_size() bytes, 8-byte aligned, of any
+ * content, for this call alone until it has completed. */
+GSQ_API size_t gsq_adjust_logits_workspace_size(int64_t rows, int64_t vocab);
+GSQ_API int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
+                              int32_t* seen, int32_t* counts, const float* repetition, const float* frequency,
+                              const float* presence, const int32_t* bias_ids, const float* bias_values,
+                              int64_t biases, const int32_t* allowed, int64_t allowed_stride, float* out,
+                              int32_t* next, int record, void* workspace, size_t workspace_bytes,
+                              gsq_stream_t stream);
+
+/* The history of row r learns tokens[r * row_stride + 0 .. n): as output
+ * (generated != 0: bit and count) or as prompt (bit only).  Tokens outside
+ * [0, vocab) are skipped (padding); a token may come any number of times. */
+GSQ_API int gsq_record_tokens(const int32_t* tokens, int64_t row_stride, int64_t rows, int64_t n, int64_t vocab,
+                              int32_t* seen, int32_t* counts, int generated, gsq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

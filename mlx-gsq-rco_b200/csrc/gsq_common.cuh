@@ -162,7 +162,8 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Error codes a kernel can record in the device status word.
-enum DeviceError : int { DEV_OK = 0, DEV_WAIT_TIMEOUT = 1 };
+// (2: an embedding id out of range).
+enum DeviceError : int { DEV_OK = 0, DEV_WAIT_TIMEOUT = 1, DEV_CACHE_POSITION = 3 };
 
 // Spin on an mbarrier phase with a time limit (~2^31 SM cycles, about a
 // second).  On expiry it records DEV_WAIT_TIMEOUT in *err and returns false so

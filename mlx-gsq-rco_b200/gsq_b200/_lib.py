@@ -63,6 +63,15 @@ SIGNATURES = {
                            ctypes.c_float, _P, _P, _I, _P]),
     "gsq_attn_decode_batch": (_I, [_P, _I64, _I64, _P, _P, ctypes.c_float, _I64, ctypes.c_float, _P, _P, _I64, _P, _P,
                                    _I, _I64, _P]),
+    "gsq_kv_append": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I, _P, _P, _P, _P, _I64, _P]),
+    "gsq_kv_read": (_I, [_I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I, _P]),
+    "gsq_cached_attention_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "gsq_cached_attention": (_I, [_P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _P, _I64, _P, _P,
+                                  _I64, _P, _P, ctypes.c_float, _P, _P, _SZ, _P]),
+    "gsq_adjust_logits_workspace_size": (_SZ, [_I64, _I64]),
+    "gsq_adjust_logits": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P, _I, _P,
+                               _SZ, _P]),
+    "gsq_record_tokens": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _I, _P]),
 }
 
 _lib = None
@@ -127,6 +136,25 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+class on_device:
+    """Makes ``device`` the current one for a launch (a launch goes to the
+    current device's context), at no cost where it is already."""
+
+    __slots__ = ("_index", "_before")
+
+    def __init__(self, device: torch.device):
+        self._index = device.index
+
+    def __enter__(self):
+        self._before = torch.cuda.current_device()
+        if self._before != self._index:
+            torch.cuda.set_device(self._index)
+
+    def __exit__(self, *exc):
+        if self._before != self._index:
+            torch.cuda.set_device(self._before)
+
+
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
@@ -165,7 +193,7 @@ DEV_WAIT_TIMEOUT = 1
 def device_status(device: torch.device | None = None) -> int:
     """Synchronise the device's current stream and return (and clear) the
     device error word: 0 none, 1 a bounded wait expired, 2 an embedding id
-    out of range.  After 1 the scratch of the calls may hold stale slots: the
+    out of range, 3 a key or value appended outside its cache.  After 1 the scratch of the calls may hold stale slots: the
     library re-zeroes its own fixed array, and this re-zeroes the workspaces
     the Python layer manages for the device."""
     dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())

@@ -1,4 +1,6 @@
-"""Runtime: packed weight container and the CUDA kernel layer."""
+"""Runtime: packed weight container, decode state and the CUDA kernel layer."""
+from .history import TokenHistory
+from .kvcache import QuantizedKVCache
 from .store import PackedModelStore, PackedWeight
 
-__all__ = ["PackedModelStore", "PackedWeight"]
+__all__ = ["PackedModelStore", "PackedWeight", "QuantizedKVCache", "TokenHistory"]

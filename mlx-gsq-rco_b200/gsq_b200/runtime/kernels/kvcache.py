@@ -1,0 +1,91 @@
+"""Quantised key/value cache: writing, and reading back (csrc/kvcache.cu).
+
+Extends the reference, which keeps an fp16 cache.  The format is in
+``include/gsq_model.h`` (``gsq_kv_append``) and ``runtime/kvcache.py``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ... import _lib
+
+Strides = ctypes.c_int64 * 3
+
+
+def check_start(start: torch.Tensor, batch: int, device) -> int:
+    """The stride of ``start``: int32, one position per sequence or one for all."""
+    if start.dtype != torch.int32:
+        raise TypeError(f"start must be int32, got {start.dtype}")
+    if start.device != device:
+        raise RuntimeError("tensors on different devices")
+    if start.dim() != 1 or start.shape[0] not in (1, batch):
+        raise ValueError(f"start must hold 1 or {batch} positions")
+    return 0 if start.shape[0] == 1 else start.stride(0)
+
+
+def check_counts(counts: torch.Tensor | None, batch: int, device) -> int | None:
+    """The address of ``counts``: int32, one per sequence; None without it."""
+    if counts is None:
+        return None
+    if counts.dtype != torch.int32:
+        raise TypeError(f"counts must be int32, got {counts.dtype}")
+    if counts.device != device:
+        raise RuntimeError("tensors on different devices")
+    if counts.shape != (batch,) or not counts.is_contiguous():
+        raise ValueError(f"counts must hold {batch} contiguous values")
+    return counts.data_ptr()
+
+
+def kv_append(cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+              counts: torch.Tensor | None = None) -> None:
+    """Quantises the new keys and values ``k``, ``v`` [batch, tokens, heads,
+    dim] (fp32, fp16 or bf16; the last dimension contiguous, any other
+    strides) into ``cache`` at positions ``start[b]``, ``start[b] + 1``, ...
+
+    ``start``: int32 on the device, one position per sequence or one for all;
+    ``counts``: int32, sequence b has only ``counts[b]`` new tokens and the
+    rest of its rows is padding.  A position outside the cache is not written
+    and shows as 3 in ``_lib.device_status``."""
+    if k.shape != v.shape or k.dim() != 4 or k.shape[0] != cache.batch or k.shape[2:] != (cache.heads, cache.dim):
+        raise ValueError(f"expected k and v [{cache.batch}, tokens, {cache.heads}, {cache.dim}], "
+                         f"got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype not in _lib.DTYPE_CODES or v.dtype != k.dtype:
+        raise TypeError(f"unsupported key/value dtypes {k.dtype}, {v.dtype}")
+    dev = cache.device
+    if k.device != dev or v.device != dev:
+        raise RuntimeError("tensors on different devices")
+    stride = check_start(start, cache.batch, dev)
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
+    kc, vc, ks, vs = cache.pointers
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().gsq_kv_append(
+            k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[k.dtype], cache.batch, k.shape[1], cache.heads, cache.dim,
+            Strides(*k.stride()[:3]), Strides(*v.stride()[:3]), start.data_ptr(), stride,
+            check_counts(counts, cache.batch, dev), cache.fmt, kc, vc, ks, vs, cache.length, _lib.stream_ptr(dev)))
+
+
+def kv_read(cache, start: torch.Tensor, tokens: int, *, counts: torch.Tensor | None = None,
+            dtype: torch.dtype = torch.float16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Reads positions ``start[b]`` .. ``start[b] + tokens - 1`` of every
+    sequence back as (k, v) [batch, tokens, heads, dim] of ``dtype``: code *
+    scale in fp32, rounded once.  Padding (``counts``) and positions outside
+    the cache read as zeros."""
+    if dtype not in _lib.DTYPE_CODES:
+        raise TypeError(f"unsupported output dtype {dtype}")
+    if tokens < 0:
+        raise ValueError("negative token count")
+    dev = cache.device
+    stride = check_start(start, cache.batch, dev)
+    shape = (cache.batch, tokens, cache.heads, cache.dim)
+    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.load().gsq_kv_read(
+            cache.fmt, *cache.pointers, cache.batch, cache.heads, cache.length, cache.dim, start.data_ptr(), stride,
+            check_counts(counts, cache.batch, dev), tokens, k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[dtype],
+            _lib.stream_ptr(dev)))
+    return k, v
