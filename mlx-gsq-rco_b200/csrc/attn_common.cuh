@@ -1,0 +1,144 @@
+// What the kernels of attention over the quantised cache share: arguments,
+// the sequences' lengths and the order of their work, dequantisation.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "gsq_common.cuh"
+#include "gsq_kv.h"
+
+namespace gsq {
+
+struct AttnArgs {
+  const void* q;
+  int64_t qb, qn, qh;  // strides in elements (sequence, token, head)
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  int batch, n, heads, kv, group, dim;
+  int64_t cap;
+  const int32_t* start;
+  int64_t start_stride;
+  const int32_t* counts;
+  const int32_t* tree;
+  int64_t tree_stride;
+  int words;  // of a tree's row
+  const float* gate;
+  int64_t gb, gn, gh;
+  float scale;
+  void* out;
+  // Work of the position-split kernels: tiles of the sequences' positions in the order
+  // (sequence, head, row block, tile), an equal run of them to each CTA.
+  int ctas, rows8;      // rows8: rows of a partial result
+  float *part, *stat;   // [2 * ctas][rows8][dim], [2 * ctas][rows8][2] (max in base 2, sum)
+};
+
+// Cached positions and new tokens of sequence b.
+struct SeqSpan {
+  int64_t base;  // position of the first new token
+  int count;     // new tokens (0: all rows are padding)
+  int64_t len;   // positions that any of them may see, from 0
+};
+
+__device__ __forceinline__ SeqSpan seq_span(const AttnArgs& a, int b) {
+  SeqSpan s;
+  s.base = a.start[(int64_t)b * a.start_stride];
+  s.count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
+  s.len = s.count > 0 ? min(max(s.base + s.count, (int64_t)0), a.cap) : 0;
+  return s;
+}
+
+// A unit of work (sequence, key/value head) is cut into tiles of TILE positions; the tiles of all units form one
+// list, sequence by sequence, and CTA c of G takes tiles [c T / G, (c + 1) T / G), where G is at most T: no CTA
+// below G is without a tile, so the parts of a unit are those of consecutive CTAs.  Every warp finds its place by
+// itself: 32 sequences at a time, one per lane.
+template <int TILE>
+struct TileList {
+  __device__ static int of_seq(const AttnArgs& a, int b) {
+    return b < a.batch ? (int)((seq_span(a, b).len + TILE - 1) / TILE) : 0;
+  }
+  __device__ static int total(const AttnArgs& a) {
+    int s = 0;
+    for (int b = threadIdx.x & 31; b < a.batch; b += 32) s += of_seq(a, b);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s * a.kv;
+  }
+  // Tiles of all sequences before sequence b.
+  __device__ static int before(const AttnArgs& a, int b) {
+    int s = 0;
+    for (int i = threadIdx.x & 31; i < b; i += 32) s += of_seq(a, i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s * a.kv;
+  }
+  // The sequence that holds tile t (t < total), and t's place in it.
+  __device__ static int locate(const AttnArgs& a, int t, int* in_seq) {
+    const int lane = threadIdx.x & 31;
+    int done = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      const int mine = of_seq(a, b0 + lane) * a.kv;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, t < done + sum);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        *in_seq = t - done - __shfl_sync(0xffffffffu, sum - mine, l);
+        return b0 + l;
+      }
+      done += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    *in_seq = 0;
+    return a.batch;
+  }
+  __device__ static int first_of(int c, int total, int ctas) { return (int)((int64_t)c * total / ctas); }
+  __device__ static int cta_of(int t, int total, int ctas) { return (int)((((int64_t)t + 1) * ctas - 1) / total); }
+};
+
+// Four codes as two half2, in order (c0, c1), (c2, c3).  int8: 0x64cc is 1024 + cc, so a code biased by 128 minus
+// 1152 is the code.  e4m3 is a subset of fp16.  Both exact.
+template <int FMT>
+__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == KV_INT8) {
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Output row r (token r / group, head r % group) of a unit, values d, d + 1.
+template <typename T>
+__device__ __forceinline__ void store_row2(const AttnArgs& a, int b, int kh, int r, int d, float x, float y) {
+  const int i = r / a.group, h = kh * a.group + r % a.group;
+  if (a.gate) {
+    const float* g = a.gate + b * a.gb + i * a.gn + h * a.gh + d;
+    x /= 1.f + __expf(-g[0]);
+    y /= 1.f + __expf(-g[1]);
+  }
+  T* o = static_cast<T*>(a.out) + (((int64_t)b * a.n + i) * a.heads + h) * a.dim + d;
+  if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(o) = __floats2half2_rn(x, y);
+  else *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x, y);
+}
+
+}  // namespace gsq

@@ -1,0 +1,510 @@
+// Attention over the quantised cache for few rows per key/value head (n *
+// group <= 16: single tokens, small trees).
+//
+// Bound: HBM bytes of the cache, each read once.  At 6.5 TB/s an SM receives
+// about 23 codes a cycle, so what is done per code has to stay small:
+//   - codes go to fp16 exactly (2 to 3 operations per pair) and their scales,
+//     one per position, are applied to the 16 x 8 tile of scores (keys) and
+//     weights (values), not to the codes;
+//   - both products run on mma.m16n8k16 with the codes as the 16-row operand
+//     (S^T = K Q^T, O^T = V^T P^T), so 8 query rows fill the tile that a
+//     token's 1 to 8 heads need, where the query as the 16-row operand (or
+//     128 rows of tcgen05) would be mostly padding;
+//   - each warp runs its own softmax over its own 16 positions of a tile of
+//     128, so no barrier or exchange between warps interrupts the stream; the
+//     eight are joined once per unit of work.
+// Every warp copies its own 16 rows of K and V through a private ring
+// (cp.async, positions past the end filled with zeros), with 16-byte units
+// exchanged by the row so that all shared loads are 16 bytes and free of
+// conflicts.  The long axis is split evenly over the CTAs (TileList); a unit
+// that falls into several CTAs is joined by a second launch.
+//
+// Weights p are rounded to fp16 (2^-11 each) for the second product; the sum
+// of weights is of the unrounded ones, in fp32.  The values' scales differ by
+// position, so the rounded weight is 2^15 p vs / 2^ref with a reference per
+// row that follows s + log2(vs): no weight that matters leaves fp16's normal
+// range, whatever the scales.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace gsq {
+
+constexpr int AT_WARPS = 8;
+constexpr int AT_TILE = 16 * AT_WARPS;
+
+template <int D, int NT>
+struct AtGeom {
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int STAGE = 2 * 16 * D + 2 * 16 * 4;  // K, V, scales of 16 positions
+  static constexpr int STAGES = D == 256 ? 3 : 6;
+  static constexpr int BUF = ROWS * D * 4;                // one warp's sums
+  static constexpr int BUFS = NT == 1 ? 2 : 1;
+  static constexpr int RING = AT_WARPS * STAGES * STAGE;
+  static constexpr int STAT = AT_WARPS * ROWS * 2 * 4;
+  static constexpr int QFRAG = NT == 1 ? 0 : D / 16 * 32 * 8 * NT;
+  static constexpr int SMEM = RING + BUFS * BUF + STAT + QFRAG;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// 16 (or 4) bytes global -> shared; zeros where !in (the source is not read).
+__device__ __forceinline__ void cp_async16_zfill(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4_zfill(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// 16-byte unit u of position p within a warp's 16 rows: rows p and p + 1 differ in bit 2 (the keys' loads read units
+// 4c .. 4c + 3 of two neighbouring rows at a time), rows p, p + 2, p + 4, p + 6 in bits 1 and 2 (the values' loads
+// read two units of four rows).
+__device__ __forceinline__ int at_unit(int p, int u) { return u ^ ((p & 6) ^ (p & 1) << 2); }
+
+// A cursor over the tiles of the list: unit (sequence, head) and tile in it.
+struct AtCursor {
+  int b, kh, tile, tiles;
+  SeqSpan span;
+  __device__ void enter(const AttnArgs& a, int seq) {
+    b = seq;
+    span = seq_span(a, seq);
+    tiles = (int)((span.len + AT_TILE - 1) / AT_TILE);
+  }
+  __device__ void next(const AttnArgs& a) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++kh < a.kv) return;
+    kh = 0;
+    do {
+      if (b + 1 >= a.batch) return;  // past the last tile: not used
+      enter(a, b + 1);
+    } while (tiles == 0);
+  }
+};
+
+// One row's eight values of q from dimension d on, in fp32.
+template <typename T>
+__device__ __forceinline__ void load_q8(const AttnArgs& a, int b, int kh, int r, int d, float (&f)[8]) {
+  if (r < a.n * a.group) {
+    const T* p = static_cast<const T*>(a.q) + b * a.qb + (r / a.group) * a.qn + (kh * a.group + r % a.group) * a.qh + d;
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = 0.f;
+  }
+}
+
+// bf16 queries are held in fp16 times a power of two that brings the row's largest value to [2^13, 2^14): exact but
+// for values 2^27 times smaller than the largest.  Returns that power's exponent.
+__device__ __forceinline__ int q_shift(float amax) {
+  const int e = (int)(__float_as_uint(amax) >> 23 & 255);
+  return e == 0 || e == 255 ? 0 : min(13 - (e - 127), 126);
+}
+__device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+
+template <typename T, int FMT, int D, int NT>
+__global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const AttnArgs a) {
+  using G = AtGeom<D, NT>;
+  constexpr int CH = D / 64;   // 64-dimension chunks of the first product
+  constexpr int MT = D / 16;   // 16-dimension tiles of the second
+  extern __shared__ __align__(128) uint8_t smem[];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * G::STAGES * G::STAGE;
+  float* buf = reinterpret_cast<float*>(smem + G::RING);
+  float* stat = reinterpret_cast<float*>(smem + G::RING + G::BUFS * G::BUF);  // [warp][row][m, l]
+  uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::BUFS * G::BUF + G::STAT);
+
+  const int total = TileList<AT_TILE>::total(a);
+  const int ctas = min(a.ctas, total);
+  if ((int)blockIdx.x >= ctas) return;
+  const int first = TileList<AT_TILE>::first_of(blockIdx.x, total, ctas);
+  const int last = TileList<AT_TILE>::first_of(blockIdx.x + 1, total, ctas);
+  AtCursor get, use;
+  {
+    int in_seq;
+    get.enter(a, TileList<AT_TILE>::locate(a, first, &in_seq));
+    get.kh = in_seq / get.tiles;
+    get.tile = in_seq % get.tiles;
+    use = get;
+  }
+  const int rows = a.n * a.group;
+
+  int fetched = first;
+  auto fetch = [&]() {
+    if (fetched < last) {
+      uint8_t* st = ring + (fetched - first) % G::STAGES * G::STAGE;
+      const int64_t p0 = (int64_t)get.tile * AT_TILE + warp * 16;
+      const int64_t row0 = ((int64_t)get.b * a.kv + get.kh) * a.cap + p0;
+      const int64_t left = get.span.len - p0;  // positions of this warp that exist
+      constexpr int U = D / 16;                // units of a row
+#pragma unroll
+      for (int i = 0; i < 16 * U / 32; i++) {
+        const int x = i * 32 + lane, p = x / U, u = x % U;
+        const bool in = p < left;
+        const int64_t src = (row0 + (in ? p : 0)) * D + u * 16;
+        const int dst = p * D + at_unit(p, u) * 16;
+        cp_async16_zfill(st + dst, a.kc + (in ? src : 0), in);
+        cp_async16_zfill(st + 16 * D + dst, a.vc + (in ? src : 0), in);
+      }
+      const int p = lane & 15;
+      const bool in = p < left;
+      cp_async4_zfill(st + 32 * D + lane * 4, (lane < 16 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
+      get.next(a);
+    }
+    fetched++;
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < G::STAGES - 1; i++) fetch();
+
+  uint32_t qr[NT == 1 ? MT : 1][2];
+  float factor[NT][2];  // of the scores of rows 8x + 2t, 8x + 2t + 1, to base 2
+  int lim[NT][2];       // tree: prefix ends; causal: positions the row sees (relative to the prefix end)
+  float o[MT][NT][4], m[NT][2], l[NT][2];
+
+  for (int tile = first; tile < last;) {
+    // ---- a unit's run of tiles ----
+    const int b = use.b, kh = use.kh;
+    const SeqSpan span = use.span;
+    const bool whole = use.tile == 0 && tile + use.tiles <= last;
+    const int slot = 2 * blockIdx.x + (tile == first ? 0 : 1);
+    const int end = min(last, tile + use.tiles - use.tile);
+    if constexpr (NT > 1) __syncthreads();  // qfrag is free
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+      float amax = 0.f;
+      float qv[CH][16];
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        float lo[8], hi[8];
+        load_q8<T>(a, b, kh, 8 * x + g, 64 * c + 16 * t, lo);
+        load_q8<T>(a, b, kh, 8 * x + g, 64 * c + 16 * t + 8, hi);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          qv[c][e] = lo[e];
+          qv[c][8 + e] = hi[e];
+          amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+        }
+      }
+      int shift = 0;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        shift = q_shift(amax);
+        const float up = exp2_int(shift);
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) qv[c][e] *= up;
+      }
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const __half2 h0 = __floats2half2_rn(qv[c][4 * j], qv[c][4 * j + 1]);
+          const __half2 h1 = __floats2half2_rn(qv[c][4 * j + 2], qv[c][4 * j + 3]);
+          const uint32_t b0 = *reinterpret_cast<const uint32_t*>(&h0), b1 = *reinterpret_cast<const uint32_t*>(&h1);
+          if constexpr (NT == 1) {
+            qr[4 * c + j][0] = b0;
+            qr[4 * c + j][1] = b1;
+          } else if (warp == x) {
+            qfrag[((4 * c + j) * NT + x) * 32 + lane] = make_uint2(b0, b1);
+          }
+        }
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const int r = 8 * x + 2 * t + c;  // this lane's columns of the score tile; their shift is held by lanes 4r'
+        factor[x][c] = a.scale * 1.4426950408889634f * exp2_int(-__shfl_sync(0xffffffffu, shift, 4 * (2 * t + c)));
+        lim[x][c] = r / a.group;
+        m[x][c] = -INFINITY;
+        l[x][c] = 0.f;
+      }
+    }
+    if constexpr (NT > 1) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < MT; j++)
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[j][x][e] = 0.f;
+
+    for (; tile < end; tile++) {
+      __syncwarp();  // every lane has read the stage that is filled next
+      fetch();
+      cp_async_wait<G::STAGES - 1>();
+      __syncwarp();
+      const uint8_t* st = ring + (tile - first) % G::STAGES * G::STAGE;
+      const int64_t p0 = (int64_t)use.tile * AT_TILE + warp * 16;
+      use.next(a);
+      if (p0 >= span.len) continue;
+      const float* sc = reinterpret_cast<const float*>(st + 32 * D);
+
+      float s[NT][4];
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[x][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(st + g * D + at_unit(g, 4 * c + t) * 16);
+        const uint4 kb = *reinterpret_cast<const uint4*>(st + (g + 8) * D + at_unit(g + 8, 4 * c + t) * 16);
+        const uint32_t* wa = reinterpret_cast<const uint32_t*>(&ka);
+        const uint32_t* wb = reinterpret_cast<const uint32_t*>(&kb);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t a0, a1, a2, a3;
+          codes_to_half2<FMT>(wa[j], a0, a2);
+          codes_to_half2<FMT>(wb[j], a1, a3);
+#pragma unroll
+          for (int x = 0; x < NT; x++) {
+            if constexpr (NT == 1) {
+              mma_f16(s[x], a0, a1, a2, a3, qr[4 * c + j][0], qr[4 * c + j][1]);
+            } else {
+              const uint2 q2 = qfrag[((4 * c + j) * NT + x) * 32 + lane];
+              mma_f16(s[x], a0, a1, a2, a3, q2.x, q2.y);
+            }
+          }
+        }
+      }
+      // scores to base 2; s[x][e]: position p0 + g + 8 (e / 2), row 8x + 2t + e % 2
+      const float ks0 = sc[g], ks1 = sc[g + 8];
+      const float lv0 = log2_approx(fmaxf(sc[16 + g], 1.4e-45f)) , lv1 = log2_approx(fmaxf(sc[24 + g], 1.4e-45f));
+      const float nan0 = sc[16 + g] - sc[16 + g], nan1 = sc[24 + g] - sc[24 + g];  // NaN scales stay NaN past fmaxf
+      const bool edge = p0 + 16 > span.base || p0 + 16 > span.len;  // warp-uniform: some row may not see all of these
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int x = 0; x < NT; x++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[x][e] *= (e < 2 ? ks0 : ks1) * factor[x][e & 1];
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int64_t p = p0 + g + (e < 2 ? 0 : 8);
+            const int64_t off = p - span.base;  // index among the new tokens
+            bool see = p < span.len;
+            if (off >= 0 && see) {
+              const int i = lim[x][e & 1];
+              see = i < span.count;
+              if (!a.tree) see = see && off <= i;
+              else if (see)
+                see = (uint32_t)a.tree[b * a.tree_stride + (int64_t)i * a.words + (off >> 5)] >> (off & 31) & 1;
+            }
+            if (!see) s[x][e] = -INFINITY;
+          }
+        }
+        float lo[2];
+        // the reference of each row: the largest of s + log2(vs) (and s - 100, so that the sum of weights stays finite)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float r = fmaxf(fmaxf(s[x][c] + fmaxf(lv0, -100.f), s[x][2 + c] + fmaxf(lv1, -100.f)), m[x][c]);
+          r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 4));
+          r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 8));
+          r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 16));
+          lo[c] = r;
+        }
+        const bool grew = lo[0] > m[x][0] || lo[1] > m[x][1];
+        if (__any_sync(0xffffffffu, grew)) {
+          const float f0 = m[x][0] == -INFINITY ? 0.f : exp2_approx(m[x][0] - lo[0]);
+          const float f1 = m[x][1] == -INFINITY ? 0.f : exp2_approx(m[x][1] - lo[1]);
+          m[x][0] = lo[0];
+          m[x][1] = lo[1];
+          l[x][0] *= f0;
+          l[x][1] *= f1;
+#pragma unroll
+          for (int j = 0; j < MT; j++) {
+            o[j][x][0] *= f0;
+            o[j][x][1] *= f1;
+            o[j][x][2] *= f0;
+            o[j][x][3] *= f1;
+          }
+        }
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float ref = m[x][e & 1] == -INFINITY ? 0.f : m[x][e & 1];
+          const float d = s[x][e] - ref;  // -inf where hidden
+          l[x][e & 1] += exp2_approx(d);
+          w[e] = s[x][e] == -INFINITY ? 0.f : exp2_approx(d + (e < 2 ? lv0 : lv1) + 15.f) + (e < 2 ? nan0 : nan1);
+        }
+        const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+        pb[x][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
+        pb[x][1] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h1));
+      }
+      // O^T += V^T P^T: rows of tile 8h + j are dimensions 128h + 16g + 2j (registers 0, 1) and + 1 (2, 3)
+#pragma unroll
+      for (int h = 0; h < D / 128; h++) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int p = 2 * t + (i & 1) + (i >> 1) * 8;
+          v[i] = *reinterpret_cast<const uint4*>(st + 16 * D + p * D + at_unit(p, 8 * h + g) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const uint32_t w0 = reinterpret_cast<const uint32_t*>(&v[0])[i], w1 = reinterpret_cast<const uint32_t*>(&v[1])[i];
+          const uint32_t w2 = reinterpret_cast<const uint32_t*>(&v[2])[i], w3 = reinterpret_cast<const uint32_t*>(&v[3])[i];
+          uint32_t a0, a1, a2, a3;
+          codes_to_half2<FMT>(__byte_perm(w0, w1, 0x5140), a0, a1);
+          codes_to_half2<FMT>(__byte_perm(w2, w3, 0x5140), a2, a3);
+#pragma unroll
+          for (int x = 0; x < NT; x++) mma_f16(o[8 * h + 2 * i][x], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+          codes_to_half2<FMT>(__byte_perm(w0, w1, 0x7362), a0, a1);
+          codes_to_half2<FMT>(__byte_perm(w2, w3, 0x7362), a2, a3);
+#pragma unroll
+          for (int x = 0; x < NT; x++) mma_f16(o[8 * h + 2 * i + 1][x], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+        }
+      }
+    }
+
+    // ---- join the warps: reference and sum of every row, then the sums, two warps (or one) at a time ----
+#pragma unroll
+    for (int x = 0; x < NT; x++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+#pragma unroll
+        for (int i = 4; i < 32; i <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], i);
+        if (g == 0) {
+          stat[(warp * G::ROWS + 8 * x + 2 * t + c) * 2] = m[x][c];
+          stat[(warp * G::ROWS + 8 * x + 2 * t + c) * 2 + 1] = l[x][c];
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < NT; x++) {
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        float top = -INFINITY;
+        for (int w = 0; w < AT_WARPS; w++) top = fmaxf(top, stat[(w * G::ROWS + 8 * x + 2 * t + c) * 2]);
+        f[c] = m[x][c] == -INFINITY ? 0.f : exp2_approx(m[x][c] - top);
+      }
+#pragma unroll
+      for (int j = 0; j < MT; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[j][x][e] = m[x][e & 1] == -INFINITY ? o[j][x][e] : o[j][x][e] * f[e & 1];
+    }
+#pragma unroll 1
+    for (int round = 0; round < AT_WARPS / G::BUFS; round++) {
+      if (warp / G::BUFS == round) {
+        float* mine = buf + warp % G::BUFS * (G::BUF / 4) + lane;
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+          for (int x = 0; x < NT; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              float* p = mine + ((j * NT + x) * 4 + e) * 32;
+              *p = round == 0 ? o[j][x][e] : *p + o[j][x][e];
+            }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < rows * (D / 2); i += 32 * AT_WARPS) {
+      const int r = i / (D / 2), d = i % (D / 2) * 2;
+      float top = -INFINITY, sum = 0.f;
+      for (int w = 0; w < AT_WARPS; w++) top = fmaxf(top, stat[(w * G::ROWS + r) * 2]);
+      for (int w = 0; w < AT_WARPS; w++) {
+        const float mw = stat[(w * G::ROWS + r) * 2], lw = stat[(w * G::ROWS + r) * 2 + 1];
+        sum += mw == -INFINITY ? lw : lw * exp2_approx(mw - top);
+      }
+      // dimension d of row r in the fragments' layout
+      const int tt = r % 8 / 2, cc = r % 2, xx = r / 8, hh = d / 128, gg = d / 16 % 8, jj = d % 16 / 2;
+      const float* p = buf + (((8 * hh + jj) * NT + xx) * 4 + cc) * 32 + gg * 4 + tt;
+      float v0 = p[0], v1 = p[64];
+      if constexpr (G::BUFS == 2) {
+        v0 += p[G::BUF / 4];
+        v1 += p[G::BUF / 4 + 64];
+      }
+      v0 *= 0x1p-15f;
+      v1 *= 0x1p-15f;
+      if (whole) {
+        const bool none = sum == 0.f || r / a.group >= span.count;
+        const float inv = none ? 0.f : 1.f / sum;
+        store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * inv, none ? 0.f : v1 * inv);
+      } else {
+        *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) = make_float2(v0, v1);
+        if (d == 0)
+          *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * G::ROWS + r) * 2) = make_float2(top, sum);
+      }
+    }
+    __syncthreads();  // buf and stat are free
+  }
+}
+
+// Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the units
+// that have no position.  One CTA per (unit, row): D / 4 threads across, the rest over the parts.
+template <typename T, int D, int TILE>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+  constexpr int ACROSS = D / 4, DOWN = 256 / ACROSS;
+  __shared__ float4 acc[DOWN][ACROSS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rows = a.n * a.group;
+  const int u = blockIdx.x / rows, r = blockIdx.x % rows, b = u / a.kv, kh = u % a.kv;
+  const SeqSpan span = seq_span(a, b);
+  const int tiles = (int)((span.len + TILE - 1) / TILE);
+  const int x = threadIdx.x % ACROSS, y = threadIdx.x / ACROSS;
+  if (tiles == 0) {
+    if (y == 0) {
+      store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
+      store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
+    }
+    return;
+  }
+  const int total = TileList<TILE>::total(a);
+  const int t0 = TileList<TILE>::before(a, b) + kh * tiles;
+  const int ctas = min(a.ctas, total);
+  const int c0 = TileList<TILE>::cta_of(t0, total, ctas), c1 = TileList<TILE>::cta_of(t0 + tiles - 1, total, ctas);
+  if (c0 == c1) return;
+  // only the first CTA can have begun another unit before this one
+  const int s0 = 2 * c0 + (TileList<TILE>::first_of(c0, total, ctas) == t0 ? 0 : 1);
+  auto slot = [&](int c) { return c == c0 ? s0 : 2 * c; };
+  float top = -INFINITY, sum = 0.f;
+  for (int c = c0; c <= c1; c++) top = fmaxf(top, a.stat[((int64_t)slot(c) * a.rows8 + r) * 2]);
+  for (int c = c0; c <= c1; c++) {
+    const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)slot(c) * a.rows8 + r) * 2);
+    sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = c0 + y; c <= c1; c += DOWN) {
+    const int64_t at = (int64_t)slot(c) * a.rows8 + r;
+    const float mc = a.stat[at * 2], f = mc == -INFINITY ? 1.f : exp2_approx(mc - top);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + 4 * x);
+    o.x = fmaf(v.x, f, o.x);
+    o.y = fmaf(v.y, f, o.y);
+    o.z = fmaf(v.z, f, o.z);
+    o.w = fmaf(v.w, f, o.w);
+  }
+  acc[y][x] = o;
+  __syncthreads();
+  if (y == 0) {
+    for (int i = 1; i < DOWN; i++) {
+      const float4 v = acc[i][x];
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    const bool none = sum == 0.f || r / a.group >= span.count;
+    const float inv = none ? 0.f : 1.f / sum;
+    store_row2<T>(a, b, kh, r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
+    store_row2<T>(a, b, kh, r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
+  }
+}
+
+}  // namespace gsq

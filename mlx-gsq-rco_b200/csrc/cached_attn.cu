@@ -1,35 +1,16 @@
 // Attention of the newest tokens of each sequence over the quantised cache
 // (gsq_cached_attention): one warp per query row, an online softmax over the
 // positions the row sees.
-#include <cuda_fp8.h>
-
+#include <atomic>
 #include <cstdio>
 
-#include "gsq_common.cuh"
+#include "attn_token.cuh"
 #include "gsq_host.h"
-#include "gsq_kv.h"
 #include "../../include/gsq_model.h"
 
 using namespace gsq;
 
 namespace {
-
-struct AttnArgs {
-  const void* q;
-  int64_t qb, qn, qh;  // strides in elements (sequence, token, head)
-  const uint8_t *kc, *vc;
-  const float *ks, *vs;
-  int64_t batch, n, heads, kv, cap;
-  const int32_t* start;
-  int64_t start_stride;
-  const int32_t* counts;
-  const int32_t* tree;
-  int64_t tree_stride;
-  const float* gate;
-  int64_t gb, gn, gh;
-  float scale;
-  void* out;
-};
 
 template <int FMT>
 __device__ __forceinline__ float code_value(uint8_t c) {
@@ -44,9 +25,9 @@ __global__ void __launch_bounds__(128) attn_simple_kernel(const AttnArgs a) {
   pdl_wait();
   const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (r >= a.batch * a.n * a.heads) return;
-  const int64_t h = r % a.heads, i = r / a.heads % a.n, b = r / (a.heads * a.n);
-  const int64_t kh = h / (a.heads / a.kv);
+  if (r >= (int64_t)a.batch * a.n * a.heads) return;
+  const int64_t h = r % a.heads, i = r / a.heads % a.n, b = r / ((int64_t)a.heads * a.n);
+  const int64_t kh = h / a.group;
   T* out = static_cast<T*>(a.out) + r * D + lane * N;
   const int64_t base = a.start[b * a.start_stride];
   const int64_t count = a.counts ? a.counts[b] : a.n;
@@ -90,11 +71,57 @@ __global__ void __launch_bounds__(128) attn_simple_kernel(const AttnArgs a) {
 }
 
 int fail(int code, const char* msg) { return set_last_error(code, msg); }
+bool al(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 template <typename T, int FMT>
 cudaError_t simple(int64_t dim, dim3 grid, cudaStream_t st, const AttnArgs& a) {
   return dim == 256 ? launch_pdl(attn_simple_kernel<T, FMT, 256>, grid, dim3(128), 0, st, a)
                     : launch_pdl(attn_simple_kernel<T, FMT, 128>, grid, dim3(128), 0, st, a);
+}
+
+constexpr int SMS = 148;
+
+// Which kernel a call takes, over how many CTAs, and its scratch.
+struct Plan {
+  int nt;           // 8-row tiles of the token kernel (0: the simple kernel)
+  int ctas, rows8;
+  size_t workspace;
+};
+
+Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, int64_t cap) {
+  Plan p = {};
+  const int64_t rows = n * (heads / kv);
+  if (rows > 16) return p;
+  p.nt = rows <= 8 ? 1 : 2;
+  p.rows8 = 8 * p.nt;
+  const int64_t tiles = batch * kv * ((cap + AT_TILE - 1) / AT_TILE);
+  p.ctas = (int)(tiles < SMS ? tiles : SMS);
+  p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float);
+  return p;
+}
+
+template <typename T, int FMT, int D, int NT>
+cudaError_t token_launch(cudaStream_t st, const AttnArgs& a) {
+  auto kernel = attn_token_kernel<T, FMT, D, NT>;
+  constexpr int smem = AtGeom<D, NT>::SMEM;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  e = launch_pdl(kernel, dim3((unsigned)a.ctas), dim3(32 * AT_WARPS), smem, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(attn_join_kernel<T, D, AT_TILE>, dim3((unsigned)(a.batch * a.kv * a.n * a.group)), dim3(256), 0, st, a);
+}
+
+template <typename T, int FMT>
+cudaError_t token(int nt, cudaStream_t st, const AttnArgs& a) {
+  if (a.dim == 256) return nt == 1 ? token_launch<T, FMT, 256, 1>(st, a) : token_launch<T, FMT, 256, 2>(st, a);
+  return nt == 1 ? token_launch<T, FMT, 128, 1>(st, a) : token_launch<T, FMT, 128, 2>(st, a);
 }
 
 }  // namespace
@@ -103,7 +130,8 @@ extern "C" {
 
 size_t gsq_cached_attention_workspace_size(int64_t batch, int64_t n, int64_t heads, int64_t kv_heads, int64_t dim,
                                            int64_t cap) {
-  return 0;
+  if (batch <= 0 || n <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || cap <= 0) return 0;
+  return plan_of(batch, n, heads, kv_heads, dim, cap).workspace;
 }
 
 int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int64_t batch, int64_t n, int64_t heads,
@@ -121,6 +149,12 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   if (batch == 0 || n == 0) return GSQ_OK;
   if (!q || !q_strides || !start || !out || (gate && !gate_strides))
     return fail(GSQ_ERR_ARG, "gsq_cached_attention: null pointer");
+  if (batch * kv_heads * ((cap + AT_TILE - 1) / AT_TILE) > INT32_MAX || batch * n * heads > INT32_MAX)
+    return fail(GSQ_ERR_SIZE, "gsq_cached_attention: too much work for one call");
+  for (int i = 0; i < 3; i++)
+    if (q_strides[i] % 8) return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: rows of q not 16-byte aligned");
+  if (!al(q, 16) || !al(out, 16) || !al(gate, 4))
+    return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: q or out not 16-byte aligned, or gate not aligned");
   AttnArgs a = {};
   a.q = q;
   a.qb = q_strides[0];
@@ -130,10 +164,13 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   a.vc = static_cast<const uint8_t*>(v_codes);
   a.ks = k_scale;
   a.vs = v_scale;
-  a.batch = batch;
-  a.n = n;
-  a.heads = heads;
-  a.kv = kv_heads;
+  a.batch = (int)batch;
+  a.n = (int)n;
+  a.heads = (int)heads;
+  a.kv = (int)kv_heads;
+  a.group = (int)(heads / kv_heads);
+  a.dim = (int)dim;
+  a.words = (int)((n + 31) / 32);
   a.cap = cap;
   a.start = start;
   a.start_stride = start_stride;
@@ -149,9 +186,24 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   a.scale = scale;
   a.out = out;
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)((batch * n * heads + 3) / 4));
-  cudaError_t e = dtype == DT_F16 ? (fmt == KV_INT8 ? simple<__half, KV_INT8>(dim, grid, st, a) : simple<__half, KV_FP8>(dim, grid, st, a))
-                                  : (fmt == KV_INT8 ? simple<__nv_bfloat16, KV_INT8>(dim, grid, st, a) : simple<__nv_bfloat16, KV_FP8>(dim, grid, st, a));
+  const Plan plan = plan_of(batch, n, heads, kv_heads, dim, cap);
+  if (plan.workspace && (!workspace || workspace_bytes < plan.workspace))
+    return fail(GSQ_ERR_WORKSPACE, "gsq_cached_attention: workspace missing or too small");
+  if (!al(workspace, 256)) return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: workspace not 256-byte aligned");
+  a.ctas = plan.ctas;
+  a.rows8 = plan.rows8;
+  a.part = static_cast<float*>(workspace);
+  a.stat = a.part + (size_t)2 * a.ctas * a.rows8 * dim;
+  cudaError_t e;
+  if (plan.nt) {
+    e = dtype == DT_F16 ? (fmt == KV_INT8 ? token<__half, KV_INT8>(plan.nt, st, a) : token<__half, KV_FP8>(plan.nt, st, a))
+                        : (fmt == KV_INT8 ? token<__nv_bfloat16, KV_INT8>(plan.nt, st, a)
+                                          : token<__nv_bfloat16, KV_FP8>(plan.nt, st, a));
+  } else {
+    const dim3 grid((unsigned)((batch * n * heads + 3) / 4));
+    e = dtype == DT_F16 ? (fmt == KV_INT8 ? simple<__half, KV_INT8>(dim, grid, st, a) : simple<__half, KV_FP8>(dim, grid, st, a))
+                        : (fmt == KV_INT8 ? simple<__nv_bfloat16, KV_INT8>(dim, grid, st, a) : simple<__nv_bfloat16, KV_FP8>(dim, grid, st, a));
+  }
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess) return GSQ_OK;
   char buf[256];
