@@ -26,9 +26,8 @@ struct AttnArgs {
   int64_t gb, gn, gh;
   float scale;
   void* out;
-  // Work of the position-split kernels: tiles of the sequences' positions in the order
-  // (sequence, head, row block, tile), an equal run of them to each CTA.
-  int ctas, rows8;      // rows8: rows of a partial result
+  int ctas, rows8;      // CTAs of the split, rows of a partial result
+  int* err;             // device error word
   float *part, *stat;   // [2 * ctas][rows8][dim], [2 * ctas][rows8][2] (max in base 2, sum)
 };
 
@@ -47,36 +46,42 @@ __device__ __forceinline__ SeqSpan seq_span(const AttnArgs& a, int b) {
   return s;
 }
 
-// A unit of work (sequence, key/value head) is cut into tiles of TILE positions; the tiles of all units form one
-// list, sequence by sequence, and CTA c of G takes tiles [c T / G, (c + 1) T / G), where G is at most T: no CTA
-// below G is without a tile, so the parts of a unit are those of consecutive CTAs.  Every warp finds its place by
-// itself: 32 sequences at a time, one per lane.
-template <int TILE>
+// The work is a list of tiles of positions, ordered by sequence, key/value head, block of rows (one, where all rows
+// of a head are taken together) and position; a unit is the tiles of one (sequence, head, block). CTA c of G takes
+// tiles [c T / G, (c + 1) T / G), where G is at most T: no CTA below G is without a tile, so the parts of a unit are
+// those of consecutive CTAs. Every warp finds its place by itself, 32 sequences at a time, one per lane.
+struct Place {
+  int b, kh, mb;    // unit
+  int tile, tiles;  // tile in it, and its tiles
+  SeqSpan span;
+};
+
+// Shape: blocks(a) row blocks of ROWS rows each; tiles(a, span, mb).
+template <typename Shape>
 struct TileList {
-  __device__ static int of_seq(const AttnArgs& a, int b) {
-    return b < a.batch ? (int)((seq_span(a, b).len + TILE - 1) / TILE) : 0;
+  // Tiles of one head of sequence b.
+  __device__ static int of_head(const AttnArgs& a, int b) {
+    if (b >= a.batch) return 0;
+    const SeqSpan s = seq_span(a, b);
+    int sum = 0;
+    for (int mb = 0; mb < Shape::blocks(a); mb++) sum += Shape::tiles(a, s, mb);
+    return sum;
   }
   __device__ static int total(const AttnArgs& a) {
     int s = 0;
-    for (int b = threadIdx.x & 31; b < a.batch; b += 32) s += of_seq(a, b);
+    const int blocks = Shape::blocks(a), pairs = a.batch * blocks;
+    for (int i = threadIdx.x & 31; i < pairs; i += 32) s += Shape::tiles(a, seq_span(a, i / blocks), i % blocks);
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s * a.kv;
   }
-  // Tiles of all sequences before sequence b.
-  __device__ static int before(const AttnArgs& a, int b) {
-    int s = 0;
-    for (int i = threadIdx.x & 31; i < b; i += 32) s += of_seq(a, i);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s * a.kv;
-  }
-  // The sequence that holds tile t (t < total), and t's place in it.
-  __device__ static int locate(const AttnArgs& a, int t, int* in_seq) {
+  // Where tile t (below the total) lies; every lane of the warp calls it.
+  __device__ static Place locate(const AttnArgs& a, int t) {
     const int lane = threadIdx.x & 31;
+    Place p = {};
     int done = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      const int mine = of_seq(a, b0 + lane) * a.kv;
+      const int mine = of_head(a, b0 + lane) * a.kv;
       int sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -86,13 +91,31 @@ struct TileList {
       const unsigned past = __ballot_sync(0xffffffffu, t < done + sum);
       if (past) {
         const int l = __ffs(past) - 1;
-        *in_seq = t - done - __shfl_sync(0xffffffffu, sum - mine, l);
-        return b0 + l;
+        const int at = t - done - __shfl_sync(0xffffffffu, sum - mine, l);
+        const int head = __shfl_sync(0xffffffffu, mine, l) / a.kv;
+        p.b = b0 + l;
+        p.kh = at / head;
+        p.tile = at % head;
+        break;
       }
       done += __shfl_sync(0xffffffffu, sum, 31);
     }
-    *in_seq = 0;
-    return a.batch;
+    p.span = seq_span(a, p.b);
+    for (; p.tile >= (p.tiles = Shape::tiles(a, p.span, p.mb)); p.mb++) p.tile -= p.tiles;
+    return p;
+  }
+  // The first tile of the unit after p's; there must be one.
+  __device__ static void next_unit(const AttnArgs& a, Place& p) {
+    p.tile = 0;
+    do {
+      if (++p.mb == Shape::blocks(a)) {
+        p.mb = 0;
+        if (++p.kh == a.kv) {
+          p.kh = 0;
+          p.span = seq_span(a, ++p.b);
+        }
+      }
+    } while ((p.tiles = Shape::tiles(a, p.span, p.mb)) == 0);
   }
   __device__ static int first_of(int c, int total, int ctas) { return (int)((int64_t)c * total / ctas); }
   __device__ static int cta_of(int t, int total, int ctas) { return (int)((((int64_t)t + 1) * ctas - 1) / total); }
@@ -139,6 +162,38 @@ __device__ __forceinline__ void store_row2(const AttnArgs& a, int b, int kh, int
   T* o = static_cast<T*>(a.out) + (((int64_t)b * a.n + i) * a.heads + h) * a.dim + d;
   if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(o) = __floats2half2_rn(x, y);
   else *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x, y);
+}
+
+// Eight values from d on.
+template <typename T>
+__device__ __forceinline__ void store_row8(const AttnArgs& a, int b, int kh, int r, int d, float (&f)[8]) {
+  const int i = r / a.group, h = kh * a.group + r % a.group;
+  if (a.gate) {
+    const float* g = a.gate + b * a.gb + i * a.gn + h * a.gh + d;
+    float w[8];
+    if (reinterpret_cast<uintptr_t>(g) % 16 == 0) {
+      const float4 x = *reinterpret_cast<const float4*>(g), y = *reinterpret_cast<const float4*>(g + 4);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) w[e] = g[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] /= 1.f + __expf(-w[e]);
+  }
+  uint4 v;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h2 = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+      u[e] = *reinterpret_cast<const uint32_t*>(&h2);
+    } else {
+      const __nv_bfloat162 h2 = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+      u[e] = *reinterpret_cast<const uint32_t*>(&h2);
+    }
+  }
+  *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (((int64_t)b * a.n + i) * a.heads + h) * a.dim + d) = v;
 }
 
 }  // namespace gsq

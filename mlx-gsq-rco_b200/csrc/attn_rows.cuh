@@ -1,0 +1,573 @@
+// Attention over the quantised cache for many rows per key/value head (n *
+// group > 16: chunks of a prompt, drafted trees), on tcgen05.
+//
+// Both products of a block of 128 rows run on the tensor core with the rows
+// as M: S = Q K^T (N = 64 positions) and O += P V (N = the head's width),
+// accumulators in TMEM.  Bound: the tensor core where the rows fill their
+// blocks (4 D operations a row and position; at D = 256 a tile of 64
+// positions takes 1024 cycles), else the bytes of the cache.  Each code is
+// read, made fp16 and stored to shared memory once per row block, and that
+// is what competes with the tensor core:
+//   - Q and P are TMEM operands, so the tensor core reads only K and V from
+//     shared memory: per tile 64 KB written and 64 KB read, 1024 cycles of
+//     its 128 bytes a cycle, where Q in shared memory would add 64 KB;
+//   - K and V tiles have one layout (64 x 64 blocks of 128-byte rows, 128-byte
+//     swizzle): K is read as a K-major operand, V as an MN-major one, so no
+//     transposition is needed;
+//   - scales stay out of the codes: a position's key scale multiplies its
+//     score, and its value scale enters the weight as 2^(s + log2 vs - ref),
+//     with one exponential; the sum of weights takes the same value times
+//     1 / vs.
+// Roles (13 warps): 0-3 softmax, one row a thread; 4-11 dequantise; 12 issues.
+// S_{j+1} is issued before P_j V_j, so the softmax of one tile overlaps the
+// products of its neighbours.  The running maximum is followed lazily: O is
+// rescaled only when a row's reference grows by more than 2^8, which weights
+// of up to 2^14 in fp16 leave room for.
+// Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded
+// ones, in fp32.  Every wait is bounded.
+#pragma once
+
+#include "attn_token.cuh"
+#include "gsq_tc.cuh"
+
+namespace gsq {
+
+constexpr int AR_M = 128, AR_TILE = 64;
+constexpr int AR_SOFTMAX = 4, AR_DEQUANT = 8;  // warps
+constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 1);
+
+template <int D>
+struct ArGeom {
+  static constexpr int ITEM = AR_TILE * D * 2;  // one K or V tile in fp16
+  static constexpr int STAGES = 6;
+  static constexpr int SCALES = AR_SOFTMAX * 3 * AR_TILE * 4;
+  static constexpr int SMEM = 1024 + STAGES * ITEM + SCALES + 256;
+  static constexpr int O = 0, Q = D, S = Q + D / 2, P = S + AR_TILE;  // TMEM columns
+  static constexpr int COLS = 512;
+  static_assert(P + AR_TILE <= COLS && SMEM <= 227 * 1024, "fits");
+};
+
+struct ArShape {  // blocks of 128 rows; with a causal mask an early block sees fewer positions
+  static constexpr int ROWS = AR_M;
+  __device__ static int blocks(const AttnArgs& a) { return (a.n * a.group + AR_M - 1) / AR_M; }
+  __device__ static int tiles(const AttnArgs& a, const SeqSpan& s, int mb) {
+    if (mb * AR_M / a.group >= s.count) return 0;
+    int64_t len = s.len;
+    if (!a.tree) {
+      const int last = min(((mb + 1) * AR_M - 1) / a.group, s.count - 1);
+      len = min(max(s.base + last + 1, (int64_t)0), a.cap);
+    }
+    return (int)((len + AR_TILE - 1) / AR_TILE);
+  }
+};
+using ArList = TileList<ArShape>;
+
+// A run: the part of one unit that lies in this CTA's tiles [first, last).
+struct ArRun {
+  int t, last, len;  // the run's first tile; the CTA's end; tiles of the run
+  bool whole;        // all of the unit
+  Place at;
+
+  __device__ void settle() {
+    len = min(at.tiles - at.tile, last - t);
+    whole = at.tile == 0 && len == at.tiles;
+  }
+  __device__ void begin(const AttnArgs& a, int first, int end) {
+    t = first;
+    last = end;
+    at = ArList::locate(a, first);
+    settle();
+  }
+  __device__ bool next(const AttnArgs& a) {
+    t += len;
+    if (t >= last) return false;
+    ArList::next_unit(a, at);
+    settle();
+    return true;
+  }
+};
+
+// ---- tcgen05 with a TMEM operand, and wide TMEM loads and stores ----
+
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+#define GSQ_R8(x, i) x[i], x[i + 1], x[i + 2], x[i + 3], x[i + 4], x[i + 5], x[i + 6], x[i + 7]
+#define GSQ_O8(x, i) "=r"(x[i]), "=r"(x[i + 1]), "=r"(x[i + 2]), "=r"(x[i + 3]), "=r"(x[i + 4]), "=r"(x[i + 5]), \
+                     "=r"(x[i + 6]), "=r"(x[i + 7])
+#define GSQ_I8(x, i) "r"(x[i]), "r"(x[i + 1]), "r"(x[i + 2]), "r"(x[i + 3]), "r"(x[i + 4]), "r"(x[i + 5]), \
+                     "r"(x[i + 6]), "r"(x[i + 7])
+// 32 columns of this thread's lane; the load is complete after tmem_wait_ld().
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : GSQ_O8(r, 0), GSQ_O8(r, 8), GSQ_O8(r, 16), GSQ_O8(r, 24)
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::GSQ_I8(r, 0), GSQ_I8(r, 8), GSQ_I8(r, 16),
+      GSQ_I8(r, 24), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major operand, 128-byte swizzle: rows of 64 values, 8 rows (of K) 1024 bytes apart from the next 8, the next 64
+// values of MN `lbo` bytes on.
+__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(lbo >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// D = fp32, A = B = fp16, M = 128; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t ar_idesc(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AR_M >> 4) << 24);
+}
+
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 c;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+// A bounded wait of a whole warp: all lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err));
+}
+
+// Which of positions p0 .. p0 + 63 token i of sequence b sees, as bits.
+__device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const SeqSpan& s, int i, int64_t p0) {
+  if (i >= s.count) return 0;
+  auto below = [](int64_t k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
+  if (!a.tree) return below(min(s.base + i + 1, s.len) - p0);
+  const int64_t off = p0 - s.base;  // of bit 0 among the new tokens
+  uint64_t m = below(-off);
+  const int32_t* row = a.tree + b * a.tree_stride + (int64_t)i * a.words;
+  const int64_t w0 = off >> 5;  // floor
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    const int64_t w = w0 + k;
+    const int shift = (int)(w * 32 - off);  // -31 .. 64
+    if (w < 0 || w >= a.words || shift >= 64) continue;
+    const uint64_t bits = (uint32_t)row[w];
+    m |= shift < 0 ? bits >> -shift : bits << shift;
+  }
+  return m & below(s.len - p0);
+}
+
+template <typename T, int FMT, int D>
+__global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs a) {
+  using G = ArGeom<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* scales = reinterpret_cast<float*>(smem + G::STAGES * G::ITEM);  // [softmax warp][ks | log2 vs | 1 / vs][64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::STAGES * G::ITEM + G::SCALES);
+  uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
+  uint64_t* empty = full + G::STAGES;     // [STAGES] commit
+  uint64_t* s_full = empty + G::STAGES;   // commit
+  uint64_t* s_free = s_full + 1;          // count AR_SOFTMAX
+  uint64_t* p_full = s_free + 1;          // [2] count AR_SOFTMAX
+  uint64_t* pv_done = p_full + 2;         // [2] commit
+  uint64_t* q_full = pv_done + 2;         // count AR_SOFTMAX
+  uint64_t* drained = q_full + 1;         // commit
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  static_assert((2 * G::STAGES + 8) * 8 + 4 <= 256, "barriers");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == AR_SOFTMAX + AR_DEQUANT) tmem_alloc(tmem_slot, G::COLS);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < G::STAGES; i++) {
+      mbar_init(&full[i], AR_DEQUANT);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, AR_SOFTMAX);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&p_full[i], AR_SOFTMAX);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, AR_SOFTMAX);
+    mbar_init(drained, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // after the allocation: the next kernel's cannot come between
+  pdl_wait();
+
+  const int total = ArList::total(a), ctas = min(a.ctas, total);
+  const bool busy = (int)blockIdx.x < ctas;
+  const int first = busy ? ArList::first_of(blockIdx.x, total, ctas) : 0;
+  const int last = busy ? ArList::first_of(blockIdx.x + 1, total, ctas) : 0;
+  bool ok = true;
+
+  if (!busy) {
+    // nothing to do but to give the TMEM back
+  } else if (warp < AR_SOFTMAX) {
+    // ---------------- softmax: thread = row ----------------
+    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    const int rows = a.n * a.group;
+    ArRun run;
+    run.begin(a, first, last);
+    int tile = 0;  // of the CTA
+    do {
+      const int r = run.at.mb * AR_M + threadIdx.x;  // row of the unit's head
+      const int i = r / a.group;
+      // Q: the row in fp16 (bf16: times a power of two), 16 dimensions in 8 columns
+      float amax = 0.f;
+      int shift = 0;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll 4
+        for (int d = 0; d < D; d += 8) {
+          float f[8];
+          load_q8<T>(a, run.at.b, run.at.kh, r, d, f);
+#pragma unroll
+          for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(f[e]));
+        }
+        shift = q_shift(amax);
+      }
+      const float up = (a.scale < 0.f ? -1.f : 1.f) * exp2_int(shift);
+      const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);
+#pragma unroll 1
+      for (int c = 0; c < D / 64; c++) {
+        uint32_t w[32];
+#pragma unroll
+        for (int d = 0; d < 64; d += 8) {
+          float f[8];
+          load_q8<T>(a, run.at.b, run.at.kh, r, 64 * c + d, f);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const __half2 h = __floats2half2_rn(f[2 * e] * up, f[2 * e + 1] * up);
+            w[d / 2 + e] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        tmem_st32(lanes + G::Q + 32 * c, w);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+
+      float2 next_k, next_v;  // scales of positions p, p + 1 of the coming tile; 0 past the end
+      const int64_t row0 = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap;
+      auto fetch_scales = [&](int64_t p0) {
+        const int64_t p = p0 + 2 * lane;
+        const bool in0 = p < run.at.span.len, in1 = p + 1 < run.at.span.len;
+        next_k = make_float2(in0 ? a.ks[row0 + p] : 0.f, in1 ? a.ks[row0 + p + 1] : 0.f);
+        next_v = make_float2(in0 ? a.vs[row0 + p] : 0.f, in1 ? a.vs[row0 + p + 1] : 0.f);
+      };
+      fetch_scales((int64_t)run.at.tile * AR_TILE);
+      float* ks = scales + warp * 3 * AR_TILE;
+
+      float ref = -INFINITY, sum = 0.f;
+      for (int j = 0; j < run.len && ok; j++, tile++) {
+        const int64_t p0 = (int64_t)(run.at.tile + j) * AR_TILE;
+        // the tile's scales, two positions a lane; each warp keeps its own, so that no barrier joins the warps
+        __syncwarp();
+        uint32_t zero_even, zero_odd;  // positions of scale 0, bit i: 2i (2i + 1)
+        {
+          const float2 kv2 = next_k, vv2 = next_v;
+          if (j + 1 < run.len) fetch_scales(p0 + AR_TILE);
+          // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of
+          // scale 0 has no part in the output, but in the sum of weights: it is weighted with the largest scale of
+          // the tile, and that weight left out of P.
+          float lx = vv2.x > 0.f ? fmaxf(log2_approx(vv2.x), -100.f) : -INFINITY;
+          float ly = vv2.y > 0.f ? fmaxf(log2_approx(vv2.y), -100.f) : -INFINITY;
+          float top = fmaxf(lx, ly);
+#pragma unroll
+          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (top == -INFINITY) top = -40.f;
+          zero_even = __ballot_sync(0xffffffffu, vv2.x == 0.f);
+          zero_odd = __ballot_sync(0xffffffffu, vv2.y == 0.f);
+          lx = vv2.x > 0.f ? lx : vv2.x == 0.f ? top : vv2.x;  // NaN stays
+          ly = vv2.y > 0.f ? ly : vv2.y == 0.f ? top : vv2.y;
+          *reinterpret_cast<float2*>(ks + 2 * lane) = kv2;
+          *reinterpret_cast<float2*>(ks + AR_TILE + 2 * lane) = make_float2(lx, ly);
+          *reinterpret_cast<float2*>(ks + 2 * AR_TILE + 2 * lane) = make_float2(exp2_approx(-lx), exp2_approx(-ly));
+        }
+        __syncwarp();
+        ok = warp_wait(s_full, (uint32_t)(tile & 1), a.err);
+        if (!ok) break;
+        tc_fence_after();
+        float s[AR_TILE];
+        tmem_ld32(lanes + G::S, reinterpret_cast<uint32_t*>(s));
+        tmem_ld32(lanes + G::S + 32, reinterpret_cast<uint32_t*>(s + 32));
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+
+        // t = score + log2 vs, to base 2
+        const float2 f2 = make_float2(factor, factor);
+#pragma unroll
+        for (int e = 0; e < AR_TILE; e += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(ks + e);
+          const float4 v4 = *reinterpret_cast<const float4*>(ks + AR_TILE + e);
+          const float2 x = fma2(mul2(make_float2(s[e], s[e + 1]), make_float2(k4.x, k4.y)), f2, make_float2(v4.x, v4.y));
+          const float2 y =
+              fma2(mul2(make_float2(s[e + 2], s[e + 3]), make_float2(k4.z, k4.w)), f2, make_float2(v4.z, v4.w));
+          s[e] = x.x;
+          s[e + 1] = x.y;
+          s[e + 2] = y.x;
+          s[e + 3] = y.y;
+        }
+        const bool edge = p0 + AR_TILE > min(run.at.span.base, run.at.span.len);  // the same for all threads
+        uint64_t see = ~0ull;
+        if (edge) {
+          see = ar_visible(a, run.at.b, run.at.span, i, p0);
+#pragma unroll
+          for (int e = 0; e < AR_TILE; e++)
+            if (!(see >> e & 1)) s[e] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < AR_TILE; e++) top = fmaxf(top, s[e]);
+        // pv_done[tile & 1] of tile - 2: its P is read, this tile's may be written
+        if (tile >= 2) ok = warp_wait(&pv_done[tile & 1], (uint32_t)((tile / 2 - 1) & 1), a.err);
+        if (!ok) break;
+        const bool grow = top > ref + 8.f || (ref == -INFINITY && top > ref);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float next = grow ? top : ref;
+          const float f = ref == -INFINITY ? 0.f : exp2_approx(ref - next);
+          sum *= ref == next ? 1.f : f;
+          if (j > 0) {
+            // O holds this unit's tiles so far: wait for the last of them and rescale it
+            ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
+            if (!ok) break;
+            tc_fence_after();
+            const float f1 = ref == next || ref == -INFINITY ? 1.f : f;  // no weight yet: O is zero (or NaN, and stays)
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(lanes + G::O + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f1);
+              tmem_st32(lanes + G::O + c, o);
+            }
+            tmem_wait_st();
+          }
+          ref = next;
+        }
+        // weights 2^(t - ref + 6), at most 2^14
+        const float shift6 = 6.f - (ref == -INFINITY ? 0.f : ref);
+        const float2 sh = make_float2(shift6, shift6);
+        uint32_t w[AR_TILE / 2];
+        float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int e = 0; e < AR_TILE; e += 4) {
+          float2 x = add2(make_float2(s[e], s[e + 1]), sh), y = add2(make_float2(s[e + 2], s[e + 3]), sh);
+          x.x = exp2_approx(x.x);
+          x.y = exp2_approx(x.y);
+          y.x = exp2_approx(y.x);
+          y.y = exp2_approx(y.y);
+          float4 i4 = *reinterpret_cast<const float4*>(ks + 2 * AR_TILE + e);
+          if (edge) {  // a hidden position's scale may be NaN
+            i4.x = see >> e & 1 ? i4.x : 0.f;
+            i4.y = see >> (e + 1) & 1 ? i4.y : 0.f;
+            i4.z = see >> (e + 2) & 1 ? i4.z : 0.f;
+            i4.w = see >> (e + 3) & 1 ? i4.w : 0.f;
+          }
+          acc0 = fma2(x, make_float2(i4.x, i4.y), acc0);
+          acc1 = fma2(y, make_float2(i4.z, i4.w), acc1);
+          if (zero_even | zero_odd) {
+            x.x = zero_even >> (e / 2) & 1 ? 0.f : x.x;
+            x.y = zero_odd >> (e / 2) & 1 ? 0.f : x.y;
+            y.x = zero_even >> (e / 2 + 1) & 1 ? 0.f : y.x;
+            y.y = zero_odd >> (e / 2 + 1) & 1 ? 0.f : y.y;
+          }
+          const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
+          w[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+          w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+        }
+        acc0 = add2(acc0, acc1);
+        sum += acc0.x + acc0.y;
+        tmem_st32(lanes + G::P + (tile & 1) * (AR_TILE / 2), w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[tile & 1]);
+      }
+      if (!ok) break;
+
+      // ---- the unit's (or its part's) result ----
+      ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
+      if (!ok) break;
+      tc_fence_after();
+      const int slot = 2 * blockIdx.x + (run.t == first ? 0 : 1);
+      const bool live = r < rows;
+      const bool none = sum == 0.f || i >= run.at.span.count;
+      const float inv = none ? 0.f : 1.f / sum;
+      float* part = a.part + ((int64_t)slot * AR_M + threadIdx.x) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(lanes + G::O + c, o);
+        tmem_wait_ld();
+        if (!live) continue;
+        if (run.whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) f[x] = none ? 0.f : __uint_as_float(o[e + x]) * inv;
+            store_row8<T>(a, run.at.b, run.at.kh, r, c + e, f);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (live && !run.whole)
+        *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * AR_M + threadIdx.x) * 2) = make_float2(ref, sum);
+      tc_fence_before();  // the loads of O come before the next unit's products (through q_full)
+    } while (run.next(a));
+  } else if (warp < AR_SOFTMAX + AR_DEQUANT) {
+    // ---------------- dequantise: items in the order K0, K1, V0, K2, V1, .. of each run ----------------
+    // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
+    // swizzled row. Rows of one lane differ by multiples of 8, so its swizzle is a constant.
+    const int w = warp - AR_SOFTMAX;
+    constexpr int LPR = D / 8;               // lanes per row
+    constexpr int RPW = 32 / LPR;            // rows per warp and step
+    constexpr int STEPS = AR_TILE / (8 * RPW);
+    const int row = w * RPW + lane / LPR, chunk = lane % LPR;  // + 8 RPW per step
+    const uint32_t dst = (uint32_t)(chunk / 8 * (AR_TILE * 128) + row * 128 + ((chunk % 8) ^ (row & 7)) * 16);
+    ArRun run;
+    run.begin(a, first, last);
+    int kpos = 0, vpos = 0;
+    bool more = true;
+    uint2 ahead[2][STEPS];
+    // Loads the next item's codes; zeros past the sequence's end.
+    auto load = [&](uint2 (&c)[STEPS]) {
+      if (!more) return;
+      const bool key = kpos < run.len && kpos - vpos < 2;
+      const int j = key ? kpos++ : vpos++;
+      const int64_t p0 = (int64_t)(run.at.tile + j) * AR_TILE + row;
+      const int64_t left = run.at.span.len - p0;
+      const uint8_t* src = (key ? a.kc : a.vc) + (((int64_t)run.at.b * a.kv + run.at.kh) * a.cap + p0) * D + chunk * 8;
+#pragma unroll
+      for (int i = 0; i < STEPS; i++)
+        c[i] = i * 8 * RPW < left ? *reinterpret_cast<const uint2*>(src + (int64_t)i * 8 * RPW * D) : make_uint2(0u, 0u);
+      if (vpos == run.len) {
+        more = run.next(a);
+        kpos = vpos = 0;
+      }
+    };
+    const int items = 2 * (last - first);
+    load(ahead[0]);
+    load(ahead[1]);
+    int stage = 0, use = 0;
+    for (int it = 0; it < items && ok; it += 2) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (use > 0) ok = ok && warp_wait(&empty[stage], (uint32_t)((use - 1) & 1), a.err);
+        if (!ok) break;
+        uint8_t* p = smem + stage * G::ITEM + dst;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+          uint4 v;
+          codes_to_half2<FMT>(ahead[h][i].x, v.x, v.y);
+          codes_to_half2<FMT>(ahead[h][i].y, v.z, v.w);
+          *reinterpret_cast<uint4*>(p + i * 8 * RPW * 128) = v;
+        }
+        load(ahead[h]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[stage]);
+        if (++stage == G::STAGES) {
+          stage = 0;
+          use++;
+        }
+      }
+    }
+  } else {
+    // ---------------- issue ----------------
+    ArRun run;
+    run.begin(a, first, last);
+    int stage = 0, use = 0, tile = 0, runs = 0;
+    auto next_item = [&]() {
+      if (++stage == G::STAGES) {
+        stage = 0;
+        use++;
+      }
+    };
+    // S of the CTA's tile t: into TMEM when the softmax has taken tile t - 1's
+    auto scores = [&](int t) {
+      ok = warp_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
+           (t == 0 || warp_wait(s_free, (uint32_t)((t - 1) & 1), a.err));
+      if (!ok) return;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t b = smem_u32(smem + stage * G::ITEM);
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+          tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, sw128_desc(b + k / 4 * (AR_TILE * 128) + k % 4 * 32),
+                        ar_idesc(AR_TILE, false), k != 0);
+        tc_commit(&empty[stage]);
+        tc_commit(s_full);
+      }
+      __syncwarp();
+      next_item();
+    };
+    do {
+      ok = warp_wait(q_full, (uint32_t)(runs++ & 1), a.err);
+      if (!ok) break;
+      scores(tile);
+      for (int j = 0; j < run.len && ok; j++, tile++) {
+        if (j + 1 < run.len) scores(tile + 1);
+        ok = ok && warp_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
+             warp_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t b = smem_u32(smem + stage * G::ITEM);
+#pragma unroll
+          for (int k = 0; k < AR_TILE / 16; k++)
+            tc_mma_f16_ts(tmem + G::O, tmem + G::P + (tile & 1) * (AR_TILE / 2) + 8 * k,
+                          sw128_mn_desc(b + k * 2048, AR_TILE * 128), ar_idesc(D, true), j + k != 0);
+          tc_commit(&empty[stage]);
+          tc_commit(&pv_done[tile & 1]);
+        }
+        __syncwarp();
+        next_item();
+      }
+    } while (ok && run.next(a));
+    // nothing may still write TMEM when it is given back
+    if (lane == 0) tc_commit(drained);
+    __syncwarp();
+    warp_wait(drained, 0, a.err);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == AR_SOFTMAX + AR_DEQUANT) tmem_dealloc(tmem, G::COLS);
+}
+
+}  // namespace gsq

@@ -70,26 +70,12 @@ __device__ __forceinline__ void cp_async4_zfill(void* dst, const void* src, bool
 // read two units of four rows).
 __device__ __forceinline__ int at_unit(int p, int u) { return u ^ ((p & 6) ^ (p & 1) << 2); }
 
-// A cursor over the tiles of the list: unit (sequence, head) and tile in it.
-struct AtCursor {
-  int b, kh, tile, tiles;
-  SeqSpan span;
-  __device__ void enter(const AttnArgs& a, int seq) {
-    b = seq;
-    span = seq_span(a, seq);
-    tiles = (int)((span.len + AT_TILE - 1) / AT_TILE);
-  }
-  __device__ void next(const AttnArgs& a) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++kh < a.kv) return;
-    kh = 0;
-    do {
-      if (b + 1 >= a.batch) return;  // past the last tile: not used
-      enter(a, b + 1);
-    } while (tiles == 0);
-  }
+struct AtShape {  // all rows of a head together
+  static constexpr int ROWS = 16;
+  __device__ static int blocks(const AttnArgs&) { return 1; }
+  __device__ static int tiles(const AttnArgs&, const SeqSpan& s, int) { return (int)((s.len + AT_TILE - 1) / AT_TILE); }
 };
+using AtList = TileList<AtShape>;
 
 // One row's eight values of q from dimension d on, in fp32.
 template <typename T>
@@ -128,19 +114,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
   float* stat = reinterpret_cast<float*>(smem + G::RING + G::BUFS * G::BUF);  // [warp][row][m, l]
   uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::BUFS * G::BUF + G::STAT);
 
-  const int total = TileList<AT_TILE>::total(a);
-  const int ctas = min(a.ctas, total);
+  const int total = AtList::total(a), ctas = min(a.ctas, total);
   if ((int)blockIdx.x >= ctas) return;
-  const int first = TileList<AT_TILE>::first_of(blockIdx.x, total, ctas);
-  const int last = TileList<AT_TILE>::first_of(blockIdx.x + 1, total, ctas);
-  AtCursor get, use;
-  {
-    int in_seq;
-    get.enter(a, TileList<AT_TILE>::locate(a, first, &in_seq));
-    get.kh = in_seq / get.tiles;
-    get.tile = in_seq % get.tiles;
-    use = get;
-  }
+  const int first = AtList::first_of(blockIdx.x, total, ctas), last = AtList::first_of(blockIdx.x + 1, total, ctas);
+  Place get = AtList::locate(a, first), use = get;
   const int rows = a.n * a.group;
 
   int fetched = first;
@@ -163,7 +140,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
       const int p = lane & 15;
       const bool in = p < left;
       cp_async4_zfill(st + 32 * D + lane * 4, (lane < 16 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
-      get.next(a);
+      if (++get.tile == get.tiles && fetched + 1 < last) AtList::next_unit(a, get);
     }
     fetched++;
     cp_async_commit();
@@ -249,7 +226,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
       __syncwarp();
       const uint8_t* st = ring + (tile - first) % G::STAGES * G::STAGE;
       const int64_t p0 = (int64_t)use.tile * AT_TILE + warp * 16;
-      use.next(a);
+      use.tile++;
       if (p0 >= span.len) continue;
       const float* sc = reinterpret_cast<const float*>(st + 32 * D);
 
@@ -442,68 +419,78 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
       }
     }
     __syncthreads();  // buf and stat are free
+    if (use.tile == use.tiles && tile < last) AtList::next_unit(a, use);
   }
 }
 
-// Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the units
-// that have no position.  One CTA per (unit, row): D / 4 threads across, the rest over the parts.
-template <typename T, int D, int TILE>
+// Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the rows
+// that no tile reaches. CTA (c, y): the unit in which CTA c begins, if c is the second that has a part of it; rows y,
+// y + gridDim.y, ..; D / 4 threads across a row, the rest over the parts.
+template <typename T, int D, typename Shape>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+  using List = TileList<Shape>;
   constexpr int ACROSS = D / 4, DOWN = 256 / ACROSS;
   __shared__ float4 acc[DOWN][ACROSS];
   pdl_launch_dependents();
   pdl_wait();
   const int rows = a.n * a.group;
-  const int u = blockIdx.x / rows, r = blockIdx.x % rows, b = u / a.kv, kh = u % a.kv;
-  const SeqSpan span = seq_span(a, b);
-  const int tiles = (int)((span.len + TILE - 1) / TILE);
   const int x = threadIdx.x % ACROSS, y = threadIdx.x / ACROSS;
-  if (tiles == 0) {
-    if (y == 0) {
-      store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
-      store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
-    }
-    return;
+  const int blocks = Shape::blocks(a);
+  for (int i = blockIdx.x; i < a.batch * blocks; i += gridDim.x) {
+    const int b = i / blocks, mb = i % blocks;
+    if (Shape::tiles(a, seq_span(a, b), mb)) continue;
+    const int r0 = mb * Shape::ROWS, r1 = min(rows, r0 + Shape::ROWS);
+    for (int kh = 0; kh < a.kv; kh++)
+      for (int r = r0 + blockIdx.y * DOWN + y; r < r1; r += gridDim.y * DOWN) {
+        store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
+        store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
+      }
   }
-  const int total = TileList<TILE>::total(a);
-  const int t0 = TileList<TILE>::before(a, b) + kh * tiles;
-  const int ctas = min(a.ctas, total);
-  const int c0 = TileList<TILE>::cta_of(t0, total, ctas), c1 = TileList<TILE>::cta_of(t0 + tiles - 1, total, ctas);
-  if (c0 == c1) return;
+  const int total = List::total(a), ctas = min(a.ctas, total), c = blockIdx.x;
+  if (c == 0 || c >= ctas) return;
+  const int t = List::first_of(c, total, ctas);
+  const Place p = List::locate(a, t);
+  const int t0 = t - p.tile;
+  const int c0 = List::cta_of(t0, total, ctas), c1 = List::cta_of(t0 + p.tiles - 1, total, ctas);
+  if (p.tile == 0 || c0 != c - 1) return;
   // only the first CTA can have begun another unit before this one
-  const int s0 = 2 * c0 + (TileList<TILE>::first_of(c0, total, ctas) == t0 ? 0 : 1);
-  auto slot = [&](int c) { return c == c0 ? s0 : 2 * c; };
-  float top = -INFINITY, sum = 0.f;
-  for (int c = c0; c <= c1; c++) top = fmaxf(top, a.stat[((int64_t)slot(c) * a.rows8 + r) * 2]);
-  for (int c = c0; c <= c1; c++) {
-    const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)slot(c) * a.rows8 + r) * 2);
-    sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);
-  }
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int c = c0 + y; c <= c1; c += DOWN) {
-    const int64_t at = (int64_t)slot(c) * a.rows8 + r;
-    const float mc = a.stat[at * 2], f = mc == -INFINITY ? 1.f : exp2_approx(mc - top);
-    const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + 4 * x);
-    o.x = fmaf(v.x, f, o.x);
-    o.y = fmaf(v.y, f, o.y);
-    o.z = fmaf(v.z, f, o.z);
-    o.w = fmaf(v.w, f, o.w);
-  }
-  acc[y][x] = o;
-  __syncthreads();
-  if (y == 0) {
-    for (int i = 1; i < DOWN; i++) {
-      const float4 v = acc[i][x];
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
+  const int s0 = 2 * c0 + (List::first_of(c0, total, ctas) == t0 ? 0 : 1);
+  auto slot = [&](int i) { return i == c0 ? s0 : 2 * i; };
+  const int r0 = p.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS);
+  for (int r = blockIdx.y; r < count; r += gridDim.y) {
+    float top = -INFINITY, sum = 0.f;
+    for (int i = c0; i <= c1; i++) top = fmaxf(top, a.stat[((int64_t)slot(i) * a.rows8 + r) * 2]);
+    for (int i = c0; i <= c1; i++) {
+      const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)slot(i) * a.rows8 + r) * 2);
+      sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);  // no position seen: 0, or NaN
     }
-    const bool none = sum == 0.f || r / a.group >= span.count;
-    const float inv = none ? 0.f : 1.f / sum;
-    store_row2<T>(a, b, kh, r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
-    store_row2<T>(a, b, kh, r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = c0 + y; i <= c1; i += DOWN) {
+      const int64_t at = (int64_t)slot(i) * a.rows8 + r;
+      const float m = a.stat[at * 2], f = m == -INFINITY ? 1.f : exp2_approx(m - top);
+      const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + 4 * x);
+      o.x = fmaf(v.x, f, o.x);
+      o.y = fmaf(v.y, f, o.y);
+      o.z = fmaf(v.z, f, o.z);
+      o.w = fmaf(v.w, f, o.w);
+    }
+    __syncthreads();  // acc is free
+    acc[y][x] = o;
+    __syncthreads();
+    if (y == 0) {
+      for (int i = 1; i < DOWN; i++) {
+        const float4 v = acc[i][x];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+      }
+      const bool none = sum == 0.f || (r0 + r) / a.group >= p.span.count;
+      const float inv = none ? 0.f : 1.f / sum;
+      store_row2<T>(a, p.b, p.kh, r0 + r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
+      store_row2<T>(a, p.b, p.kh, r0 + r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
+    }
   }
 }
 
