@@ -29,6 +29,7 @@ struct AttnArgs {
   int ctas, rows8;      // CTAs of the split, rows of a partial result
   int* err;             // device error word
   float *part, *stat;   // [2 * ctas][rows8][dim], [2 * ctas][rows8][2] (max in base 2, sum)
+  struct Joint* joints;  // [ctas]
 };
 
 // Cached positions and new tokens of sequence b.
@@ -56,6 +57,12 @@ struct Place {
   SeqSpan span;
 };
 
+// A unit in several CTAs' parts, noted by the second of them (c0 + 1): part of CTA c0 in slot s0, of c0 + 1 .. c1 in
+// slots 2 c. parts == 0: CTA c does not begin in a unit's second part.
+struct Joint {
+  int parts, b, kh, mb, c0, s0, count, pad;
+};
+
 // Shape: blocks(a) row blocks of ROWS rows each; tiles(a, span, mb).
 template <typename Shape>
 struct TileList {
@@ -75,34 +82,75 @@ struct TileList {
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s * a.kv;
   }
-  // Where tile t (below the total) lies; every lane of the warp calls it.
+  // Where tile t (below the total) lies; every lane of the warp calls it. The lanes take a sequence each, or where a
+  // head has many blocks a block each of one sequence after the other.
   __device__ static Place locate(const AttnArgs& a, int t) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, blocks = Shape::blocks(a);
     Place p = {};
-    int done = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      const int mine = of_head(a, b0 + lane) * a.kv;
-      int sum = mine;
+    auto scan = [&](int v) {
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, t < done + sum);
+      return v;
+    };
+    int done = 0, head = 0;
+    if (blocks <= 4) {
+      for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const int mine = of_head(a, b0 + lane) * a.kv;
+        const int sum = scan(mine);
+        const unsigned past = __ballot_sync(0xffffffffu, t < done + sum);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          done += __shfl_sync(0xffffffffu, sum - mine, l);
+          head = __shfl_sync(0xffffffffu, mine, l) / a.kv;
+          p.b = b0 + l;
+          break;
+        }
+        done += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    } else {
+      for (;; p.b++) {
+        const SeqSpan span = seq_span(a, p.b);
+        head = 0;
+        for (int mb = lane; mb < blocks; mb += 32) head += Shape::tiles(a, span, mb);
+        head = __reduce_add_sync(0xffffffffu, head);
+        if (t < done + head * a.kv) break;
+        done += head * a.kv;
+      }
+    }
+    p.kh = (t - done) / head;
+    p.tile = (t - done) % head;
+    p.span = seq_span(a, p.b);
+    for (;; p.mb += 32) {
+      const int mine = p.mb + lane < blocks ? Shape::tiles(a, p.span, p.mb + lane) : 0;
+      const int sum = scan(mine);
+      const unsigned past = __ballot_sync(0xffffffffu, p.tile < sum);
       if (past) {
         const int l = __ffs(past) - 1;
-        const int at = t - done - __shfl_sync(0xffffffffu, sum - mine, l);
-        const int head = __shfl_sync(0xffffffffu, mine, l) / a.kv;
-        p.b = b0 + l;
-        p.kh = at / head;
-        p.tile = at % head;
-        break;
+        p.tile -= __shfl_sync(0xffffffffu, sum - mine, l);
+        p.tiles = __shfl_sync(0xffffffffu, mine, l);
+        p.mb += l;
+        return p;
       }
-      done += __shfl_sync(0xffffffffu, sum, 31);
+      p.tile -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    p.span = seq_span(a, p.b);
-    for (; p.tile >= (p.tiles = Shape::tiles(a, p.span, p.mb)); p.mb++) p.tile -= p.tiles;
-    return p;
+  }
+  // What the joining launch has to know of CTA c, which begins with tile t at p (one thread).
+  __device__ static void note(const AttnArgs& a, int c, int t, const Place& p, int total, int ctas) {
+    Joint j = {};
+    const int t0 = t - p.tile;
+    j.c0 = cta_of(t0, total, ctas);
+    if (p.tile && j.c0 == c - 1) {
+      j.parts = cta_of(t0 + p.tiles - 1, total, ctas) - j.c0 + 1;
+      j.b = p.b;
+      j.kh = p.kh;
+      j.mb = p.mb;
+      j.s0 = 2 * j.c0 + (first_of(j.c0, total, ctas) == t0 ? 0 : 1);  // CTA c0 may have begun another unit before it
+      j.count = p.span.count;
+    }
+    a.joints[c] = j;
   }
   // The first tile of the unit after p's; there must be one.
   __device__ static void next_unit(const AttnArgs& a, Place& p) {

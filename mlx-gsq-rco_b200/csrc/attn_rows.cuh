@@ -18,7 +18,8 @@
 //     score, and its value scale enters the weight as 2^(s + log2 vs - ref),
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs.
-// Roles (13 warps): 0-3 softmax, one row a thread; 4-11 dequantise; 12 issues.
+// Roles (16 warps): 0-3 softmax, one row a thread; 4-11 dequantise; 12 issues
+// (13-15 complete its warpgroup, so that registers can be shared out by role).
 // S_{j+1} is issued before P_j V_j, so the softmax of one tile overlaps the
 // products of its neighbours.  The running maximum is followed lazily: O is
 // rescaled only when a row's reference grows by more than 2^8, which weights
@@ -34,7 +35,7 @@ namespace gsq {
 
 constexpr int AR_M = 128, AR_TILE = 64;
 constexpr int AR_SOFTMAX = 4, AR_DEQUANT = 8;  // warps
-constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 1);
+constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // the last warpgroup: one warp issues, three idle
 
 template <int D>
 struct ArGeom {
@@ -230,8 +231,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 
   if (!busy) {
     // nothing to do but to give the TMEM back
+    if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
   } else if (warp < AR_SOFTMAX) {
     // ---------------- softmax: thread = row ----------------
+    // of 128 registers a thread at the launch (512 in all): 208 here, 104 for each dequantising warpgroup, 96
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
     const int rows = a.n * a.group;
     ArRun run;
@@ -454,6 +458,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     // ---------------- dequantise: items in the order K0, K1, V0, K2, V1, .. of each run ----------------
     // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
     // swizzled row. Rows of one lane differ by multiples of 8, so its swizzle is a constant.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int w = warp - AR_SOFTMAX;
     constexpr int LPR = D / 8;               // lanes per row
     constexpr int RPW = 32 / LPR;            // rows per warp and step
@@ -509,9 +514,12 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       }
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == AR_SOFTMAX + AR_DEQUANT) {
     // ---------------- issue ----------------
     ArRun run;
     run.begin(a, first, last);
+    if (lane == 0) ArList::note(a, blockIdx.x, first, run.at, total, ctas);
     int stage = 0, use = 0, tile = 0, runs = 0;
     auto next_item = [&]() {
       if (++stage == G::STAGES) {
@@ -564,6 +572,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     if (lane == 0) tc_commit(drained);
     __syncwarp();
     warp_wait(drained, 0, a.err);
+    }
   }
   tc_fence_before();
   __syncthreads();

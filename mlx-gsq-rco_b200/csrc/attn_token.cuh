@@ -115,9 +115,13 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
   uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::BUFS * G::BUF + G::STAT);
 
   const int total = AtList::total(a), ctas = min(a.ctas, total);
-  if ((int)blockIdx.x >= ctas) return;
+  if ((int)blockIdx.x >= ctas) {
+    if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
+    return;
+  }
   const int first = AtList::first_of(blockIdx.x, total, ctas), last = AtList::first_of(blockIdx.x + 1, total, ctas);
   Place get = AtList::locate(a, first), use = get;
+  if (threadIdx.x == 0) AtList::note(a, blockIdx.x, first, get, total, ctas);
   const int rows = a.n * a.group;
 
   int fetched = first;
@@ -424,52 +428,56 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
 }
 
 // Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the rows
-// that no tile reaches. CTA (c, y): the unit in which CTA c begins, if c is the second that has a part of it; rows y,
-// y + gridDim.y, ..; D / 4 threads across a row, the rest over the parts.
+// that no tile reaches. CTA (c, y): the unit that CTA c noted, rows y, y + gridDim.y, ..; D / 4 threads across a row,
+// the rest over the parts.
 template <typename T, int D, typename Shape>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
-  using List = TileList<Shape>;
   constexpr int ACROSS = D / 4, DOWN = 256 / ACROSS;
   __shared__ float4 acc[DOWN][ACROSS];
   pdl_launch_dependents();
   pdl_wait();
   const int rows = a.n * a.group;
   const int x = threadIdx.x % ACROSS, y = threadIdx.x / ACROSS;
-  const int blocks = Shape::blocks(a);
-  for (int i = blockIdx.x; i < a.batch * blocks; i += gridDim.x) {
-    const int b = i / blocks, mb = i % blocks;
-    if (Shape::tiles(a, seq_span(a, b), mb)) continue;
-    const int r0 = mb * Shape::ROWS, r1 = min(rows, r0 + Shape::ROWS);
-    for (int kh = 0; kh < a.kv; kh++)
-      for (int r = r0 + blockIdx.y * DOWN + y; r < r1; r += gridDim.y * DOWN) {
-        store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
-        store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
-      }
+  if (blockIdx.y == 0) {
+    const int blocks = Shape::blocks(a);
+    for (int i = blockIdx.x; i < a.batch * blocks; i += gridDim.x) {
+      const int b = i / blocks, mb = i % blocks;
+      if (Shape::tiles(a, seq_span(a, b), mb)) continue;
+      const int r0 = mb * Shape::ROWS, r1 = min(rows, r0 + Shape::ROWS);
+      for (int kh = 0; kh < a.kv; kh++)
+        for (int r = r0 + y; r < r1; r += DOWN) {
+          store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
+          store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
+        }
+    }
   }
-  const int total = List::total(a), ctas = min(a.ctas, total), c = blockIdx.x;
-  if (c == 0 || c >= ctas) return;
-  const int t = List::first_of(c, total, ctas);
-  const Place p = List::locate(a, t);
-  const int t0 = t - p.tile;
-  const int c0 = List::cta_of(t0, total, ctas), c1 = List::cta_of(t0 + p.tiles - 1, total, ctas);
-  if (p.tile == 0 || c0 != c - 1) return;
-  // only the first CTA can have begun another unit before this one
-  const int s0 = 2 * c0 + (List::first_of(c0, total, ctas) == t0 ? 0 : 1);
-  auto slot = [&](int i) { return i == c0 ? s0 : 2 * i; };
-  const int r0 = p.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS);
+  const Joint j = a.joints[blockIdx.x];
+  if (j.parts == 0) return;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? j.s0 : 2 * (j.c0 + i)) * a.rows8; };
+  const int r0 = j.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS);
   for (int r = blockIdx.y; r < count; r += gridDim.y) {
+    // reference and sum of all parts: the warp's lanes take a part each
     float top = -INFINITY, sum = 0.f;
-    for (int i = c0; i <= c1; i++) top = fmaxf(top, a.stat[((int64_t)slot(i) * a.rows8 + r) * 2]);
-    for (int i = c0; i <= c1; i++) {
-      const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)slot(i) * a.rows8 + r) * 2);
-      sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);  // no position seen: 0, or NaN
+    for (int i = threadIdx.x & 31; i < j.parts; i += 32) {
+      const float2 s = *reinterpret_cast<const float2*>(a.stat + (slot(i) + r) * 2);
+      const float next = fmaxf(top, s.x);
+      sum = sum * (top == next ? 1.f : exp2_approx(top - next)) +
+            (s.x == -INFINITY || s.x == next ? s.y : s.y * exp2_approx(s.x - next));  // no position seen: 0, or NaN
+      top = next;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float next = fmaxf(top, t2);
+      sum = (top == next || top == -INFINITY ? sum : sum * exp2_approx(top - next)) +
+            (t2 == next || t2 == -INFINITY ? s2 : s2 * exp2_approx(t2 - next));
+      top = next;
     }
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = c0 + y; i <= c1; i += DOWN) {
-      const int64_t at = (int64_t)slot(i) * a.rows8 + r;
-      const float m = a.stat[at * 2], f = m == -INFINITY ? 1.f : exp2_approx(m - top);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + 4 * x);
+    for (int i = y; i < j.parts; i += DOWN) {
+      const float m = a.stat[(slot(i) + r) * 2], f = m == -INFINITY ? 1.f : exp2_approx(m - top);
+      const float4 v = *reinterpret_cast<const float4*>(a.part + (slot(i) + r) * D + 4 * x);
       o.x = fmaf(v.x, f, o.x);
       o.y = fmaf(v.y, f, o.y);
       o.z = fmaf(v.z, f, o.z);
@@ -486,10 +494,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
         o.z += v.z;
         o.w += v.w;
       }
-      const bool none = sum == 0.f || (r0 + r) / a.group >= p.span.count;
+      const bool none = sum == 0.f || (r0 + r) / a.group >= j.count;
       const float inv = none ? 0.f : 1.f / sum;
-      store_row2<T>(a, p.b, p.kh, r0 + r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
-      store_row2<T>(a, p.b, p.kh, r0 + r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
+      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
+      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
     }
   }
 }

@@ -41,7 +41,7 @@ Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, i
     p.tiles = batch * kv * ((rows + AR_M - 1) / AR_M) * ((cap + AR_TILE - 1) / AR_TILE);
   }
   p.ctas = (int)(p.tiles < SMS ? p.tiles : SMS);
-  p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float);
+  p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float) + p.ctas * sizeof(Joint);
   return p;
 }
 
@@ -76,7 +76,7 @@ cudaError_t rows_launch(cudaStream_t st, const AttnArgs& a) {
   if (e == cudaSuccess)
     e = launch_pdl(attn_rows_kernel<T, FMT, D>, dim3((unsigned)a.ctas), dim3(AR_THREADS), smem, st, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, 8), dim3(256), 0, st, a);
+  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, 32), dim3(256), 0, st, a);
 }
 
 template <typename T, int FMT>
@@ -156,6 +156,7 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   a.rows8 = plan.rows8;
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + (size_t)2 * a.ctas * a.rows8 * dim;
+  a.joints = reinterpret_cast<Joint*>(a.stat + (size_t)2 * a.ctas * a.rows8 * 2);
   a.err = device_error_word();
   cudaError_t e;
   if (dtype == DT_F16)
