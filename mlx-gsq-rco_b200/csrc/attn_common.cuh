@@ -189,7 +189,7 @@ __device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float log2_approx(float x) {

@@ -18,12 +18,13 @@
 //     score, and its value scale enters the weight as 2^(s + log2 vs - ref),
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs.
-// Roles (16 warps): 0-3 softmax, one row a thread; 4-11 dequantise; 12 issues
-// (13-15 complete its warpgroup, so that registers can be shared out by role).
-// S_{j+1} is issued before P_j V_j, so the softmax of one tile overlaps the
-// products of its neighbours.  The running maximum is followed lazily: O is
-// rescaled only when a row's reference grows by more than 2^8, which weights
-// of up to 2^14 in fp16 leave room for.
+// Roles (20 warps): two softmax warpgroups that take the tiles in turn, one
+// row a thread; two that dequantise; one warp issues. S of the next two tiles
+// is issued before P V of this one, so that two tiles are in the softmax
+// while the tensor core works on their neighbours; what the two groups share
+// is each row's reference (the running maximum), passed from tile to tile.
+// The reference is followed lazily: O is rescaled only when it grows by more
+// than 2^8, which weights of up to 2^14 in fp16 leave room for.
 // Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded
 // ones, in fp32.  Every wait is bounded.
 #pragma once
@@ -34,15 +35,16 @@
 namespace gsq {
 
 constexpr int AR_M = 128, AR_TILE = 64;
-constexpr int AR_SOFTMAX = 4, AR_DEQUANT = 8;  // warps
-constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // the last warpgroup: one warp issues, three idle
+constexpr int AR_GROUP = 4, AR_SOFTMAX = 2 * AR_GROUP, AR_DEQUANT = 8;  // warps
+constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four one issues, the others end its warpgroup
 
 template <int D>
 struct ArGeom {
   static constexpr int ITEM = AR_TILE * D * 2;  // one K or V tile in fp16
   static constexpr int STAGES = 6;
-  static constexpr int SCALES = AR_SOFTMAX * 3 * AR_TILE * 4;
-  static constexpr int SMEM = 1024 + STAGES * ITEM + SCALES + 256;
+  static constexpr int SCALES = AR_SOFTMAX * 5 * AR_TILE * 4;
+  static constexpr int STATE = 3 * AR_M * 4;    // references, and the two groups' sums
+  static constexpr int SMEM = 1024 + STAGES * ITEM + SCALES + STATE + 512;
   static constexpr int O = 0, Q = D, S = Q + D / 2, P = S + AR_TILE;  // TMEM columns
   static constexpr int COLS = 512;
   static_assert(P + AR_TILE <= COLS && SMEM <= 227 * 1024, "fits");
@@ -181,23 +183,108 @@ __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const S
   return m & below(s.len - p0);
 }
 
+// Scales of two positions of a tile a lane, as the softmax uses them: keys' scales, log2 of the values' and its
+// inverse in linear terms, in the warp's own copy.
+struct ArZeros {
+  uint32_t even, odd;  // bit i: the value scale of position 2i (2i + 1) is 0
+};
+__device__ __forceinline__ ArZeros ar_scales(float* ks, float2 k2, float2 v2) {
+  const int lane = threadIdx.x & 31;
+  // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of scale 0 has
+  // no part in the output, but in the sum of weights: it is weighted with the largest scale of the tile, and that
+  // weight left out of P.
+  float lx = v2.x > 0.f ? fmaxf(log2_approx(v2.x), -100.f) : -INFINITY;
+  float ly = v2.y > 0.f ? fmaxf(log2_approx(v2.y), -100.f) : -INFINITY;
+  const ArZeros z = {__ballot_sync(0xffffffffu, v2.x == 0.f), __ballot_sync(0xffffffffu, v2.y == 0.f)};
+  float top = -40.f;
+  if (z.even | z.odd) {
+    top = fmaxf(lx, ly);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = -40.f;
+  }
+  lx = v2.x > 0.f ? lx : v2.x == 0.f ? top : v2.x;  // NaN stays
+  ly = v2.y > 0.f ? ly : v2.y == 0.f ? top : v2.y;
+  *reinterpret_cast<float2*>(ks + 2 * lane) = k2;
+  *reinterpret_cast<float2*>(ks + AR_TILE + 2 * lane) = make_float2(lx, ly);
+  *reinterpret_cast<float2*>(ks + 2 * AR_TILE + 2 * lane) = make_float2(exp2_approx(-lx), exp2_approx(-ly));
+  return z;
+}
+
+// s: raw scores of a row -> t = factor * ks * s + log2 vs; -inf where a bit of `see` is off (EDGE). Returns the maximum.
+template <bool EDGE>
+__device__ __forceinline__ float ar_scores(float2 (&s)[AR_TILE / 2], const float* ks, float factor, uint64_t see) {
+  const float2 f2 = make_float2(factor, factor);
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int e = 0; e < AR_TILE; e += 4) {
+    const float4 k4 = *reinterpret_cast<const float4*>(ks + e);
+    const float4 v4 = *reinterpret_cast<const float4*>(ks + AR_TILE + e);
+    float2 x = fma2(mul2(s[e / 2], make_float2(k4.x, k4.y)), f2, make_float2(v4.x, v4.y));
+    float2 y = fma2(mul2(s[e / 2 + 1], make_float2(k4.z, k4.w)), f2, make_float2(v4.z, v4.w));
+    if constexpr (EDGE) {
+      x.x = see >> e & 1 ? x.x : -INFINITY;
+      x.y = see >> (e + 1) & 1 ? x.y : -INFINITY;
+      y.x = see >> (e + 2) & 1 ? y.x : -INFINITY;
+      y.y = see >> (e + 3) & 1 ? y.y : -INFINITY;
+    }
+    s[e / 2] = x;
+    s[e / 2 + 1] = y;
+    top[e / 4 % 2] = fmaxf(fmaxf(top[e / 4 % 2], x.x), x.y);
+    top[2 + e / 4 % 2] = fmaxf(fmaxf(top[2 + e / 4 % 2], y.x), y.y);
+  }
+  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// Weights 2^(t + shift) in fp16, and the sum of the unrounded ones over their value scales.
+template <bool EDGE>
+__device__ __forceinline__ float ar_weights(const float2 (&t)[AR_TILE / 2], const float* inv, float shift, uint64_t see,
+                                            uint32_t (&w)[AR_TILE / 2]) {
+  const float2 sh = make_float2(shift, shift);
+  float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < AR_TILE; e += 4) {
+    float2 x = add2(t[e / 2], sh), y = add2(t[e / 2 + 1], sh);
+    x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+    y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+    float4 i4 = *reinterpret_cast<const float4*>(inv + e);
+    if constexpr (EDGE) {  // a hidden position's scale may be NaN
+      i4.x = see >> e & 1 ? i4.x : 0.f;
+      i4.y = see >> (e + 1) & 1 ? i4.y : 0.f;
+      i4.z = see >> (e + 2) & 1 ? i4.z : 0.f;
+      i4.w = see >> (e + 3) & 1 ? i4.w : 0.f;
+    }
+    acc0 = fma2(x, make_float2(i4.x, i4.y), acc0);
+    acc1 = fma2(y, make_float2(i4.z, i4.w), acc1);
+    const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
+    w[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
+    w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+  }
+  acc0 = add2(acc0, acc1);
+  return acc0.x + acc0.y;
+}
+
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs a) {
   using G = ArGeom<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* scales = reinterpret_cast<float*>(smem + G::STAGES * G::ITEM);  // [softmax warp][ks | log2 vs | 1 / vs][64]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::STAGES * G::ITEM + G::SCALES);
+  float* scales = reinterpret_cast<float*>(smem + G::STAGES * G::ITEM);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][64]
+  float* refs = scales + G::SCALES / 4;                                   // [128], base-2 exponents
+  float* sums = refs + AR_M;                                              // [group][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::STAGES * G::ITEM + G::SCALES + G::STATE);
   uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
   uint64_t* empty = full + G::STAGES;     // [STAGES] commit
-  uint64_t* s_full = empty + G::STAGES;   // commit
-  uint64_t* s_free = s_full + 1;          // count AR_SOFTMAX
-  uint64_t* p_full = s_free + 1;          // [2] count AR_SOFTMAX
-  uint64_t* pv_done = p_full + 2;         // [2] commit
+  uint64_t* s_full = empty + G::STAGES;   // [group] commit
+  uint64_t* s_free = s_full + 2;          // count AR_GROUP
+  uint64_t* p_full = s_free + 1;          // [group] count AR_GROUP
+  uint64_t* pv_done = p_full + 2;         // [group] commit
   uint64_t* q_full = pv_done + 2;         // count AR_SOFTMAX
-  uint64_t* drained = q_full + 1;         // commit
+  uint64_t* ref_done = q_full + 1;        // [32 rows] count 1: the references are those of one more tile
+  uint64_t* sum_done = ref_done + 4;      // [32 rows] count 2: both groups' sums are there
+  uint64_t* drained = sum_done + 4;       // commit
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  static_assert((2 * G::STAGES + 8) * 8 + 4 <= 256, "barriers");
+  static_assert((2 * G::STAGES + 17) * 8 + 4 <= 512, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == AR_SOFTMAX + AR_DEQUANT) tmem_alloc(tmem_slot, G::COLS);
@@ -206,13 +293,17 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       mbar_init(&full[i], AR_DEQUANT);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, AR_SOFTMAX);
+    mbar_init(s_free, AR_GROUP);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&p_full[i], AR_SOFTMAX);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], AR_GROUP);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, AR_SOFTMAX);
+    for (int i = 0; i < 4; i++) {
+      mbar_init(&ref_done[i], 1);
+      mbar_init(&sum_done[i], 2);
+    }
     mbar_init(drained, 1);
     fence_mbar_init();
   }
@@ -234,20 +325,22 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
   } else if (warp < AR_SOFTMAX) {
     // ---------------- softmax: thread = row ----------------
-    // of 128 registers a thread at the launch (512 in all): 208 here, 104 for each dequantising warpgroup, 96
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const uint32_t lanes = tmem + ((uint32_t)(32 * warp) << 16);
+    // of 96 registers a thread at the launch (480 in all): 136 for each group here, 80 for each that dequantises, 48
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    const int group = warp / AR_GROUP, quarter = warp % AR_GROUP, row = threadIdx.x % AR_M;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     const int rows = a.n * a.group;
+    float* ks = scales + warp * 5 * AR_TILE;
     ArRun run;
     run.begin(a, first, last);
-    int tile = 0;  // of the CTA
+    int tile = 0, runs = 0;  // of the CTA
     do {
-      const int r = run.at.mb * AR_M + threadIdx.x;  // row of the unit's head
+      const int r = run.at.mb * AR_M + row;  // row of the unit's head
       const int i = r / a.group;
-      // Q: the row in fp16 (bf16: times a power of two), 16 dimensions in 8 columns
-      float amax = 0.f;
+      // Q: the row in fp16 (bf16: times a power of two), 16 dimensions in 8 columns; a half of it by each group
       int shift = 0;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        float amax = 0.f;
 #pragma unroll 4
         for (int d = 0; d < D; d += 8) {
           float f[8];
@@ -260,7 +353,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       const float up = (a.scale < 0.f ? -1.f : 1.f) * exp2_int(shift);
       const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);
 #pragma unroll 1
-      for (int c = 0; c < D / 64; c++) {
+      for (int c = group * (D / 128); c < (group + 1) * (D / 128); c++) {
         uint32_t w[32];
 #pragma unroll
         for (int d = 0; d < 64; d += 8) {
@@ -279,159 +372,127 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
 
-      float2 next_k, next_v;  // scales of positions p, p + 1 of the coming tile; 0 past the end
       const int64_t row0 = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap;
+      // Scales of this group's coming tile, copied while the last one is worked on (loads into registers would be
+      // waited for at the next arrival on a barrier); 0 past the end
       auto fetch_scales = [&](int64_t p0) {
-        const int64_t p = p0 + 2 * lane;
-        const bool in0 = p < run.at.span.len, in1 = p + 1 < run.at.span.len;
-        next_k = make_float2(in0 ? a.ks[row0 + p] : 0.f, in1 ? a.ks[row0 + p + 1] : 0.f);
-        next_v = make_float2(in0 ? a.vs[row0 + p] : 0.f, in1 ? a.vs[row0 + p + 1] : 0.f);
-      };
-      fetch_scales((int64_t)run.at.tile * AR_TILE);
-      float* ks = scales + warp * 3 * AR_TILE;
-
-      float ref = -INFINITY, sum = 0.f;
-      for (int j = 0; j < run.len && ok; j++, tile++) {
-        const int64_t p0 = (int64_t)(run.at.tile + j) * AR_TILE;
-        // the tile's scales, two positions a lane; each warp keeps its own, so that no barrier joins the warps
-        __syncwarp();
-        uint32_t zero_even, zero_odd;  // positions of scale 0, bit i: 2i (2i + 1)
-        {
-          const float2 kv2 = next_k, vv2 = next_v;
-          if (j + 1 < run.len) fetch_scales(p0 + AR_TILE);
-          // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of
-          // scale 0 has no part in the output, but in the sum of weights: it is weighted with the largest scale of
-          // the tile, and that weight left out of P.
-          float lx = vv2.x > 0.f ? fmaxf(log2_approx(vv2.x), -100.f) : -INFINITY;
-          float ly = vv2.y > 0.f ? fmaxf(log2_approx(vv2.y), -100.f) : -INFINITY;
-          float top = fmaxf(lx, ly);
 #pragma unroll
-          for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          if (top == -INFINITY) top = -40.f;
-          zero_even = __ballot_sync(0xffffffffu, vv2.x == 0.f);
-          zero_odd = __ballot_sync(0xffffffffu, vv2.y == 0.f);
-          lx = vv2.x > 0.f ? lx : vv2.x == 0.f ? top : vv2.x;  // NaN stays
-          ly = vv2.y > 0.f ? ly : vv2.y == 0.f ? top : vv2.y;
-          *reinterpret_cast<float2*>(ks + 2 * lane) = kv2;
-          *reinterpret_cast<float2*>(ks + AR_TILE + 2 * lane) = make_float2(lx, ly);
-          *reinterpret_cast<float2*>(ks + 2 * AR_TILE + 2 * lane) = make_float2(exp2_approx(-lx), exp2_approx(-ly));
+        for (int c = 0; c < 4; c++) {
+          const int64_t p = p0 + (c & 1) * 32 + lane;
+          const bool in = p < run.at.span.len;
+          cp_async4_zfill(ks + (3 + c / 2) * AR_TILE + (c & 1) * 32 + lane, (c < 2 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
         }
+        cp_async_commit();
+      };
+      const int run0 = tile;  // the run's first tile
+      if ((tile & 1) != group) tile++;
+      if (tile < run0 + run.len) fetch_scales((int64_t)(run.at.tile + tile - run0) * AR_TILE);
+
+      float ref = -INFINITY, sum = 0.f;  // of the row, as this group knows them
+      for (; tile < run0 + run.len; tile += 2) {
+        const int64_t p0 = (int64_t)(run.at.tile + tile - run0) * AR_TILE;
+        cp_async_wait<0>();
+        __syncwarp();  // this tile's are there, and the warp has read the last tile's
+        const ArZeros zeros = ar_scales(ks, *reinterpret_cast<const float2*>(ks + 3 * AR_TILE + 2 * lane),
+                                        *reinterpret_cast<const float2*>(ks + 4 * AR_TILE + 2 * lane));
         __syncwarp();
-        ok = warp_wait(s_full, (uint32_t)(tile & 1), a.err);
+        if (tile + 2 < run0 + run.len) fetch_scales(p0 + 2 * AR_TILE);
+        ok = warp_wait(&s_full[group], (uint32_t)((tile / 2) & 1), a.err);
         if (!ok) break;
         tc_fence_after();
-        float s[AR_TILE];
+        float2 s[AR_TILE / 2];
         tmem_ld32(lanes + G::S, reinterpret_cast<uint32_t*>(s));
-        tmem_ld32(lanes + G::S + 32, reinterpret_cast<uint32_t*>(s + 32));
+        tmem_ld32(lanes + G::S + 32, reinterpret_cast<uint32_t*>(s) + 32);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
 
-        // t = score + log2 vs, to base 2
-        const float2 f2 = make_float2(factor, factor);
-#pragma unroll
-        for (int e = 0; e < AR_TILE; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(ks + e);
-          const float4 v4 = *reinterpret_cast<const float4*>(ks + AR_TILE + e);
-          const float2 x = fma2(mul2(make_float2(s[e], s[e + 1]), make_float2(k4.x, k4.y)), f2, make_float2(v4.x, v4.y));
-          const float2 y =
-              fma2(mul2(make_float2(s[e + 2], s[e + 3]), make_float2(k4.z, k4.w)), f2, make_float2(v4.z, v4.w));
-          s[e] = x.x;
-          s[e + 1] = x.y;
-          s[e + 2] = y.x;
-          s[e + 3] = y.y;
-        }
         const bool edge = p0 + AR_TILE > min(run.at.span.base, run.at.span.len);  // the same for all threads
-        uint64_t see = ~0ull;
-        if (edge) {
-          see = ar_visible(a, run.at.b, run.at.span, i, p0);
-#pragma unroll
-          for (int e = 0; e < AR_TILE; e++)
-            if (!(see >> e & 1)) s[e] = -INFINITY;
+        const uint64_t see = edge ? ar_visible(a, run.at.b, run.at.span, i, p0) : ~0ull;
+        const float top = edge ? ar_scores<true>(s, ks, factor, see) : ar_scores<false>(s, ks, factor, see);
+        // the reference after the last tile, which the other group has set
+        if (tile > run0) {
+          ok = warp_wait(&ref_done[quarter], (uint32_t)((tile - 1) & 1), a.err);
+          if (!ok) break;
+          const float now = refs[row];
+          if (now != ref) {
+            if (ref != -INFINITY) sum *= exp2_approx(ref - now);
+            ref = now;
+          }
         }
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < AR_TILE; e++) top = fmaxf(top, s[e]);
-        // pv_done[tile & 1] of tile - 2: its P is read, this tile's may be written
-        if (tile >= 2) ok = warp_wait(&pv_done[tile & 1], (uint32_t)((tile / 2 - 1) & 1), a.err);
-        if (!ok) break;
         const bool grow = top > ref + 8.f || (ref == -INFINITY && top > ref);
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? top : ref;
-          const float f = ref == -INFINITY ? 0.f : exp2_approx(ref - next);
-          sum *= ref == next ? 1.f : f;
-          if (j > 0) {
+          const float f = ref == next || ref == -INFINITY ? 1.f : exp2_approx(ref - next);  // no weight yet: 0, or NaN
+          sum *= f;
+          if (tile > run0) {
             // O holds this unit's tiles so far: wait for the last of them and rescale it
             ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
             if (!ok) break;
             tc_fence_after();
-            const float f1 = ref == next || ref == -INFINITY ? 1.f : f;  // no weight yet: O is zero (or NaN, and stays)
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
               uint32_t o[32];
               tmem_ld32(lanes + G::O + c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f1);
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st32(lanes + G::O + c, o);
             }
             tmem_wait_st();
           }
           ref = next;
         }
+        refs[row] = ref;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ref_done[quarter]);
+
         // weights 2^(t - ref + 6), at most 2^14
-        const float shift6 = 6.f - (ref == -INFINITY ? 0.f : ref);
-        const float2 sh = make_float2(shift6, shift6);
         uint32_t w[AR_TILE / 2];
-        float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+        const float lift = 6.f - (ref == -INFINITY ? 0.f : ref);
+        sum += edge ? ar_weights<true>(s, ks + 2 * AR_TILE, lift, see, w)
+                    : ar_weights<false>(s, ks + 2 * AR_TILE, lift, see, w);
+        if (zeros.even | zeros.odd) {
 #pragma unroll
-        for (int e = 0; e < AR_TILE; e += 4) {
-          float2 x = add2(make_float2(s[e], s[e + 1]), sh), y = add2(make_float2(s[e + 2], s[e + 3]), sh);
-          x.x = exp2_approx(x.x);
-          x.y = exp2_approx(x.y);
-          y.x = exp2_approx(y.x);
-          y.y = exp2_approx(y.y);
-          float4 i4 = *reinterpret_cast<const float4*>(ks + 2 * AR_TILE + e);
-          if (edge) {  // a hidden position's scale may be NaN
-            i4.x = see >> e & 1 ? i4.x : 0.f;
-            i4.y = see >> (e + 1) & 1 ? i4.y : 0.f;
-            i4.z = see >> (e + 2) & 1 ? i4.z : 0.f;
-            i4.w = see >> (e + 3) & 1 ? i4.w : 0.f;
-          }
-          acc0 = fma2(x, make_float2(i4.x, i4.y), acc0);
-          acc1 = fma2(y, make_float2(i4.z, i4.w), acc1);
-          if (zero_even | zero_odd) {
-            x.x = zero_even >> (e / 2) & 1 ? 0.f : x.x;
-            x.y = zero_odd >> (e / 2) & 1 ? 0.f : x.y;
-            y.x = zero_even >> (e / 2 + 1) & 1 ? 0.f : y.x;
-            y.y = zero_odd >> (e / 2 + 1) & 1 ? 0.f : y.y;
-          }
-          const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
-          w[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-          w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
+          for (int e = 0; e < AR_TILE / 2; e++)
+            w[e] &= (zeros.even >> e & 1 ? 0u : 0xffffu) | (zeros.odd >> e & 1 ? 0u : 0xffff0000u);
         }
-        acc0 = add2(acc0, acc1);
-        sum += acc0.x + acc0.y;
-        tmem_st32(lanes + G::P + (tile & 1) * (AR_TILE / 2), w);
+        if (tile >= 2) {  // this group's last P has been read
+          ok = warp_wait(&pv_done[group], (uint32_t)((tile / 2 - 1) & 1), a.err);
+          if (!ok) break;
+        }
+        tmem_st32(lanes + G::P + group * (AR_TILE / 2), w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[tile & 1]);
+        if (lane == 0) mbar_arrive(&p_full[group]);
       }
       if (!ok) break;
 
-      // ---- the unit's (or its part's) result ----
-      ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
+      // ---- the unit's (or its part's) result: the columns' halves by the two groups ----
+      const int end = run0 + run.len - 1;  // the run's last tile
+      tile = end + 1;
+      ok = warp_wait(&ref_done[quarter], (uint32_t)(end & 1), a.err);
       if (!ok) break;
+      const float now = refs[row];
+      if (now != ref && ref != -INFINITY) sum *= exp2_approx(ref - now);
+      ref = now;
+      sums[group * AR_M + row] = sum;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sum_done[quarter]);
+      ok = warp_wait(&sum_done[quarter], (uint32_t)(runs++ & 1), a.err) &&
+           warp_wait(&pv_done[end & 1], (uint32_t)((end / 2) & 1), a.err);
+      if (!ok) break;
+      sum = sums[row] + sums[AR_M + row];
       tc_fence_after();
       const int slot = 2 * blockIdx.x + (run.t == first ? 0 : 1);
       const bool live = r < rows;
       const bool none = sum == 0.f || i >= run.at.span.count;
       const float inv = none ? 0.f : 1.f / sum;
-      float* part = a.part + ((int64_t)slot * AR_M + threadIdx.x) * D;
+      float* part = a.part + ((int64_t)slot * AR_M + row) * D;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
+      for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += 32) {
         uint32_t o[32];
         tmem_ld32(lanes + G::O + c, o);
         tmem_wait_ld();
@@ -450,15 +511,15 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
             *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
-      if (live && !run.whole)
-        *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * AR_M + threadIdx.x) * 2) = make_float2(ref, sum);
+      if (live && !run.whole && group == 0)
+        *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * AR_M + row) * 2) = make_float2(ref, sum);
       tc_fence_before();  // the loads of O come before the next unit's products (through q_full)
     } while (run.next(a));
   } else if (warp < AR_SOFTMAX + AR_DEQUANT) {
-    // ---------------- dequantise: items in the order K0, K1, V0, K2, V1, .. of each run ----------------
+    // ---------------- dequantise: items in the order K0, K1, K2, V0, K3, V1, .. of each run ----------------
     // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
     // swizzled row. Rows of one lane differ by multiples of 8, so its swizzle is a constant.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int w = warp - AR_SOFTMAX;
     constexpr int LPR = D / 8;               // lanes per row
     constexpr int RPW = 32 / LPR;            // rows per warp and step
@@ -473,7 +534,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     // Loads the next item's codes; zeros past the sequence's end.
     auto load = [&](uint2 (&c)[STEPS]) {
       if (!more) return;
-      const bool key = kpos < run.len && kpos - vpos < 2;
+      const bool key = kpos < run.len && kpos - vpos < 3;
       const int j = key ? kpos++ : vpos++;
       const int64_t p0 = (int64_t)(run.at.tile + j) * AR_TILE + row;
       const int64_t left = run.at.span.len - p0;
@@ -503,10 +564,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           codes_to_half2<FMT>(ahead[h][i].y, v.z, v.w);
           *reinterpret_cast<uint4*>(p + i * 8 * RPW * 128) = v;
         }
-        load(ahead[h]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[stage]);
+        load(ahead[h]);  // after the arrival, which as a release waits for the loads before it
         if (++stage == G::STAGES) {
           stage = 0;
           use++;
@@ -514,7 +575,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == AR_SOFTMAX + AR_DEQUANT) {
     // ---------------- issue ----------------
     ArRun run;
@@ -540,7 +601,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, sw128_desc(b + k / 4 * (AR_TILE * 128) + k % 4 * 32),
                         ar_idesc(AR_TILE, false), k != 0);
         tc_commit(&empty[stage]);
-        tc_commit(s_full);
+        tc_commit(&s_full[t & 1]);
       }
       __syncwarp();
       next_item();
@@ -549,8 +610,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       ok = warp_wait(q_full, (uint32_t)(runs++ & 1), a.err);
       if (!ok) break;
       scores(tile);
+      if (ok && run.len > 1) scores(tile + 1);
       for (int j = 0; j < run.len && ok; j++, tile++) {
-        if (j + 1 < run.len) scores(tile + 1);
+        if (j + 2 < run.len) scores(tile + 2);
         ok = ok && warp_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
              warp_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
         if (!ok) break;
