@@ -2,10 +2,9 @@
 // the sequences' lengths and the order of their work, dequantisation.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "gsq_common.cuh"
 #include "gsq_kv.h"
+#include "kv_codes.cuh"
 
 namespace gsq {
 
@@ -169,24 +168,6 @@ struct TileList {
   __device__ static int cta_of(int t, int total, int ctas) { return (int)((((int64_t)t + 1) * ctas - 1) / total); }
 };
 
-// Four codes as two half2, in order (c0, c1), (c2, c3).  int8: 0x64cc is 1024 + cc, so a code biased by 128 minus
-// 1152 is the code.  e4m3 is a subset of fp16.  Both exact.
-template <int FMT>
-__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (FMT == KV_INT8) {
-    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
-    w ^= 0x80808080u;
-    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
-        : "=r"(lo), "=r"(hi) : "r"(w));
-  }
-}
-
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -198,15 +179,15 @@ __device__ __forceinline__ float log2_approx(float x) {
   return y;
 }
 
-// Output row r (token r / group, head r % group) of a unit, values d, d + 1.
+// Output row r (token r / group, head r % group) of a unit, values d, d + 1, times the gate's sigmoid.
+__device__ __forceinline__ float2 load_gate2(const AttnArgs& a, int b, int kh, int r, int d) {
+  const float* g = a.gate + b * a.gb + r / a.group * a.gn + (kh * a.group + r % a.group) * a.gh + d;
+  return make_float2(g[0], g[1]);
+}
+__device__ __forceinline__ float sigmoid(float x) { return 1.f / (1.f + __expf(-x)); }
 template <typename T>
 __device__ __forceinline__ void store_row2(const AttnArgs& a, int b, int kh, int r, int d, float x, float y) {
   const int i = r / a.group, h = kh * a.group + r % a.group;
-  if (a.gate) {
-    const float* g = a.gate + b * a.gb + i * a.gn + h * a.gh + d;
-    x /= 1.f + __expf(-g[0]);
-    y /= 1.f + __expf(-g[1]);
-  }
   T* o = static_cast<T*>(a.out) + (((int64_t)b * a.n + i) * a.heads + h) * a.dim + d;
   if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(o) = __floats2half2_rn(x, y);
   else *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(x, y);

@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 #pragma unroll 4
         for (int d = 0; d < D; d += 8) {
           float f[8];
-          load_q8<T>(a, run.at.b, run.at.kh, r, d, f);
+          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r, d), f);
 #pragma unroll
           for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(f[e]));
         }
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 #pragma unroll
         for (int d = 0; d < 64; d += 8) {
           float f[8];
-          load_q8<T>(a, run.at.b, run.at.kh, r, 64 * c + d, f);
+          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r, 64 * c + d), f);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const __half2 h = __floats2half2_rn(f[2 * e] * up, f[2 * e + 1] * up);

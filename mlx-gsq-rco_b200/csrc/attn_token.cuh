@@ -38,12 +38,11 @@ struct AtGeom {
   static constexpr int ROWS = 8 * NT;
   static constexpr int STAGE = 2 * 16 * D + 2 * 16 * 4;  // K, V, scales of 16 positions
   static constexpr int STAGES = D == 256 ? 3 : 6;
-  static constexpr int BUF = ROWS * D * 4;                // one warp's sums
-  static constexpr int BUFS = NT == 1 ? 2 : 1;
   static constexpr int RING = AT_WARPS * STAGES * STAGE;
   static constexpr int STAT = AT_WARPS * ROWS * 2 * 4;
   static constexpr int QFRAG = NT == 1 ? 0 : D / 16 * 32 * 8 * NT;
-  static constexpr int SMEM = RING + BUFS * BUF + STAT + QFRAG;
+  static constexpr int SMEM = RING + STAT + QFRAG;
+  static_assert(STAGE >= 8 * D * 4, "a stage holds the sums of eight rows");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -77,19 +76,18 @@ struct AtShape {  // all rows of a head together
 };
 using AtList = TileList<AtShape>;
 
-// One row's eight values of q from dimension d on, in fp32.
+// One row's eight values of q from dimension d on; zeros for rows that are not there.
 template <typename T>
-__device__ __forceinline__ void load_q8(const AttnArgs& a, int b, int kh, int r, int d, float (&f)[8]) {
-  if (r < a.n * a.group) {
-    const T* p = static_cast<const T*>(a.q) + b * a.qb + (r / a.group) * a.qn + (kh * a.group + r % a.group) * a.qh + d;
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&v);
+__device__ __forceinline__ uint4 load_q8(const AttnArgs& a, int b, int kh, int r, int d) {
+  if (r >= a.n * a.group) return make_uint4(0u, 0u, 0u, 0u);
+  return *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qb + (r / a.group) * a.qn +
+                                         (kh * a.group + r % a.group) * a.qh + d);
+}
+template <typename T>
+__device__ __forceinline__ void q8_values(const uint4& v, float* f) {
+  const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = 0.f;
-  }
+  for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
 }
 
 // bf16 queries are held in fp16 times a power of two that brings the row's largest value to [2^13, 2^14): exact but
@@ -110,9 +108,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * G::STAGES * G::STAGE;
-  float* buf = reinterpret_cast<float*>(smem + G::RING);
-  float* stat = reinterpret_cast<float*>(smem + G::RING + G::BUFS * G::BUF);  // [warp][row][m, l]
-  uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::BUFS * G::BUF + G::STAT);
+  float* stat = reinterpret_cast<float*>(smem + G::RING);  // [warp][row][m, l]
+  uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::STAT);
 
   const int total = AtList::total(a), ctas = min(a.ctas, total);
   if ((int)blockIdx.x >= ctas) {
@@ -156,6 +153,15 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
   float factor[NT][2];  // of the scores of rows 8x + 2t, 8x + 2t + 1, to base 2
   int lim[NT][2];       // tree: prefix ends; causal: positions the row sees (relative to the prefix end)
   float o[MT][NT][4], m[NT][2], l[NT][2];
+  uint4 raw[NT][2 * CH];  // q of the coming unit: row 8x + g, dimensions 64c + 16t ..
+  auto fetch_q = [&]() {
+#pragma unroll
+    for (int x = 0; x < NT; x++)
+#pragma unroll
+      for (int c = 0; c < 2 * CH; c++)
+        raw[x][c] = load_q8<T>(a, use.b, use.kh, 8 * x + g, 64 * (c / 2) + 16 * t + 8 * (c % 2));
+  };
+  fetch_q();
 
   for (int tile = first; tile < last;) {
     // ---- a unit's run of tiles ----
@@ -164,22 +170,16 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
     const bool whole = use.tile == 0 && tile + use.tiles <= last;
     const int slot = 2 * blockIdx.x + (tile == first ? 0 : 1);
     const int end = min(last, tile + use.tiles - use.tile);
-    if constexpr (NT > 1) __syncthreads();  // qfrag is free
 #pragma unroll
     for (int x = 0; x < NT; x++) {
       float amax = 0.f;
       float qv[CH][16];
 #pragma unroll
       for (int c = 0; c < CH; c++) {
-        float lo[8], hi[8];
-        load_q8<T>(a, b, kh, 8 * x + g, 64 * c + 16 * t, lo);
-        load_q8<T>(a, b, kh, 8 * x + g, 64 * c + 16 * t + 8, hi);
+        q8_values<T>(raw[x][2 * c], qv[c]);
+        q8_values<T>(raw[x][2 * c + 1], qv[c] + 8);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          qv[c][e] = lo[e];
-          qv[c][8 + e] = hi[e];
-          amax = fmaxf(amax, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-        }
+        for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(qv[c][e]));
       }
       int shift = 0;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -351,79 +351,90 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
       }
     }
 
-    // ---- join the warps: reference and sum of every row, then the sums, two warps (or one) at a time ----
+    // ---- join the warps. Each puts its sums into the stage it has just read, in the fragments' order with the lanes
+    // exchanged by the tile, and warp w adds the eight warps' up for dimensions 16w .. of every 128: lane (jj, tt) for
+    // dimensions 2jj, 2jj + 1 of rows 2tt, 2tt + 1, free of conflicts on both sides.
+    const int tt = lane & 3, jj = lane >> 2;
+    float2 gate[NT][2][D / 128];
+    if (whole && a.gate) {
+#pragma unroll
+      for (int x = 0; x < NT; x++)
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+          for (int h = 0; h < D / 128; h++) {
+            const int r = 8 * x + 2 * tt + c;
+            gate[x][c][h] = r < rows ? load_gate2(a, b, kh, r, 128 * h + 16 * warp + 2 * jj) : make_float2(0.f, 0.f);
+          }
+    }
 #pragma unroll
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
 #pragma unroll
         for (int i = 4; i < 32; i <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], i);
-        if (g == 0) {
-          stat[(warp * G::ROWS + 8 * x + 2 * t + c) * 2] = m[x][c];
-          stat[(warp * G::ROWS + 8 * x + 2 * t + c) * 2 + 1] = l[x][c];
-        }
+        if (g == 0)
+          *reinterpret_cast<float2*>(stat + (warp * G::ROWS + 8 * x + 2 * t + c) * 2) = make_float2(m[x][c], l[x][c]);
       }
     __syncthreads();
+    const int spare = (tile - 1 - first) % G::STAGES * G::STAGE;
+    float* mine = reinterpret_cast<float*>(ring + spare);
+    const float* all = reinterpret_cast<const float*>(smem + spare);  // warp w's is w * STAGES * STAGE bytes on
+    if (tile < last) AtList::next_unit(a, use);
 #pragma unroll
     for (int x = 0; x < NT; x++) {
-      float f[2];
+      if (x > 0) __syncthreads();  // the stages have been read
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         float top = -INFINITY;
+#pragma unroll
         for (int w = 0; w < AT_WARPS; w++) top = fmaxf(top, stat[(w * G::ROWS + 8 * x + 2 * t + c) * 2]);
-        f[c] = m[x][c] == -INFINITY ? 0.f : exp2_approx(m[x][c] - top);
+        const float f = m[x][c] == -INFINITY ? 1.f : exp2_approx(m[x][c] - top);  // no weight: 0, or NaN
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+          mine[(j * 4 + c) * 32 + (lane ^ (j & 7) << 2)] = o[j][x][c] * f;
+          mine[(j * 4 + c + 2) * 32 + (lane ^ (j & 7) << 2)] = o[j][x][c + 2] * f;
+        }
       }
-#pragma unroll
-      for (int j = 0; j < MT; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[j][x][e] = m[x][e & 1] == -INFINITY ? o[j][x][e] : o[j][x][e] * f[e & 1];
-    }
-#pragma unroll 1
-    for (int round = 0; round < AT_WARPS / G::BUFS; round++) {
-      if (warp / G::BUFS == round) {
-        float* mine = buf + warp % G::BUFS * (G::BUF / 4) + lane;
-#pragma unroll
-        for (int j = 0; j < MT; j++)
-#pragma unroll
-          for (int x = 0; x < NT; x++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float* p = mine + ((j * NT + x) * 4 + e) * 32;
-              *p = round == 0 ? o[j][x][e] : *p + o[j][x][e];
-            }
-      }
+      if (x == NT - 1 && tile < last) fetch_q();  // of the next unit, while this one is joined
       __syncthreads();
-    }
-    for (int i = threadIdx.x; i < rows * (D / 2); i += 32 * AT_WARPS) {
-      const int r = i / (D / 2), d = i % (D / 2) * 2;
-      float top = -INFINITY, sum = 0.f;
-      for (int w = 0; w < AT_WARPS; w++) top = fmaxf(top, stat[(w * G::ROWS + r) * 2]);
-      for (int w = 0; w < AT_WARPS; w++) {
-        const float mw = stat[(w * G::ROWS + r) * 2], lw = stat[(w * G::ROWS + r) * 2 + 1];
-        sum += mw == -INFINITY ? lw : lw * exp2_approx(mw - top);
-      }
-      // dimension d of row r in the fragments' layout
-      const int tt = r % 8 / 2, cc = r % 2, xx = r / 8, hh = d / 128, gg = d / 16 % 8, jj = d % 16 / 2;
-      const float* p = buf + (((8 * hh + jj) * NT + xx) * 4 + cc) * 32 + gg * 4 + tt;
-      float v0 = p[0], v1 = p[64];
-      if constexpr (G::BUFS == 2) {
-        v0 += p[G::BUF / 4];
-        v1 += p[G::BUF / 4 + 64];
-      }
-      v0 *= 0x1p-15f;
-      v1 *= 0x1p-15f;
-      if (whole) {
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const int r = 8 * x + 2 * tt + c;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; w++) top = fmaxf(top, stat[(w * G::ROWS + r) * 2]);
+#pragma unroll
+        for (int w = 0; w < AT_WARPS; w++) {
+          const float2 s = *reinterpret_cast<const float2*>(stat + (w * G::ROWS + r) * 2);
+          sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);
+        }
         const bool none = sum == 0.f || r / a.group >= span.count;
-        const float inv = none ? 0.f : 1.f / sum;
-        store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * inv, none ? 0.f : v1 * inv);
-      } else {
-        *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) = make_float2(v0, v1);
-        if (d == 0)
-          *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * G::ROWS + r) * 2) = make_float2(top, sum);
+        const float inv = none ? 0.f : 0x1p-15f / sum;
+#pragma unroll
+        for (int h = 0; h < D / 128; h++) {
+          const float* p = all + ((8 * h + jj) * 4 + c) * 32 + ((warp ^ jj) << 2 | tt);
+          float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+          for (int w = 0; w < AT_WARPS; w++) {
+            v0 += p[w * (G::STAGES * G::STAGE / 4)];
+            v1 += p[w * (G::STAGES * G::STAGE / 4) + 64];
+          }
+          const int d = 128 * h + 16 * warp + 2 * jj;
+          if (r >= rows) continue;
+          if (whole) {
+            const float f0 = a.gate ? inv * sigmoid(gate[x][c][h].x) : inv, f1 = a.gate ? inv * sigmoid(gate[x][c][h].y) : inv;
+            store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
+          } else {
+            *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) =
+                make_float2(v0 * 0x1p-15f, v1 * 0x1p-15f);
+            if (warp == 0 && h == 0 && jj == 0)
+              *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * G::ROWS + r) * 2) = make_float2(top, sum);
+          }
+        }
       }
     }
-    __syncthreads();  // buf and stat are free
-    if (use.tile == use.tiles && tile < last) AtList::next_unit(a, use);
+    __syncthreads();  // the stages and stat are free
   }
 }
 
@@ -496,8 +507,15 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
       }
       const bool none = sum == 0.f || (r0 + r) / a.group >= j.count;
       const float inv = none ? 0.f : 1.f / sum;
-      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x, none ? 0.f : o.x * inv, none ? 0.f : o.y * inv);
-      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x + 2, none ? 0.f : o.z * inv, none ? 0.f : o.w * inv);
+      if (none) o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float2 g0 = make_float2(inv, inv), g1 = g0;
+      if (a.gate) {
+        const float2 x0 = load_gate2(a, j.b, j.kh, r0 + r, 4 * x), x1 = load_gate2(a, j.b, j.kh, r0 + r, 4 * x + 2);
+        g0 = make_float2(inv * sigmoid(x0.x), inv * sigmoid(x0.y));
+        g1 = make_float2(inv * sigmoid(x1.x), inv * sigmoid(x1.y));
+      }
+      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x, o.x * g0.x, o.y * g0.y);
+      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x + 2, o.z * g1.x, o.w * g1.y);
     }
   }
 }

@@ -1,0 +1,27 @@
+// Codes of the quantised key/value cache as fp16.
+#pragma once
+
+#include "gsq_common.cuh"
+#include "gsq_kv.h"
+
+namespace gsq {
+
+// Four codes as two half2, in order (c0, c1), (c2, c3).  int8: 0x64cc is 1024 + cc, so a code biased by 128 minus
+// 1152 is the code.  e4m3 is a subset of fp16.  Both exact.
+template <int FMT>
+__device__ __forceinline__ void codes_to_half2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (FMT == KV_INT8) {
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    w ^= 0x80808080u;
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
+  } else {
+    asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
+}  // namespace gsq

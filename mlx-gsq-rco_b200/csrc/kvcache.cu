@@ -10,7 +10,8 @@
 //
 // Bound: HBM bytes (input + D + 4 a vector), or the launch for one token.
 // One warp per vector: the whole vector sits in the warp's registers (D / 32
-// values a lane), so the maximum is five shuffles and nothing is read twice.
+// values a lane), so nothing is read twice; a warp takes KV_EACH vectors, all
+// loaded before the first is worked on.
 #include <cuda_fp8.h>
 
 #include <cstdio>
@@ -18,13 +19,15 @@
 #include "gsq_common.cuh"
 #include "gsq_host.h"
 #include "gsq_kv.h"
+#include "kv_codes.cuh"
 #include "../../include/gsq_model.h"
 
 using namespace gsq;
 
 namespace {
 
-constexpr int KV_WARPS = 4;
+constexpr int KV_WARPS = 4;  // per CTA
+constexpr int KV_EACH = 2;   // vectors per warp
 
 struct KvArgs {
   const void* src[2];     // k, v (append)
@@ -35,15 +38,16 @@ struct KvArgs {
   const int32_t* start;   // first position of sequence b: start[b * start_stride]
   int64_t start_stride;
   const int32_t* counts;  // tokens of sequence b (null: all)
-  int64_t tokens, heads, cap, vectors;
+  int tokens, heads;
+  int64_t cap;
   int* err;
 };
 
 // Position of vector (b, t) in the cache, or -1: past the sequence's count, or outside the cache.
-__device__ __forceinline__ int64_t kv_position(const KvArgs& a, int64_t b, int64_t t, bool* outside) {
+__device__ __forceinline__ int64_t kv_position(const KvArgs& a, int b, int t, bool* outside) {
   *outside = false;
   if (a.counts && t >= a.counts[b]) return -1;
-  const int64_t p = (int64_t)a.start[b * a.start_stride] + t;
+  const int64_t p = (int64_t)a.start[(int64_t)b * a.start_stride] + t;
   if (p >= 0 && p < a.cap) return p;
   *outside = true;
   return -1;
@@ -70,41 +74,67 @@ __device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
   }
 }
 
-// Codes and scale of the warp's vector, N values a lane.
+// Codes (one byte each, in order) and scale of the warp's vector, N values a lane.
 template <int FMT, int N>
-__device__ __forceinline__ void quantise(const float (&f)[N], uint8_t (&code)[N], float& scale) {
-  float m = 0.f;
-  bool finite = true;
+__device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N / 4], float& scale) {
+  // the largest |x| by its bits, which for Inf and NaN are above every finite number's
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    m = fmaxf(m, fabsf(f[i]));
-    finite = finite && isfinite(f[i]);
-  }
-  finite = __all_sync(0xffffffffu, finite);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int i = 0; i < N; i++) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float m = __uint_as_float(top);
   constexpr float M = FMT == KV_INT8 ? 127.f : 448.f;
   scale = __fmul_rn(m, 1.f / M);
   if (m > 1e38f) scale = fminf(scale, __fdiv_rd(3.402823466e38f, M));  // M * scale stays finite
-  if (!finite) scale = __int_as_float(0x7fffffff);
+  if (top >= 0x7f800000u) scale = __int_as_float(0x7fffffff);
+  // code = nearest of fl(x / scale). x * (1 / scale) is within 2^-22 of that quotient, so where both ends of
+  // +-2^-21 around it have the same nearest code, that is the code, without a division; near a tie, or where the
+  // reciprocal may leave the normal range, it is divided.
+  uint32_t differ = scale > 1e-30f ? 0u : 1u;
+  const float inv = __frcp_rn(scale), up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    const float y = scale > 0.f ? __fdiv_rn(f[i], scale) : 0.f;  // scale 0 (a zero vector) and NaN: code 0
+  for (int i = 0; i < N; i += 4) {
     if constexpr (FMT == KV_INT8) {
-      // a subnormal scale is coarse enough for a quotient past 127
-      code[i] = (uint8_t)(int8_t)(int)rintf(fminf(fmaxf(y, -127.f), 127.f));
+      constexpr float R = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest integer, ties to even
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        u[e] = __float_as_uint(fmaf(f[i + e], up, R));
+        differ |= u[e] ^ __float_as_uint(fmaf(f[i + e], down, R));
+      }
+      code[i / 4] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
     } else {
-      code[i] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+      uint32_t u[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float x = f[i + 2 * e], y = f[i + 2 * e + 1];
+        u[e] = __nv_cvt_float2_to_fp8x2(make_float2(x * up, y * up), __NV_SATFINITE, __NV_E4M3);
+        differ |= u[e] ^ __nv_cvt_float2_to_fp8x2(make_float2(x * down, y * down), __NV_SATFINITE, __NV_E4M3);
+      }
+      code[i / 4] = __byte_perm(u[0], u[1], 0x5410);
+    }
+  }
+  if (differ) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float y = scale > 0.f ? __fdiv_rn(f[i + e], scale) : 0.f;  // scale 0 (a zero vector) and NaN: code 0
+        uint32_t c;
+        if constexpr (FMT == KV_INT8)  // a subnormal scale is coarse enough for a quotient past 127
+          c = (uint32_t)(int)rintf(fminf(fmaxf(y, -127.f), 127.f)) & 0xffu;
+        else
+          c = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+        w |= c << 8 * e;
+      }
+      code[i / 4] = w;
     }
   }
 }
 
 template <int N>
-__device__ __forceinline__ void store_codes(uint8_t* p, const uint8_t (&c)[N]) {
-  uint32_t w[N / 4];
-#pragma unroll
-  for (int i = 0; i < N / 4; i++)
-    w[i] = (uint32_t)c[4 * i] | (uint32_t)c[4 * i + 1] << 8 | (uint32_t)c[4 * i + 2] << 16 | (uint32_t)c[4 * i + 3] << 24;
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&w)[N / 4]) {
   if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
   else *reinterpret_cast<uint32_t*>(p) = w[0];
 }
@@ -114,32 +144,33 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_append_kernel(const KvArgs a
   constexpr int N = D / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t u = (int64_t)blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (u >= a.vectors) return;
-  const int which = blockIdx.y;
-  const int64_t h = u % a.heads, t = u / a.heads % a.tokens, b = u / (a.heads * a.tokens);
-  bool outside;
-  const int64_t p = kv_position(a, b, t, &outside);
-  if (p < 0) {
+  const unsigned first = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * KV_EACH;  // token and head
+  const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
+  float f[KV_EACH][N];
+  int64_t row[KV_EACH];  // of codes and scales, or -1
+#pragma unroll
+  for (int i = 0; i < KV_EACH; i++) {
+    row[i] = -1;
+    const unsigned u = first + i;
+    if (u >= (unsigned)(a.tokens * a.heads)) continue;
+    const int t = u / (unsigned)a.heads, h = u % (unsigned)a.heads;
+    bool outside;
+    const int64_t p = kv_position(a, b, t, &outside);
     if (outside && lane == 0 && a.err) atomicExch(a.err, DEV_CACHE_POSITION);
-    return;
+    if (p < 0) continue;
+    row[i] = ((int64_t)b * a.heads + h) * a.cap + p;
+    load_n<T, N, VEC>(
+        static_cast<const T*>(a.src[which]) + b * a.sb[which] + t * a.st[which] + h * a.sh[which] + lane * N, f[i]);
   }
-  float f[N];
-  load_n<T, N, VEC>(static_cast<const T*>(a.src[which]) + b * a.sb[which] + t * a.st[which] + h * a.sh[which] + lane * N,
-                    f);
-  uint8_t code[N];
-  float scale;
-  quantise<FMT, N>(f, code, scale);
-  const int64_t row = (b * a.heads + h) * a.cap + p;
-  store_codes<N>(a.codes[which] + row * D + lane * N, code);
-  if (lane == 0) a.scale[which][row] = scale;
-}
-
-template <int FMT>
-__device__ __forceinline__ float code_value(uint8_t c) {
-  if constexpr (FMT == KV_INT8) return (float)(int8_t)c;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+#pragma unroll
+  for (int i = 0; i < KV_EACH; i++) {
+    if (row[i] < 0) continue;
+    uint32_t code[N / 4];
+    float scale;
+    quantise<FMT, N>(f[i], code, scale);
+    store_codes<N>(a.codes[which] + row[i] * D + lane * N, code);
+    if (lane == 0) a.scale[which][row[i]] = scale;
+  }
 }
 
 // Positions outside the cache, and past a sequence's count, read as zeros.
@@ -148,33 +179,51 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvArgs a) 
   constexpr int N = D / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t u = (int64_t)blockIdx.x * KV_WARPS + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (u >= a.vectors) return;
-  const int which = blockIdx.y;
-  const int64_t h = u % a.heads, t = u / a.heads % a.tokens, b = u / (a.heads * a.tokens);
-  bool outside;
-  const int64_t p = kv_position(a, b, t, &outside);
-  alignas(16) T e[N];
+  const unsigned first = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * KV_EACH, vectors = a.tokens * a.heads;
+  const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
+  uint32_t c[KV_EACH][N / 4];
+  float scale[KV_EACH];
 #pragma unroll
-  for (int i = 0; i < N; i++) e[i] = T(0.f);
-  if (p >= 0) {
-    const int64_t row = (b * a.heads + h) * a.cap + p;
-    const float scale = a.scale[which][row];
-    alignas(8) uint8_t c[N];
+  for (int i = 0; i < KV_EACH; i++) {
+    const unsigned u = first + i;
+    scale[i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < N / 4; e++) c[i][e] = 0u;
+    if (u >= vectors) break;
+    bool outside;
+    const int64_t p = kv_position(a, b, u / (unsigned)a.heads, &outside);
+    if (p < 0) continue;
+    const int64_t row = ((int64_t)b * a.heads + u % (unsigned)a.heads) * a.cap + p;
+    scale[i] = a.scale[which][row];
     const uint8_t* src = a.codes[which] + row * D + lane * N;
-    if constexpr (N == 8) *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(src);
-    else *reinterpret_cast<uint32_t*>(c) = *reinterpret_cast<const uint32_t*>(src);
-#pragma unroll
-    for (int i = 0; i < N; i++) store_out(e, sizeof(T) == 4 ? DT_F32 : std::is_same<T, __half>::value ? DT_F16 : DT_BF16, i,
-                                          code_value<FMT>(c[i]) * scale);
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(src);
+    else c[i][0] = *reinterpret_cast<const uint32_t*>(src);
   }
-  T* dst = static_cast<T*>(a.dst[which]) + u * D + lane * N;
-  constexpr int B = sizeof(T) * N;
-  if constexpr (B == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(e);
-  else
 #pragma unroll
-    for (int i = 0; i < B / 16; i++) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(e)[i];
+  for (int i = 0; i < KV_EACH; i++) {
+    if (first + i >= vectors) break;
+    T* dst = static_cast<T*>(a.dst[which]) + ((int64_t)b * vectors + first + i) * D + lane * N;
+#pragma unroll
+    for (int e = 0; e < N / 4; e++) {
+      uint32_t lo, hi;
+      codes_to_half2<FMT>(c[i][e], lo, hi);
+      float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+      float2 y = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+      x.x *= scale[i];
+      x.y *= scale[i];
+      y.x *= scale[i];
+      y.y *= scale[i];
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(dst)[e] = make_float4(x.x, x.y, y.x, y.y);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(y.x, y.y)};
+        reinterpret_cast<uint2*>(dst)[e] = *reinterpret_cast<const uint2*>(v);
+      } else {
+        const __nv_bfloat162 v[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(y.x, y.y)};
+        reinterpret_cast<uint2*>(dst)[e] = *reinterpret_cast<const uint2*>(v);
+      }
+    }
+  }
 }
 
 int fail(int code, const char* msg) { return set_last_error(code, msg); }
@@ -248,7 +297,7 @@ int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_
   int rc = kv_check("gsq_kv_append", fmt, k_codes, v_codes, k_scale, v_scale, batch, heads, dim, cap);
   if (rc) return rc;
   if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return fail(GSQ_ERR_ARG, "gsq_kv_append: bad dtype");
-  if (tokens < 0 || tokens > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_append: bad token count");
+  if (tokens < 0 || tokens * heads > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_append: bad token count");
   if (batch == 0 || tokens == 0) return GSQ_OK;
   if (!k || !v || !start || !k_strides || !v_strides) return fail(GSQ_ERR_ARG, "gsq_kv_append: null pointer");
   const int64_t size = dtype == DT_F32 ? 4 : 2;
@@ -272,13 +321,11 @@ int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_
   a.start = start;
   a.start_stride = start_stride;
   a.counts = counts;
-  a.tokens = tokens;
-  a.heads = heads;
+  a.tokens = (int)tokens;
+  a.heads = (int)heads;
   a.cap = cap;
-  a.vectors = batch * tokens * heads;
   a.err = device_error_word();
-  if ((a.vectors + KV_WARPS - 1) / KV_WARPS > INT32_MAX) return fail(GSQ_ERR_SIZE, "gsq_kv_append: too many vectors");
-  const dim3 grid((unsigned)((a.vectors + KV_WARPS - 1) / KV_WARPS), 2);
+  const dim3 grid((unsigned)((tokens * heads + KV_WARPS * KV_EACH - 1) / (KV_WARPS * KV_EACH)), (unsigned)batch, 2);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = fmt == KV_INT8 ? (dim == 256 ? append_launch<KV_INT8, 256>(dtype, vec, grid, st, a)
                                                      : append_launch<KV_INT8, 128>(dtype, vec, grid, st, a))
@@ -293,7 +340,7 @@ int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* 
   int rc = kv_check("gsq_kv_read", fmt, k_codes, v_codes, k_scale, v_scale, batch, heads, dim, cap);
   if (rc) return rc;
   if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return fail(GSQ_ERR_ARG, "gsq_kv_read: bad dtype");
-  if (tokens < 0 || tokens > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_read: bad token count");
+  if (tokens < 0 || tokens * heads > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_read: bad token count");
   if (batch == 0 || tokens == 0) return GSQ_OK;
   if (!k || !v || !start) return fail(GSQ_ERR_ARG, "gsq_kv_read: null pointer");
   if (!al16(k) || !al16(v)) return fail(GSQ_ERR_ALIGN, "gsq_kv_read: outputs not 16-byte aligned");
@@ -307,12 +354,10 @@ int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* 
   a.start = start;
   a.start_stride = start_stride;
   a.counts = counts;
-  a.tokens = tokens;
-  a.heads = heads;
+  a.tokens = (int)tokens;
+  a.heads = (int)heads;
   a.cap = cap;
-  a.vectors = batch * tokens * heads;
-  if ((a.vectors + KV_WARPS - 1) / KV_WARPS > INT32_MAX) return fail(GSQ_ERR_SIZE, "gsq_kv_read: too many vectors");
-  const dim3 grid((unsigned)((a.vectors + KV_WARPS - 1) / KV_WARPS), 2);
+  const dim3 grid((unsigned)((tokens * heads + KV_WARPS * KV_EACH - 1) / (KV_WARPS * KV_EACH)), (unsigned)batch, 2);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = fmt == KV_INT8 ? (dim == 256 ? read_launch<KV_INT8, 256>(dtype, grid, st, a)
                                                      : read_launch<KV_INT8, 128>(dtype, grid, st, a))

@@ -6,15 +6,16 @@
 // result is the formula's in any order of evaluation a host would use, and
 // ties go to the lowest token.
 //
-// Bound: HBM bytes, one read and one write of the rows.  A warp takes 32
-// consecutive tokens at a time, one word of each bit mask, so rows of any
-// length and alignment are read in whole sectors; a row is cut into chunks of
-// LG_CHUNK tokens, one CTA each, so that one row still fills the GPU
-// (248320 tokens: 122 CTAs).  The counts of a token are read only where its
-// seen bit is set (some thousand of 248320 tokens).  Biases of a chunk are
-// gathered into shared memory first, duplicates summed in list order by one
-// thread, so no atomic orders the sum.  Each CTA leaves its best token; a
-// second launch (one warp per row) takes the best of them and records it.
+// Bound: HBM bytes, one read and one write of the rows.  A row is cut into
+// chunks of LG_CHUNK tokens, one CTA each, so that one row still fills the GPU
+// (248320 tokens: 122 CTAs).  A thread holds eight tokens, as two 16-byte
+// pieces where every row starts on such a boundary, else one by one in
+// neighbouring lanes.  The penalties run only where a token's seen bit is set
+// (some thousand of 248320 tokens), and only there the counts are read.  Biases
+// of a chunk are gathered into shared memory first, duplicates summed in list
+// order by one thread, so no atomic orders the sum.  Each CTA leaves its best
+// token; a second launch (one warp per row) takes the best of them and
+// records it.
 #include <cstdio>
 
 #include "gsq_common.cuh"
@@ -26,8 +27,7 @@ using namespace gsq;
 namespace {
 
 constexpr int LG_THREADS = 256;
-constexpr int LG_CHUNK = 2048;                          // tokens per CTA
-constexpr int LG_ITERS = LG_CHUNK / LG_THREADS;
+constexpr int LG_CHUNK = 8 * LG_THREADS;  // tokens per CTA
 
 struct LogitsArgs {
   const void* logits;
@@ -62,66 +62,135 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   return k;
 }
 
+// Four tokens from v on, aligned for one load.
 template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* f) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = to_f32(e[i]);
+  }
+}
+
+// VEC: the rows of logits and out start on 16-byte (two-byte types: 8-byte) boundaries, and vocab % 4 == 0.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) {
-  __shared__ float bias[LG_CHUNK];
+  __shared__ __align__(16) float bias[LG_CHUNK];
   __shared__ unsigned long long part[LG_THREADS / 32];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t row = blockIdx.y;
-  const int64_t c0 = (int64_t)blockIdx.x * LG_CHUNK;
+  const int vocab = (int)a.vocab, c0 = blockIdx.x * LG_CHUNK;
   const int tid = threadIdx.x, lane = tid & 31;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  float z[LG_ITERS];
-  uint32_t seen[LG_ITERS], allowed[LG_ITERS];
+  const int32_t* seen_row = a.seen ? a.seen + row * a.words : nullptr;
+  const int32_t* allowed_row = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  // token e of this thread, and its bits of the masks (bit e), one word for 4 tokens of 8 lanes or 1 of 32
+  auto token = [&](int e) { return VEC ? c0 + e / 4 * (4 * LG_THREADS) + 4 * tid + e % 4 : c0 + e * LG_THREADS + tid; };
+  alignas(16) float z[8] = {};
+  uint32_t seen = 0, allowed = 0xffu;
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < LG_ITERS; i++) {
-    const int64_t v = c0 + i * LG_THREADS + tid;
-    const bool in = v < a.vocab;
-    z[i] = in ? to_f32(x[v]) : 0.f;
-    seen[i] = in && a.seen ? (uint32_t)a.seen[row * a.words + (v >> 5)] : 0u;
-    allowed[i] = in && a.allowed ? (uint32_t)a.allowed[row * a.allowed_stride + (v >> 5)] : 0xffffffffu;
+    for (int i = 0; i < 2; i++) {
+      const int v = token(4 * i);
+      if (v < vocab) {
+        load4(x + v, z + 4 * i);
+        if (seen_row) seen |= ((uint32_t)seen_row[v >> 5] >> (v & 31) & 15u) << 4 * i;
+        if (allowed_row) allowed &= ((uint32_t)allowed_row[v >> 5] >> (v & 31) & 15u) << 4 * i | 15u << 4 * (1 - i);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const int v = token(e);
+      if (v < vocab) {
+        z[e] = to_f32(x[v]);
+        if (seen_row) seen |= ((uint32_t)seen_row[v >> 5] >> lane & 1u) << e;
+        if (allowed_row && !((uint32_t)allowed_row[v >> 5] >> lane & 1u)) allowed &= ~(1u << e);
+      }
+    }
   }
   if (a.biases) {
-    for (int i = tid; i < LG_CHUNK; i += LG_THREADS) bias[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) reinterpret_cast<float4*>(bias)[tid + i * LG_THREADS] = make_float4(0.f, 0.f, 0.f, 0.f);
     __syncthreads();
     const int32_t* ids = a.bias_ids + row * a.biases;
     const float* val = a.bias_values + row * a.biases;
-    for (int64_t i = tid; i < a.biases; i += LG_THREADS) {
-      const int32_t id = ids[i];
-      if (id < c0 || id >= c0 + LG_CHUNK || id >= a.vocab) continue;
+    const int n = (int)a.biases;
+    for (int i = tid; i < n; i += LG_THREADS) {
+      const int id = ids[i];
+      if (id < c0 || id - c0 >= LG_CHUNK || id >= vocab) continue;
       bool first = true;
-      for (int64_t j = 0; j < i && first; j++) first = ids[j] != id;
+      for (int j = 0; j < i && first; j++) first = ids[j] != id;
       if (!first) continue;
       float s = 0.f;
-      for (int64_t j = i; j < a.biases; j++)
+      for (int j = i; j < n; j++)
         if (ids[j] == id) s = __fadd_rn(s, val[j]);
       bias[id - c0] = s;
     }
     __syncthreads();
   }
-  const float rep = a.repetition ? a.repetition[row] : 1.f;
-  const float freq = a.frequency ? a.frequency[row] : 0.f;
-  const float pres = a.presence ? a.presence[row] : 0.f;
-  unsigned long long best = 0;
+  if (seen) {
+    const float rep = a.repetition ? a.repetition[row] : 1.f;
+    const float freq = a.frequency ? a.frequency[row] : 0.f;
+    const float pres = a.presence ? a.presence[row] : 0.f;
 #pragma unroll
-  for (int i = 0; i < LG_ITERS; i++) {
-    const int64_t v = c0 + i * LG_THREADS + tid;
-    if (v >= a.vocab) continue;
-    float y = z[i];
-    if (seen[i] >> lane & 1) {
-      y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-      const int32_t n = a.counts[row * a.vocab + v];
-      if (n > 0) {
-        y = __fsub_rn(y, __fmul_rn(freq, (float)n));
-        y = __fsub_rn(y, pres);
+    for (int e = 0; e < 8; e++) {
+      if (seen >> e & 1) {
+        float y = z[e];
+        y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+        const int32_t n = a.counts[row * vocab + token(e)];
+        if (n > 0) {
+          y = __fsub_rn(y, __fmul_rn(freq, (float)n));
+          y = __fsub_rn(y, pres);
+        }
+        z[e] = y;
       }
     }
-    if (a.biases) y = __fadd_rn(y, bias[i * LG_THREADS + tid]);
-    if (!(allowed[i] >> lane & 1)) y = -INFINITY;
-    a.out[row * a.vocab + v] = y;
-    const unsigned long long k = (unsigned long long)order_key(y) << 32 | (uint32_t)~(uint32_t)v;
-    best = k > best ? k : best;
+  }
+  if (a.biases) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = __fadd_rn(z[e], bias[token(e) - c0]);
+  }
+  if (allowed != 0xffu) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = allowed >> e & 1 ? z[e] : -INFINITY;
+  }
+  float* out = a.out + row * vocab;
+  // the thread's best token: tokens rise with e, so those past the end come after the others
+  if (c0 + LG_CHUNK > vocab) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) z[e] = token(e) < vocab ? z[e] : -INFINITY;
+  }
+  float top = z[0];
+  bool nan = isnan(z[0]);
+#pragma unroll
+  for (int e = 1; e < 8; e++) {
+    top = fmaxf(top, z[e]);
+    nan = nan || isnan(z[e]);
+  }
+  int at = 0;
+  if (nan) {
+#pragma unroll
+    for (int e = 7; e >= 0; e--) at = isnan(z[e]) ? e : at;
+    top = __int_as_float(0x7fffffff);
+  } else {
+#pragma unroll
+    for (int e = 7; e >= 0; e--) at = z[e] == top ? e : at;
+  }
+  unsigned long long best = 0;
+  if (token(at) < vocab) best = (unsigned long long)order_key(top) << 32 | (uint32_t)~(uint32_t)token(at);
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      if (token(4 * i) < vocab) *reinterpret_cast<float4*>(out + token(4 * i)) = *reinterpret_cast<const float4*>(z + 4 * i);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (token(e) < vocab) out[token(e)] = z[e];
   }
   best = warp_max(best);
   if (lane == 0) part[tid >> 5] = best;
@@ -178,6 +247,12 @@ int launched(cudaError_t rc, const char* what) {
   return fail(GSQ_ERR_CUDA, buf);
 }
 
+template <typename T>
+cudaError_t adjust_launch(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
+  return vec ? launch_pdl(adjust_kernel<T, true>, grid, dim3(LG_THREADS), 0, st, a)
+             : launch_pdl(adjust_kernel<T, false>, grid, dim3(LG_THREADS), 0, st, a);
+}
+
 int64_t chunks_of(int64_t vocab) { return (vocab + LG_CHUNK - 1) / LG_CHUNK; }
 bool al4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
@@ -231,10 +306,13 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
   a.best = static_cast<unsigned long long*>(workspace);
   a.record = record;
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)a.chunks, (unsigned)rows), block(LG_THREADS);
-  cudaError_t e = dtype == DT_F32   ? launch_pdl(adjust_kernel<float>, grid, block, 0, st, a)
-                  : dtype == DT_F16 ? launch_pdl(adjust_kernel<__half>, grid, block, 0, st, a)
-                                    : launch_pdl(adjust_kernel<__nv_bfloat16>, grid, block, 0, st, a);
+  const dim3 grid((unsigned)a.chunks, (unsigned)rows);
+  const size_t size = dtype == DT_F32 ? 4 : 2;
+  const bool vec = vocab % 4 == 0 && row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  cudaError_t e = dtype == DT_F32   ? adjust_launch<float>(vec, grid, st, a)
+                  : dtype == DT_F16 ? adjust_launch<__half>(vec, grid, st, a)
+                                    : adjust_launch<__nv_bfloat16>(vec, grid, st, a);
   if (e == cudaSuccess) e = launch_pdl(pick_kernel, dim3((unsigned)rows), dim3(32), 0, st, a);
   return launched(e, "gsq_adjust_logits");
 }

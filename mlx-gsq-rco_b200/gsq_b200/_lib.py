@@ -136,27 +136,24 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-class on_device:
-    """Makes ``device`` the current one for a launch (a launch goes to the
-    current device's context), at no cost where it is already."""
-
-    __slots__ = ("_index", "_before")
-
-    def __init__(self, device: torch.device):
-        self._index = device.index
-
-    def __enter__(self):
-        self._before = torch.cuda.current_device()
-        if self._before != self._index:
-            torch.cuda.set_device(self._index)
-
-    def __exit__(self, *exc):
-        if self._before != self._index:
-            torch.cuda.set_device(self._before)
+# The current stream's handle without building a torch.cuda.Stream (2.3 -> 0.1 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def launch(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on ``device``'s current stream, with ``device``
+    current (a launch goes to the current device's context)."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, stream_ptr(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_ptr(device)))
 
 
 class _Workspaces:

@@ -6,13 +6,13 @@ tokens; the formula is in ``include/gsq_model.h`` (``gsq_cached_attention``).
 """
 from __future__ import annotations
 
-import math
-
 import numpy as np
 import torch
 
 from ... import _lib
-from .kvcache import Strides, check_counts, check_start
+from .kvcache import check_counts, check_start, strides3
+
+_WORKSPACE_BYTES: dict[tuple, int] = {}  # gsq_cached_attention_workspace_size per shape: a pure function of it
 
 
 def tree_mask(parents, device="cuda") -> torch.Tensor:
@@ -68,7 +68,6 @@ def cached_attention(q: torch.Tensor, cache, start: torch.Tensor, *, counts: tor
     qs = q.stride()
     if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() % 16:
         q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)
-        qs = q.stride()
     tree_ptr, tree_stride = None, 0
     if tree is not None:
         if tree.dtype != torch.int32:
@@ -89,19 +88,21 @@ def cached_attention(q: torch.Tensor, cache, start: torch.Tensor, *, counts: tor
             raise RuntimeError("tensors on different devices")
         if gate.stride(3) != 1:
             gate = gate.contiguous()
-        gate_ptr, gate_strides = gate.data_ptr(), Strides(*gate.stride()[:3])
+        gate_ptr, gate_strides = gate.data_ptr(), strides3(gate)
     if out is None:
-        out = torch.empty((batch, n, heads, dim), dtype=q.dtype, device=dev)
+        out = q.new_empty((batch, n, heads, dim))
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
     lib = _lib.load()
-    with _lib.on_device(dev):
-        need = lib.gsq_cached_attention_workspace_size(batch, n, heads, cache.heads, dim, cache.length)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.gsq_cached_attention(
-            q.data_ptr(), _lib.DTYPE_CODES[q.dtype], Strides(*qs[:3]), batch, n, heads, cache.heads, dim, cache.fmt,
-            *cache.pointers, cache.length, start.data_ptr(), stride, check_counts(counts, batch, dev), tree_ptr,
-            tree_stride, gate_ptr, gate_strides, 1.0 / math.sqrt(dim) if scale is None else float(scale),
-            out.data_ptr(), ws.data_ptr() if need else None, need, _lib.stream_ptr(dev)))
+    key = (batch, n, heads, cache.heads, dim, cache.length)
+    need = _WORKSPACE_BYTES.get(key)
+    if need is None:
+        need = _WORKSPACE_BYTES[key] = lib.gsq_cached_attention_workspace_size(*key)
+    ws = q.new_empty(need // 2) if need else None  # of two-byte values: new_empty is the cheapest allocation
+    _lib.launch(dev, lib.gsq_cached_attention, q.data_ptr(), _lib.DTYPE_CODES[q.dtype], strides3(q), batch, n, heads,
+                cache.heads, dim, cache.fmt, *cache.pointers, cache.length, start.data_ptr(), stride,
+                None if counts is None else check_counts(counts, batch, dev), tree_ptr, tree_stride, gate_ptr,
+                gate_strides, dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                ws.data_ptr() if need else None, need)
     return out

@@ -12,6 +12,18 @@ import torch
 from ... import _lib
 
 Strides = ctypes.c_int64 * 3
+_STRIDES: dict[tuple, ctypes.Array] = {}
+
+
+def strides3(t: torch.Tensor) -> ctypes.Array:
+    """The first three strides of a 4-dimensional tensor for the C ABI, which only reads them."""
+    key = t.stride()
+    s = _STRIDES.get(key)
+    if s is None:
+        if len(_STRIDES) > 4096:
+            _STRIDES.clear()
+        s = _STRIDES[key] = Strides(*key[:3])
+    return s
 
 
 def check_start(start: torch.Tensor, batch: int, device) -> int:
@@ -61,12 +73,9 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    kc, vc, ks, vs = cache.pointers
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().gsq_kv_append(
-            k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[k.dtype], cache.batch, k.shape[1], cache.heads, cache.dim,
-            Strides(*k.stride()[:3]), Strides(*v.stride()[:3]), start.data_ptr(), stride,
-            check_counts(counts, cache.batch, dev), cache.fmt, kc, vc, ks, vs, cache.length, _lib.stream_ptr(dev)))
+    _lib.launch(dev, _lib.load().gsq_kv_append, k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[k.dtype], cache.batch,
+                k.shape[1], cache.heads, cache.dim, strides3(k), strides3(v), start.data_ptr(), stride,
+                check_counts(counts, cache.batch, dev), cache.fmt, *cache.pointers, cache.length)
 
 
 def kv_read(cache, start: torch.Tensor, tokens: int, *, counts: torch.Tensor | None = None,
@@ -83,9 +92,7 @@ def kv_read(cache, start: torch.Tensor, tokens: int, *, counts: torch.Tensor | N
     stride = check_start(start, cache.batch, dev)
     shape = (cache.batch, tokens, cache.heads, cache.dim)
     k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().gsq_kv_read(
-            cache.fmt, *cache.pointers, cache.batch, cache.heads, cache.length, cache.dim, start.data_ptr(), stride,
-            check_counts(counts, cache.batch, dev), tokens, k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[dtype],
-            _lib.stream_ptr(dev)))
+    _lib.launch(dev, _lib.load().gsq_kv_read, cache.fmt, *cache.pointers, cache.batch, cache.heads, cache.length,
+                cache.dim, start.data_ptr(), stride, check_counts(counts, cache.batch, dev), tokens, k.data_ptr(),
+                v.data_ptr(), _lib.DTYPE_CODES[dtype])
     return k, v

@@ -10,6 +10,8 @@ import torch
 
 from ... import _lib
 
+_WORKSPACE_BYTES: dict[tuple[int, int], int] = {}  # gsq_adjust_logits_workspace_size per shape: a pure function of it
+
 
 def _per_row(t: torch.Tensor | None, name: str, rows: int, dev) -> int | None:
     if t is None:
@@ -84,15 +86,17 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
         raise ValueError("out must be a contiguous float32 tensor of the logits' shape and device")
     nxt = torch.empty(rows, dtype=torch.int32, device=dev)
     lib = _lib.load()
-    with _lib.on_device(dev):
-        need = lib.gsq_adjust_logits_workspace_size(rows, vocab)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.gsq_adjust_logits(
-            logits.data_ptr(), _lib.DTYPE_CODES[logits.dtype], max(logits.stride(0), vocab), rows, vocab, seen_ptr,
-            counts_ptr, _per_row(repetition, "repetition", rows, dev), _per_row(frequency, "frequency", rows, dev),
-            _per_row(presence, "presence", rows, dev), bias_ids.data_ptr() if biases else None,
-            bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
-            nxt.data_ptr(), int(record), ws.data_ptr() if need else None, need, _lib.stream_ptr(dev)))
+    key = (rows, vocab)
+    need = _WORKSPACE_BYTES.get(key)
+    if need is None:
+        need = _WORKSPACE_BYTES[key] = lib.gsq_adjust_logits_workspace_size(rows, vocab)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.launch(dev, lib.gsq_adjust_logits, logits.data_ptr(), _lib.DTYPE_CODES[logits.dtype],
+                max(logits.stride(0), vocab), rows, vocab, seen_ptr, counts_ptr,
+                _per_row(repetition, "repetition", rows, dev), _per_row(frequency, "frequency", rows, dev),
+                _per_row(presence, "presence", rows, dev), bias_ids.data_ptr() if biases else None,
+                bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
+                nxt.data_ptr(), int(record), ws.data_ptr() if need else None, need)
     return out, nxt
 
 
@@ -108,7 +112,5 @@ def record_tokens(history, tokens: torch.Tensor, *, generated: bool = True) -> N
     if tokens.device != dev:
         raise RuntimeError("tensors on different devices")
     tokens = tokens.contiguous()
-    with _lib.on_device(dev):
-        _lib.check(_lib.load().gsq_record_tokens(
-            tokens.data_ptr(), tokens.shape[1], tokens.shape[0], tokens.shape[1], history.vocab,
-            history.seen.data_ptr(), history.counts.data_ptr(), int(generated), _lib.stream_ptr(dev)))
+    _lib.launch(dev, _lib.load().gsq_record_tokens, tokens.data_ptr(), tokens.shape[1], tokens.shape[0],
+                tokens.shape[1], history.vocab, history.seen.data_ptr(), history.counts.data_ptr(), int(generated))
