@@ -30,7 +30,7 @@
 
 namespace gsq {
 
-constexpr int AT_WARPS = 8;
+constexpr int AT_WARPS = 4;  // of a CTA, two CTAs on an SM: one is read for while the other joins its warps
 constexpr int AT_TILE = 16 * AT_WARPS;
 
 template <int D, int NT>
@@ -43,7 +43,7 @@ struct AtGeom {
   static constexpr int QFRAG = NT == 1 ? 0 : D / 16 * 32 * 8 * NT;
   static constexpr int SMEM = RING + STAT + QFRAG;
   static_assert(STAGE >= 8 * D * 4, "a stage holds the sums of eight rows");
-  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs on an SM");
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -99,7 +99,7 @@ __device__ __forceinline__ int q_shift(float amax) {
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
 template <typename T, int FMT, int D, int NT>
-__global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const AttnArgs a) {
   using G = AtGeom<D, NT>;
   constexpr int CH = D / 64;   // 64-dimension chunks of the first product
   constexpr int MT = D / 16;   // 16-dimension tiles of the second
@@ -352,19 +352,20 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
     }
 
     // ---- join the warps. Each puts its sums into the stage it has just read, in the fragments' order with the lanes
-    // exchanged by the tile, and warp w adds the eight warps' up for dimensions 16w .. of every 128: lane (jj, tt) for
-    // dimensions 2jj, 2jj + 1 of rows 2tt, 2tt + 1, free of conflicts on both sides.
+    // exchanged by the tile, and warp w adds all warps' up for dimensions 16w .. and 64 + 16w .. of every 128: lane
+    // (jj, tt) for dimensions 2jj, 2jj + 1 of rows 2tt, 2tt + 1, free of conflicts on both sides.
+    constexpr int PIECES = D / (16 * AT_WARPS);
     const int tt = lane & 3, jj = lane >> 2;
-    float2 gate[NT][2][D / 128];
+    float2 gate[NT][2][PIECES];
     if (whole && a.gate) {
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-          for (int h = 0; h < D / 128; h++) {
+          for (int i = 0; i < PIECES; i++) {
             const int r = 8 * x + 2 * tt + c;
-            gate[x][c][h] = r < rows ? load_gate2(a, b, kh, r, 128 * h + 16 * warp + 2 * jj) : make_float2(0.f, 0.f);
+            gate[x][c][i] = r < rows ? load_gate2(a, b, kh, r, 16 * (warp + i * AT_WARPS) + 2 * jj) : make_float2(0.f, 0.f);
           }
     }
 #pragma unroll
@@ -412,23 +413,25 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 1) attn_token_kernel(const Attn
         const bool none = sum == 0.f || r / a.group >= span.count;
         const float inv = none ? 0.f : 0x1p-15f / sum;
 #pragma unroll
-        for (int h = 0; h < D / 128; h++) {
-          const float* p = all + ((8 * h + jj) * 4 + c) * 32 + ((warp ^ jj) << 2 | tt);
+        for (int i = 0; i < PIECES; i++) {
+          const int piece = warp + i * AT_WARPS, h = piece / 8;  // dimensions 16 piece ..
+          const float* p = all + ((8 * h + jj) * 4 + c) * 32 + (((piece & 7) ^ jj) << 2 | tt);
           float v0 = 0.f, v1 = 0.f;
 #pragma unroll
           for (int w = 0; w < AT_WARPS; w++) {
             v0 += p[w * (G::STAGES * G::STAGE / 4)];
             v1 += p[w * (G::STAGES * G::STAGE / 4) + 64];
           }
-          const int d = 128 * h + 16 * warp + 2 * jj;
+          const int d = 16 * piece + 2 * jj;
           if (r >= rows) continue;
           if (whole) {
-            const float f0 = a.gate ? inv * sigmoid(gate[x][c][h].x) : inv, f1 = a.gate ? inv * sigmoid(gate[x][c][h].y) : inv;
+            const float f0 = a.gate ? inv * sigmoid(gate[x][c][i].x) : inv;
+            const float f1 = a.gate ? inv * sigmoid(gate[x][c][i].y) : inv;
             store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
           } else {
             *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) =
                 make_float2(v0 * 0x1p-15f, v1 * 0x1p-15f);
-            if (warp == 0 && h == 0 && jj == 0)
+            if (piece == 0 && jj == 0)
               *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * G::ROWS + r) * 2) = make_float2(top, sum);
           }
         }

@@ -40,7 +40,8 @@ Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, i
     p.rows8 = AR_M;
     p.tiles = batch * kv * ((rows + AR_M - 1) / AR_M) * ((cap + AR_TILE - 1) / AR_TILE);
   }
-  p.ctas = (int)(p.tiles < SMS ? p.tiles : SMS);
+  const int64_t most = p.nt ? 2 * SMS : SMS;  // CTAs that run at once
+  p.ctas = (int)(p.tiles < most ? p.tiles : most);
   p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float) + p.ctas * sizeof(Joint);
   return p;
 }
