@@ -28,21 +28,24 @@ struct AttnArgs {
   int ctas, rows8;      // CTAs of the split, rows of a partial result
   int* err;             // device error word
   float *part, *stat;   // [2 * ctas][rows8][dim], [2 * ctas][rows8][2] (max in base 2, sum)
-  struct Joint* joints;  // [ctas]
+  struct Joint* joints;  // [ctas], for the joining launch
+  int cluster;           // CTAs per unit (token kernel by units)
 };
 
-// Cached positions and new tokens of sequence b.
+// Cached positions and new tokens of sequence b. Caches hold at most 2^30 positions, so a start past that sees all of
+// them as cached text, and one below -2^29 leaves no row anything (n <= 65536): within these bounds an int holds
+// every sum and difference of positions.
 struct SeqSpan {
-  int64_t base;  // position of the first new token
-  int count;     // new tokens (0: all rows are padding)
-  int64_t len;   // positions that any of them may see, from 0
+  int base;   // position of the first new token
+  int count;  // new tokens (0: all rows are padding)
+  int len;    // positions that any of them may see, from 0
 };
 
 __device__ __forceinline__ SeqSpan seq_span(const AttnArgs& a, int b) {
   SeqSpan s;
-  s.base = a.start[(int64_t)b * a.start_stride];
+  s.base = min(max(a.start[(int64_t)b * a.start_stride], -(1 << 29)), 1 << 30);
   s.count = a.counts ? min(max(a.counts[b], 0), a.n) : a.n;
-  s.len = s.count > 0 ? min(max(s.base + s.count, (int64_t)0), a.cap) : 0;
+  s.len = s.count > 0 ? min(max(s.base + s.count, 0), (int)a.cap) : 0;
   return s;
 }
 
@@ -60,6 +63,8 @@ struct Place {
 // slots 2 c. parts == 0: CTA c does not begin in a unit's second part.
 struct Joint {
   int parts, b, kh, mb, c0, s0, count, pad;
+  // Slot of part i among the partial results.
+  __device__ int slot(int i) const { return i == 0 ? s0 : 2 * (c0 + i); }
 };
 
 // Shape: blocks(a) row blocks of ROWS rows each; tiles(a, span, mb).
@@ -136,7 +141,8 @@ struct TileList {
       p.tile -= __shfl_sync(0xffffffffu, sum, 31);
     }
   }
-  // What the joining launch has to know of CTA c, which begins with tile t at p (one thread).
+  // What the joining launch has to know of CTA c, which begins with tile t at p (one thread): the unit, if c is the
+  // second that has a part of it.
   __device__ static void note(const AttnArgs& a, int c, int t, const Place& p, int total, int ctas) {
     Joint j = {};
     const int t0 = t - p.tile;

@@ -55,12 +55,12 @@ struct ArShape {  // blocks of 128 rows; with a causal mask an early block sees 
   __device__ static int blocks(const AttnArgs& a) { return (a.n * a.group + AR_M - 1) / AR_M; }
   __device__ static int tiles(const AttnArgs& a, const SeqSpan& s, int mb) {
     if (mb * AR_M / a.group >= s.count) return 0;
-    int64_t len = s.len;
+    int len = s.len;
     if (!a.tree) {
       const int last = min(((mb + 1) * AR_M - 1) / a.group, s.count - 1);
-      len = min(max(s.base + last + 1, (int64_t)0), a.cap);
+      len = min(max(s.base + last + 1, 0), (int)a.cap);
     }
-    return (int)((len + AR_TILE - 1) / AR_TILE);
+    return (len + AR_TILE - 1) / AR_TILE;
   }
 };
 using ArList = TileList<ArShape>;
@@ -164,18 +164,18 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
 }
 
 // Which of positions p0 .. p0 + 63 token i of sequence b sees, as bits.
-__device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const SeqSpan& s, int i, int64_t p0) {
+__device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const SeqSpan& s, int i, int p0) {
   if (i >= s.count) return 0;
-  auto below = [](int64_t k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
+  auto below = [](int k) { return k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1; };
   if (!a.tree) return below(min(s.base + i + 1, s.len) - p0);
-  const int64_t off = p0 - s.base;  // of bit 0 among the new tokens
+  const int off = p0 - s.base;  // of bit 0 among the new tokens
   uint64_t m = below(-off);
   const int32_t* row = a.tree + b * a.tree_stride + (int64_t)i * a.words;
-  const int64_t w0 = off >> 5;  // floor
+  const int w0 = off >> 5;  // floor
 #pragma unroll
   for (int k = 0; k < 3; k++) {
-    const int64_t w = w0 + k;
-    const int shift = (int)(w * 32 - off);  // -31 .. 64
+    const int w = w0 + k;
+    const int shift = w * 32 - off;  // -31 .. 64
     if (w < 0 || w >= a.words || shift >= 64) continue;
     const uint64_t bits = (uint32_t)row[w];
     m |= shift < 0 ? bits >> -shift : bits << shift;
@@ -375,10 +375,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       const int64_t row0 = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap;
       // Scales of this group's coming tile, copied while the last one is worked on (loads into registers would be
       // waited for at the next arrival on a barrier); 0 past the end
-      auto fetch_scales = [&](int64_t p0) {
+      auto fetch_scales = [&](int p0) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          const int64_t p = p0 + (c & 1) * 32 + lane;
+          const int p = p0 + (c & 1) * 32 + lane;
           const bool in = p < run.at.span.len;
           cp_async4_zfill(ks + (3 + c / 2) * AR_TILE + (c & 1) * 32 + lane, (c < 2 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
         }
@@ -386,11 +386,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       };
       const int run0 = tile;  // the run's first tile
       if ((tile & 1) != group) tile++;
-      if (tile < run0 + run.len) fetch_scales((int64_t)(run.at.tile + tile - run0) * AR_TILE);
+      if (tile < run0 + run.len) fetch_scales((run.at.tile + tile - run0) * AR_TILE);
 
       float ref = -INFINITY, sum = 0.f;  // of the row, as this group knows them
       for (; tile < run0 + run.len; tile += 2) {
-        const int64_t p0 = (int64_t)(run.at.tile + tile - run0) * AR_TILE;
+        const int p0 = (run.at.tile + tile - run0) * AR_TILE;
         cp_async_wait<0>();
         __syncwarp();  // this tile's are there, and the warp has read the last tile's
         const ArZeros zeros = ar_scales(ks, *reinterpret_cast<const float2*>(ks + 3 * AR_TILE + 2 * lane),
@@ -536,8 +536,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       if (!more) return;
       const bool key = kpos < run.len && kpos - vpos < 3;
       const int j = key ? kpos++ : vpos++;
-      const int64_t p0 = (int64_t)(run.at.tile + j) * AR_TILE + row;
-      const int64_t left = run.at.span.len - p0;
+      const int p0 = (run.at.tile + j) * AR_TILE + row, left = run.at.span.len - p0;
       const uint8_t* src = (key ? a.kc : a.vc) + (((int64_t)run.at.b * a.kv + run.at.kh) * a.cap + p0) * D + chunk * 8;
 #pragma unroll
       for (int i = 0; i < STEPS; i++)

@@ -24,6 +24,13 @@
 // position, so the rounded weight is 2^15 p vs / 2^ref with a reference per
 // row that follows s + log2(vs): no weight that matters leaves fp16's normal
 // range, whatever the scales.
+//
+// The work is divided in one of two ways.  UNITS: one cluster of 1 to 8 CTAs
+// for a sequence's head, whose CTAs take a share of its positions each and are
+// joined through distributed shared memory; one launch, no scratch.  Else the
+// tiles of all units are split evenly over the CTAs, and a unit that falls
+// into several is joined by a second launch: for long caches, where units of
+// very different length would leave SMs idle.
 #pragma once
 
 #include "attn_common.cuh"
@@ -37,13 +44,14 @@ template <int D, int NT>
 struct AtGeom {
   static constexpr int ROWS = 8 * NT;
   static constexpr int STAGE = 2 * 16 * D + 2 * 16 * 4;  // K, V, scales of 16 positions
-  static constexpr int STAGES = D == 256 ? 3 : 6;
+  static constexpr int CTAS = D == 128 && NT == 1 ? 3 : 2;  // on an SM (registers)
+  static constexpr int STAGES = D == 256 ? 3 : NT == 1 ? 4 : 6;
   static constexpr int RING = AT_WARPS * STAGES * STAGE;
   static constexpr int STAT = AT_WARPS * ROWS * 2 * 4;
   static constexpr int QFRAG = NT == 1 ? 0 : D / 16 * 32 * 8 * NT;
-  static constexpr int SMEM = RING + STAT + QFRAG;
+  static constexpr int SMEM = RING + STAT + QFRAG + ROWS * 2 * 4;
   static_assert(STAGE >= 8 * D * 4, "a stage holds the sums of eight rows");
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs on an SM");
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs on an SM");
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -58,8 +66,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 // 16 (or 4) bytes global -> shared; zeros where !in (the source is not read).
-__device__ __forceinline__ void cp_async16_zfill(void* dst, const void* src, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async4_zfill(void* dst, const void* src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0) : "memory");
@@ -98,8 +109,38 @@ __device__ __forceinline__ int q_shift(float amax) {
 }
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
-template <typename T, int FMT, int D, int NT>
-__global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const AttnArgs a) {
+// Adds another part's (reference, sum) to (top, sum). No position seen: reference -inf, sum 0 (or NaN).
+__device__ __forceinline__ void add_stat(float& top, float& sum, float t2, float s2) {
+  const float next = fmaxf(top, t2);
+  sum = (top == next || top == -INFINITY ? sum : sum * exp2_approx(top - next)) +
+        (t2 == next || t2 == -INFINITY ? s2 : s2 * exp2_approx(t2 - next));
+  top = next;
+}
+// What a part's sums are multiplied with: to the common reference, 1 where it has seen nothing (its sums are 0, or NaN).
+__device__ __forceinline__ float part_factor(float m, float top) { return m == -INFINITY ? 1.f : exp2_approx(m - top); }
+
+// Zeros for rows r0 .. r1 of a unit.
+template <typename T, int D>
+__device__ __forceinline__ void zero_unit(const AttnArgs& a, int b, int kh, int r0, int r1) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int r = r0 + warp; r < r1; r += blockDim.x / 32)
+    for (int d = 2 * lane; d < D; d += 64) store_row2<T>(a, b, kh, r, d, 0.f, 0.f);
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Two floats at the address that p has in this CTA, of CTA `rank` of the cluster.
+__device__ __forceinline__ float2 ld_cluster2(const float* p, int rank) {
+  uint32_t remote;
+  float2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote) : "memory");
+  return v;
+}
+
+template <typename T, int FMT, int D, int NT, bool UNITS>
+__global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token_kernel(const AttnArgs a) {
   using G = AtGeom<D, NT>;
   constexpr int CH = D / 64;   // 64-dimension chunks of the first product
   constexpr int MT = D / 16;   // 16-dimension tiles of the second
@@ -111,43 +152,71 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
   float* stat = reinterpret_cast<float*>(smem + G::RING);  // [warp][row][m, l]
   uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::STAT);
 
-  const int total = AtList::total(a), ctas = min(a.ctas, total);
-  if ((int)blockIdx.x >= ctas) {
-    if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
-    return;
+  int first, last;
+  Place get = {};
+  if constexpr (UNITS) {
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;  // rank == %cluster_ctarank
+    get.b = unit / a.kv;
+    get.kh = unit % a.kv;
+    get.span = seq_span(a, get.b);
+    get.tiles = AtShape::tiles(a, get.span, 0);
+    if (get.tiles == 0) {  // the whole cluster
+      if (rank == 0) zero_unit<T, D>(a, get.b, get.kh, 0, a.n * a.group);
+      return;
+    }
+    get.tile = first = rank * get.tiles / a.cluster;
+    last = (rank + 1) * get.tiles / a.cluster;
+  } else {
+    const int total = AtList::total(a), ctas = min(a.ctas, total);
+    if ((int)blockIdx.x >= ctas) {
+      if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
+      return;
+    }
+    first = AtList::first_of(blockIdx.x, total, ctas);
+    last = AtList::first_of(blockIdx.x + 1, total, ctas);
+    get = AtList::locate(a, first);
+    if (threadIdx.x == 0) AtList::note(a, blockIdx.x, first, get, total, ctas);
   }
-  const int first = AtList::first_of(blockIdx.x, total, ctas), last = AtList::first_of(blockIdx.x + 1, total, ctas);
-  Place get = AtList::locate(a, first), use = get;
-  if (threadIdx.x == 0) AtList::note(a, blockIdx.x, first, get, total, ctas);
+  Place use = get;
   const int rows = a.n * a.group;
 
-  int fetched = first;
+  // A warp's 16 positions of K and V, copied STEP rows at a time, a 16-byte unit a lane.
+  constexpr int U = D / 16, STEP = 32 / U;
+  const uint32_t lane_dst = smem_u32(ring) + lane / U * D + at_unit(lane / U, lane % U) * 16;
+  int fetched = first, put = 0;
   auto fetch = [&]() {
     if (fetched < last) {
-      uint8_t* st = ring + (fetched - first) % G::STAGES * G::STAGE;
-      const int64_t p0 = (int64_t)get.tile * AT_TILE + warp * 16;
+      const uint32_t st = put * G::STAGE;
+      const int p0 = get.tile * AT_TILE + warp * 16, left = get.span.len - p0;  // positions of this warp that exist
       const int64_t row0 = ((int64_t)get.b * a.kv + get.kh) * a.cap + p0;
-      const int64_t left = get.span.len - p0;  // positions of this warp that exist
-      constexpr int U = D / 16;                // units of a row
+      const uint8_t *kp = a.kc + row0 * D + lane * 16, *vp = a.vc + row0 * D + lane * 16;
+      if (left >= 16) {
 #pragma unroll
-      for (int i = 0; i < 16 * U / 32; i++) {
-        const int x = i * 32 + lane, p = x / U, u = x % U;
-        const bool in = p < left;
-        const int64_t src = (row0 + (in ? p : 0)) * D + u * 16;
-        const int dst = p * D + at_unit(p, u) * 16;
-        cp_async16_zfill(st + dst, a.kc + (in ? src : 0), in);
-        cp_async16_zfill(st + 16 * D + dst, a.vc + (in ? src : 0), in);
+        for (int i = 0; i < 16 / STEP; i++) {
+          const uint32_t dst = (lane_dst ^ (i * STEP & 6) << 4) + st + i * STEP * D;
+          cp_async16(dst, kp + i * STEP * D);
+          cp_async16(dst + 16 * D, vp + i * STEP * D);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16 / STEP; i++) {
+          const uint32_t dst = (lane_dst ^ (i * STEP & 6) << 4) + st + i * STEP * D;
+          const bool in = i * STEP + lane / U < left;
+          cp_async16_zfill(dst, in ? kp + i * STEP * D : a.kc, in);
+          cp_async16_zfill(dst + 16 * D, in ? vp + i * STEP * D : a.vc, in);
+        }
       }
-      const int p = lane & 15;
-      const bool in = p < left;
-      cp_async4_zfill(st + 32 * D + lane * 4, (lane < 16 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
-      if (++get.tile == get.tiles && fetched + 1 < last) AtList::next_unit(a, get);
+      const bool in = (lane & 15) < left;
+      cp_async4_zfill(ring + st + 32 * D + lane * 4, (lane < 16 ? a.ks : a.vs) + (in ? row0 + (lane & 15) : 0), in);
+      if (++get.tile == get.tiles && fetched + 1 < last && !UNITS) AtList::next_unit(a, get);
     }
     fetched++;
+    put = put + 1 == G::STAGES ? 0 : put + 1;
     cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < G::STAGES - 1; i++) fetch();
+  int coming = 0, read = 0;  // the stage that is read next, and the one read last, free until the next copy
 
   uint32_t qr[NT == 1 ? MT : 1][2];
   float factor[NT][2];  // of the scores of rows 8x + 2t, 8x + 2t + 1, to base 2
@@ -163,11 +232,11 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
   };
   fetch_q();
 
-  for (int tile = first; tile < last;) {
+  for (int tile = first; tile < last || UNITS;) {
     // ---- a unit's run of tiles ----
     const int b = use.b, kh = use.kh;
     const SeqSpan span = use.span;
-    const bool whole = use.tile == 0 && tile + use.tiles <= last;
+    const bool whole = UNITS ? a.cluster == 1 : use.tile == 0 && tile + use.tiles <= last;
     const int slot = 2 * blockIdx.x + (tile == first ? 0 : 1);
     const int end = min(last, tile + use.tiles - use.tile);
 #pragma unroll
@@ -228,17 +297,19 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
       fetch();
       cp_async_wait<G::STAGES - 1>();
       __syncwarp();
-      const uint8_t* st = ring + (tile - first) % G::STAGES * G::STAGE;
-      const int64_t p0 = (int64_t)use.tile * AT_TILE + warp * 16;
+      const uint8_t* st = ring + coming * G::STAGE;
+      read = coming;
+      coming = coming + 1 == G::STAGES ? 0 : coming + 1;
+      const int p0 = use.tile * AT_TILE + warp * 16;
       use.tile++;
       if (p0 >= span.len) continue;
       const float* sc = reinterpret_cast<const float*>(st + 32 * D);
 
-      float s[NT][4];
+      float s[NT][4], s2[NT][4];  // two chains of products
 #pragma unroll
       for (int x = 0; x < NT; x++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[x][e] = 0.f;
+        for (int e = 0; e < 4; e++) s[x][e] = s2[x][e] = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; c++) {
         const uint4 ka = *reinterpret_cast<const uint4*>(st + g * D + at_unit(g, 4 * c + t) * 16);
@@ -253,10 +324,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
 #pragma unroll
           for (int x = 0; x < NT; x++) {
             if constexpr (NT == 1) {
-              mma_f16(s[x], a0, a1, a2, a3, qr[4 * c + j][0], qr[4 * c + j][1]);
+              mma_f16(j & 1 ? s2[x] : s[x], a0, a1, a2, a3, qr[4 * c + j][0], qr[4 * c + j][1]);
             } else {
               const uint2 q2 = qfrag[((4 * c + j) * NT + x) * 32 + lane];
-              mma_f16(s[x], a0, a1, a2, a3, q2.x, q2.y);
+              mma_f16(j & 1 ? s2[x] : s[x], a0, a1, a2, a3, q2.x, q2.y);
             }
           }
         }
@@ -270,12 +341,12 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
 #pragma unroll
       for (int x = 0; x < NT; x++) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[x][e] *= (e < 2 ? ks0 : ks1) * factor[x][e & 1];
+        for (int e = 0; e < 4; e++) s[x][e] = (s[x][e] + s2[x][e]) * ((e < 2 ? ks0 : ks1) * factor[x][e & 1]);
         if (edge) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int64_t p = p0 + g + (e < 2 ? 0 : 8);
-            const int64_t off = p - span.base;  // index among the new tokens
+            const int p = p0 + g + (e < 2 ? 0 : 8);
+            const int off = p - span.base;  // index among the new tokens
             bool see = p < span.len;
             if (off >= 0 && see) {
               const int i = lim[x][e & 1];
@@ -378,10 +449,15 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
           *reinterpret_cast<float2*>(stat + (warp * G::ROWS + 8 * x + 2 * t + c) * 2) = make_float2(m[x][c], l[x][c]);
       }
     __syncthreads();
-    const int spare = (tile - 1 - first) % G::STAGES * G::STAGE;
+    const int spare = UNITS ? 0 : read * G::STAGE;  // (UNITS: every stage is free at the end)
+    // UNITS: the CTA's sums of rows 8x .., in the last stage of warp x, the same place in every CTA
+    auto result = [&](int x) {
+      return reinterpret_cast<float*>(smem + x * G::STAGES * G::STAGE + (G::STAGES - 1) * G::STAGE);
+    };
+    float* unit_stat = reinterpret_cast<float*>(smem + G::RING + G::STAT + G::QFRAG);
     float* mine = reinterpret_cast<float*>(ring + spare);
     const float* all = reinterpret_cast<const float*>(smem + spare);  // warp w's is w * STAGES * STAGE bytes on
-    if (tile < last) AtList::next_unit(a, use);
+    if (!UNITS && tile < last) AtList::next_unit(a, use);
 #pragma unroll
     for (int x = 0; x < NT; x++) {
       if (x > 0) __syncthreads();  // the stages have been read
@@ -397,7 +473,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
           mine[(j * 4 + c + 2) * 32 + (lane ^ (j & 7) << 2)] = o[j][x][c + 2] * f;
         }
       }
-      if (x == NT - 1 && tile < last) fetch_q();  // of the next unit, while this one is joined
+      if (!UNITS && x == NT - 1 && tile < last) fetch_q();  // of the next unit, while this one is joined
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < 2; c++) {
@@ -428,6 +504,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
             const float f0 = a.gate ? inv * sigmoid(gate[x][c][i].x) : inv;
             const float f1 = a.gate ? inv * sigmoid(gate[x][c][i].y) : inv;
             store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
+          } else if constexpr (UNITS) {
+            *reinterpret_cast<float2*>(result(x) + (2 * tt + c) * D + d) = make_float2(v0, v1);
+            if (piece == 0 && jj == 0) *reinterpret_cast<float2*>(unit_stat + r * 2) = make_float2(top, sum);
           } else {
             *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) =
                 make_float2(v0 * 0x1p-15f, v1 * 0x1p-15f);
@@ -437,88 +516,115 @@ __global__ void __launch_bounds__(32 * AT_WARPS, 2) attn_token_kernel(const Attn
         }
       }
     }
+    if constexpr (UNITS) {
+      if (whole) return;
+      // every CTA of the cluster takes its share of the outputs from all of them
+      cluster_sync_all();
+      const int ctas = a.cluster, rank = blockIdx.x % ctas;
+      for (int i = rank * 32 * AT_WARPS + threadIdx.x; i < rows * (D / 2); i += ctas * 32 * AT_WARPS) {
+        const int r = i / (D / 2), d = i % (D / 2) * 2;
+        float2 s[8], v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          if (k >= ctas) continue;
+          s[k] = ld_cluster2(unit_stat + r * 2, k);
+          v[k] = ld_cluster2(result(r / 8) + r % 8 * D + d, k);
+        }
+        float2 gate2 = a.gate ? load_gate2(a, b, kh, r, d) : make_float2(0.f, 0.f);
+        float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          if (k < ctas) add_stat(top, sum, s[k].x, s[k].y);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          if (k >= ctas) continue;
+          const float f = part_factor(s[k].x, top);
+          x = fmaf(v[k].x, f, x);
+          y = fmaf(v[k].y, f, y);
+        }
+        const bool none = sum == 0.f || r / a.group >= span.count;
+        const float inv = none ? 0.f : 0x1p-15f / sum;
+        const float f0 = a.gate ? inv * sigmoid(gate2.x) : inv, f1 = a.gate ? inv * sigmoid(gate2.y) : inv;
+        store_row2<T>(a, b, kh, r, d, none ? 0.f : x * f0, none ? 0.f : y * f1);
+      }
+      cluster_sync_all();  // no CTA leaves while another may read its shared memory
+      return;
+    }
     __syncthreads();  // the stages and stat are free
   }
 }
 
 // Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the rows
-// that no tile reaches. CTA (c, y): the unit that CTA c noted, rows y, y + gridDim.y, ..; D / 4 threads across a row,
-// the rest over the parts.
+// that no tile reaches. CTA (c, y): the unit that CTA c noted, its rows y, y + gridDim.y, ..; a row's parts over the
+// eight warps, D / 32 values a lane.
 template <typename T, int D, typename Shape>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
-  constexpr int ACROSS = D / 4, DOWN = 256 / ACROSS;
-  __shared__ float4 acc[DOWN][ACROSS];
+  constexpr int NV = D / 32;
+  __shared__ float acc[8][D];
   pdl_launch_dependents();
   pdl_wait();
-  const int rows = a.n * a.group;
-  const int x = threadIdx.x % ACROSS, y = threadIdx.x / ACROSS;
+  const int rows = a.n * a.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.y == 0) {
     const int blocks = Shape::blocks(a);
     for (int i = blockIdx.x; i < a.batch * blocks; i += gridDim.x) {
       const int b = i / blocks, mb = i % blocks;
-      if (Shape::tiles(a, seq_span(a, b), mb)) continue;
-      const int r0 = mb * Shape::ROWS, r1 = min(rows, r0 + Shape::ROWS);
-      for (int kh = 0; kh < a.kv; kh++)
-        for (int r = r0 + y; r < r1; r += DOWN) {
-          store_row2<T>(a, b, kh, r, 4 * x, 0.f, 0.f);
-          store_row2<T>(a, b, kh, r, 4 * x + 2, 0.f, 0.f);
-        }
+      if (Shape::tiles(a, seq_span(a, b), mb) == 0)
+        for (int kh = 0; kh < a.kv; kh++) zero_unit<T, D>(a, b, kh, mb * Shape::ROWS, min(rows, (mb + 1) * Shape::ROWS));
     }
   }
   const Joint j = a.joints[blockIdx.x];
   if (j.parts == 0) return;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? j.s0 : 2 * (j.c0 + i)) * a.rows8; };
   const int r0 = j.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS);
-  for (int r = blockIdx.y; r < count; r += gridDim.y) {
-    // reference and sum of all parts: the warp's lanes take a part each
+  // few parts: a warp has a row to itself
+  const bool alone = j.parts <= 4;
+  const int step = alone ? 1 : 8;
+  for (int r = alone ? blockIdx.y * 8 + warp : blockIdx.y; r < count; r += alone ? gridDim.y * 8 : gridDim.y) {
     float top = -INFINITY, sum = 0.f;
-    for (int i = threadIdx.x & 31; i < j.parts; i += 32) {
-      const float2 s = *reinterpret_cast<const float2*>(a.stat + (slot(i) + r) * 2);
-      const float next = fmaxf(top, s.x);
-      sum = sum * (top == next ? 1.f : exp2_approx(top - next)) +
-            (s.x == -INFINITY || s.x == next ? s.y : s.y * exp2_approx(s.x - next));  // no position seen: 0, or NaN
-      top = next;
+    for (int i = lane; i < j.parts; i += 32) {
+      const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)j.slot(i) * a.rows8 + r) * 2);
+      add_stat(top, sum, s.x, s.y);
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float t2 = __shfl_xor_sync(0xffffffffu, top, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float next = fmaxf(top, t2);
-      sum = (top == next || top == -INFINITY ? sum : sum * exp2_approx(top - next)) +
-            (t2 == next || t2 == -INFINITY ? s2 : s2 * exp2_approx(t2 - next));
-      top = next;
-    }
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int o = 16; o; o >>= 1)
+      add_stat(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
+    float o[NV] = {};
 #pragma unroll 4
-    for (int i = y; i < j.parts; i += DOWN) {
-      const float m = a.stat[(slot(i) + r) * 2], f = m == -INFINITY ? 1.f : exp2_approx(m - top);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + (slot(i) + r) * D + 4 * x);
-      o.x = fmaf(v.x, f, o.x);
-      o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z);
-      o.w = fmaf(v.w, f, o.w);
+    for (int i = alone ? 0 : warp; i < j.parts; i += step) {
+      const int64_t at = (int64_t)j.slot(i) * a.rows8 + r;
+      const float f = part_factor(a.stat[at * 2], top);
+#pragma unroll
+      for (int e = 0; e < NV; e += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + lane * NV + e);
+        o[e] = fmaf(v.x, f, o[e]);
+        o[e + 1] = fmaf(v.y, f, o[e + 1]);
+        o[e + 2] = fmaf(v.z, f, o[e + 2]);
+        o[e + 3] = fmaf(v.w, f, o[e + 3]);
+      }
     }
-    __syncthreads();  // acc is free
-    acc[y][x] = o;
-    __syncthreads();
-    if (y == 0) {
-      for (int i = 1; i < DOWN; i++) {
-        const float4 v = acc[i][x];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
+    if (!alone) {
+#pragma unroll
+      for (int e = 0; e < NV; e += 4)
+        *reinterpret_cast<float4*>(&acc[warp][lane * NV + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 1; w < 8; w++)
+#pragma unroll
+          for (int e = 0; e < NV; e++) o[e] += acc[w][lane * NV + e];
       }
-      const bool none = sum == 0.f || (r0 + r) / a.group >= j.count;
-      const float inv = none ? 0.f : 1.f / sum;
-      if (none) o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float2 g0 = make_float2(inv, inv), g1 = g0;
+      __syncthreads();
+      if (warp) continue;
+    }
+    const bool none = sum == 0.f || (r0 + r) / a.group >= j.count;
+    const float inv = none ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int e = 0; e < NV; e += 2) {
+      float2 f = make_float2(inv, inv);
       if (a.gate) {
-        const float2 x0 = load_gate2(a, j.b, j.kh, r0 + r, 4 * x), x1 = load_gate2(a, j.b, j.kh, r0 + r, 4 * x + 2);
-        g0 = make_float2(inv * sigmoid(x0.x), inv * sigmoid(x0.y));
-        g1 = make_float2(inv * sigmoid(x1.x), inv * sigmoid(x1.y));
+        const float2 x = load_gate2(a, j.b, j.kh, r0 + r, lane * NV + e);
+        f = make_float2(inv * sigmoid(x.x), inv * sigmoid(x.y));
       }
-      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x, o.x * g0.x, o.y * g0.y);
-      store_row2<T>(a, j.b, j.kh, r0 + r, 4 * x + 2, o.z * g1.x, o.w * g1.y);
+      store_row2<T>(a, j.b, j.kh, r0 + r, lane * NV + e, none ? 0.f : o[e] * f.x, none ? 0.f : o[e + 1] * f.y);
     }
   }
 }

@@ -2,6 +2,7 @@
 // (gsq_cached_attention): which kernel, its launches and checks.  The kernels
 // are in attn_token.cuh (few rows per key/value head: the cache's bytes bound
 // it) and attn_rows.cuh (many rows: the tensor core).
+#include <algorithm>
 #include <atomic>
 #include <cstdio>
 
@@ -22,6 +23,7 @@ constexpr int SMS = 148;
 // Which kernel a call takes, over how many CTAs, and its scratch.
 struct Plan {
   int nt;           // 8-row tiles of the token kernel; 0: the row-block kernel
+  int cluster;      // token kernel by units: CTAs of a unit; 0: tiles split evenly
   int ctas, rows8;
   int64_t tiles;    // at most, over all sequences at full length
   size_t workspace;
@@ -40,8 +42,17 @@ Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, i
     p.rows8 = AR_M;
     p.tiles = batch * kv * ((rows + AR_M - 1) / AR_M) * ((cap + AR_TILE - 1) / AR_TILE);
   }
-  const int64_t most = p.nt ? 2 * SMS : SMS;  // CTAs that run at once
+  const int64_t most = p.nt == 0 ? SMS : SMS * (dim == 128 && p.nt == 1 ? 3 : 2);  // CTAs that run at once
   p.ctas = (int)(p.tiles < most ? p.tiles : most);
+  // By units where that fills the GPU's `most` CTA slots, or the cache is short. Units of a long cache may differ by
+  // more than the slots even out, and few units of one need more than 8 CTAs each.
+  if (p.nt && cap <= 8192) {
+    const int64_t units = batch * kv;
+    p.cluster = 1;
+    while (p.cluster < 8 && units * p.cluster * 2 <= most) p.cluster *= 2;
+    p.ctas = (int)(units * p.cluster);
+    return p;
+  }
   p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float) + p.ctas * sizeof(Joint);
   return p;
 }
@@ -57,14 +68,17 @@ cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   return e;
 }
 
-template <typename T, int FMT, int D, int NT>
+template <typename T, int FMT, int D, int NT, bool UNITS>
 cudaError_t token_launch(cudaStream_t st, const AttnArgs& a) {
   static std::atomic<uint64_t> done{0};
   constexpr int smem = AtGeom<D, NT>::SMEM;
-  cudaError_t e = allow_smem(attn_token_kernel<T, FMT, D, NT>, smem, done);
-  if (e == cudaSuccess)
-    e = launch_pdl(attn_token_kernel<T, FMT, D, NT>, dim3((unsigned)a.ctas), dim3(32 * AT_WARPS), smem, st, a);
+  auto kernel = attn_token_kernel<T, FMT, D, NT, UNITS>;
+  cudaError_t e = allow_smem(kernel, smem, done);
   if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)a.ctas), block(32 * AT_WARPS);
+  if (UNITS && a.cluster > 1) return launch_pdl_cluster(kernel, grid, block, a.cluster, st, smem, a);
+  e = launch_pdl(kernel, grid, block, smem, st, a);
+  if (e != cudaSuccess || UNITS) return e;
   return launch_pdl(attn_join_kernel<T, D, AtShape>, dim3((unsigned)a.ctas, (unsigned)(a.n * a.group)), dim3(256), 0, st,
                     a);
 }
@@ -77,14 +91,20 @@ cudaError_t rows_launch(cudaStream_t st, const AttnArgs& a) {
   if (e == cudaSuccess)
     e = launch_pdl(attn_rows_kernel<T, FMT, D>, dim3((unsigned)a.ctas), dim3(AR_THREADS), smem, st, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, 32), dim3(256), 0, st, a);
+  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, 16), dim3(256), 0, st, a);
 }
 
-template <typename T, int FMT>
-cudaError_t attend(int nt, cudaStream_t st, const AttnArgs& a) {
-  if (nt == 0) return a.dim == 256 ? rows_launch<T, FMT, 256>(st, a) : rows_launch<T, FMT, 128>(st, a);
-  if (a.dim == 256) return nt == 1 ? token_launch<T, FMT, 256, 1>(st, a) : token_launch<T, FMT, 256, 2>(st, a);
-  return nt == 1 ? token_launch<T, FMT, 128, 1>(st, a) : token_launch<T, FMT, 128, 2>(st, a);
+template <typename T, int FMT, int D>
+cudaError_t attend(const Plan& p, cudaStream_t st, const AttnArgs& a) {
+  if (p.nt == 0) return rows_launch<T, FMT, D>(st, a);
+  if (p.nt == 1) return p.cluster ? token_launch<T, FMT, D, 1, true>(st, a) : token_launch<T, FMT, D, 1, false>(st, a);
+  return p.cluster ? token_launch<T, FMT, D, 2, true>(st, a) : token_launch<T, FMT, D, 2, false>(st, a);
+}
+
+template <typename T>
+cudaError_t attend(int fmt, const Plan& p, cudaStream_t st, const AttnArgs& a) {
+  if (fmt == KV_INT8) return a.dim == 256 ? attend<T, KV_INT8, 256>(p, st, a) : attend<T, KV_INT8, 128>(p, st, a);
+  return a.dim == 256 ? attend<T, KV_FP8, 256>(p, st, a) : attend<T, KV_FP8, 128>(p, st, a);
 }
 
 }  // namespace
@@ -158,12 +178,9 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   a.part = static_cast<float*>(workspace);
   a.stat = a.part + (size_t)2 * a.ctas * a.rows8 * dim;
   a.joints = reinterpret_cast<Joint*>(a.stat + (size_t)2 * a.ctas * a.rows8 * 2);
+  a.cluster = plan.cluster;
   a.err = device_error_word();
-  cudaError_t e;
-  if (dtype == DT_F16)
-    e = fmt == KV_INT8 ? attend<__half, KV_INT8>(plan.nt, st, a) : attend<__half, KV_FP8>(plan.nt, st, a);
-  else
-    e = fmt == KV_INT8 ? attend<__nv_bfloat16, KV_INT8>(plan.nt, st, a) : attend<__nv_bfloat16, KV_FP8>(plan.nt, st, a);
+  cudaError_t e = dtype == DT_F16 ? attend<__half>(fmt, plan, st, a) : attend<__nv_bfloat16>(fmt, plan, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e == cudaSuccess) return GSQ_OK;
   char buf[256];

@@ -30,14 +30,14 @@ static inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 b
 }
 
 // launch_pdl with thread-block clusters of `cluster_x` CTAs along x (grid.x
-// a multiple of cluster_x), no dynamic shared memory.
+// a multiple of cluster_x) and `smem` bytes of dynamic shared memory.
 template <typename... KArgs, typename... Args>
 static inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, unsigned cluster_x,
-                                             cudaStream_t st, Args&&... args) {
+                                             cudaStream_t st, size_t smem, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
-  cfg.dynamicSmemBytes = 0;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

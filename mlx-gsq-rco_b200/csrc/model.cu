@@ -815,7 +815,7 @@ int gdn_run(const float* proj, int64_t proj_stride, const uint16_t* ab, int64_t 
   cudaStream_t st = (cudaStream_t)stream;
   if (T == 1) {
     if (nv * batch < 2 * 148)  // few heads x sequences: 4 CTAs (a cluster) per head
-      launch_pdl_cluster(gdn_decode_kernel<4>, dim3((unsigned)(nv * 4), (unsigned)batch), dim3(2 * GDN_D), 4, st, a);
+      launch_pdl_cluster(gdn_decode_kernel<4>, dim3((unsigned)(nv * 4), (unsigned)batch), dim3(2 * GDN_D), 4, st, 0, a);
     else
       launch_pdl(gdn_decode_kernel<1>, dim3((unsigned)nv, (unsigned)batch), dim3(8 * GDN_D), 0, st, a);
     return launched("gsq_gdn (one token)");
