@@ -10,9 +10,7 @@ import numpy as np
 import torch
 
 from ... import _lib
-from .kvcache import check_counts, check_start, strides3
-
-_WORKSPACE_BYTES: dict[tuple, int] = {}  # gsq_cached_attention_workspace_size per shape: a pure function of it
+from .kvcache import _I, _I64, Strides, check_counts, check_start
 
 
 def tree_mask(parents, device="cuda") -> torch.Tensor:
@@ -53,26 +51,24 @@ def cached_attention(q: torch.Tensor, cache, start: torch.Tensor, *, counts: tor
     counts[b]), give zeros.  ``gate``: fp32 of q's shape, any strides with
     the last dimension contiguous; ``scale``: dim ** -0.5 by default.
     Returns [batch, n, heads, dim] in q's dtype (``out``, when given)."""
-    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
-        raise ValueError(f"expected q [{cache.batch}, n, heads, {cache.dim}], got {tuple(q.shape)}")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"queries must be float16 or bfloat16, got {q.dtype}")
-    batch, n, heads, dim = q.shape
-    if heads == 0 or heads % cache.heads:
-        raise ValueError(f"{heads} query heads are not a multiple of the cache's {cache.heads}")
+    lib = _lib.load()
+    key = ("attend", q.shape, q.stride(), q.dtype)
+    call = cache.checked.get(key)
+    if call is None:
+        call = _check_queries(q, cache, key)
+    direct, need, words, args = call
     dev = cache.device
+    batch, n = q.shape[:2]
     if q.device != dev:
         raise RuntimeError("tensors on different devices")
     stride = check_start(start, batch, dev)
-    # the kernels read rows of q with 16-byte loads
-    qs = q.stride()
-    if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() % 16:
-        q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)
+    if not direct or q.data_ptr() % 16:  # the kernels read rows of q with 16-byte loads
+        return cached_attention(torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q), cache, start, counts=counts,
+                                tree=tree, gate=gate, scale=scale, out=out)
     tree_ptr, tree_stride = None, 0
     if tree is not None:
         if tree.dtype != torch.int32:
             raise TypeError(f"a tree mask is int32 words, got {tree.dtype}")
-        words = (n + 31) // 32
         if tree.shape not in ((n, words), (batch, n, words)) or n > 1024:
             raise ValueError(f"expected a tree mask [{n}, {words}] or [{batch}, {n}, {words}] with n at most 1024, "
                              f"got {tuple(tree.shape)}")
@@ -86,23 +82,34 @@ def cached_attention(q: torch.Tensor, cache, start: torch.Tensor, *, counts: tor
             raise ValueError(f"the gate must be float32 of q's shape {tuple(q.shape)}")
         if gate.device != dev:
             raise RuntimeError("tensors on different devices")
-        if gate.stride(3) != 1:
+        gs = gate.stride()
+        if gs[3] != 1:
             gate = gate.contiguous()
-        gate_ptr, gate_strides = gate.data_ptr(), strides3(gate)
+            gs = gate.stride()
+        gate_ptr, gate_strides = gate.data_ptr(), Strides(*gs[:3])
     if out is None:
-        out = q.new_empty((batch, n, heads, dim))
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
-    lib = _lib.load()
-    key = (batch, n, heads, cache.heads, dim, cache.length)
-    need = _WORKSPACE_BYTES.get(key)
-    if need is None:
-        need = _WORKSPACE_BYTES[key] = lib.gsq_cached_attention_workspace_size(*key)
-    ws = q.new_empty(need // 2) if need else None  # of two-byte values: new_empty is the cheapest allocation
-    _lib.launch(dev, lib.gsq_cached_attention, q.data_ptr(), _lib.DTYPE_CODES[q.dtype], strides3(q), batch, n, heads,
-                cache.heads, dim, cache.fmt, *cache.pointers, cache.length, start.data_ptr(), stride,
-                None if counts is None else check_counts(counts, batch, dev), tree_ptr, tree_stride, gate_ptr,
-                gate_strides, dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
-                ws.data_ptr() if need else None, need)
+    ws = q.new_empty(need // 2).data_ptr() if need else None  # this call's alone: the stream orders its next use
+    _lib.launch(dev, lib.gsq_cached_attention, q.data_ptr(), *args, *cache.pointers, cache.length, start.data_ptr(),
+                stride, None if counts is None else check_counts(counts, batch, dev), tree_ptr, tree_stride, gate_ptr,
+                gate_strides, cache.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ws, need)
     return out
+
+
+def _check_queries(q: torch.Tensor, cache, key: tuple) -> tuple:
+    """(whether the kernels read q as it is, workspace bytes, words of a tree's row, C arguments) for q's shape."""
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
+        raise ValueError(f"expected q [{cache.batch}, n, heads, {cache.dim}], got {tuple(q.shape)}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"queries must be float16 or bfloat16, got {q.dtype}")
+    batch, n, heads, dim = q.shape
+    if heads == 0 or heads % cache.heads:
+        raise ValueError(f"{heads} query heads are not a multiple of the cache's {cache.heads}")
+    s = q.stride()
+    need = _lib.load().gsq_cached_attention_workspace_size(batch, n, heads, cache.heads, dim, cache.length)
+    args = (_I(_lib.DTYPE_CODES[q.dtype]), Strides(*s[:3]), _I64(batch), _I64(n), _I64(heads), _I64(cache.heads),
+            _I64(dim), _I(cache.fmt))
+    return cache.remember(key, (s[3] == 1 and not (s[0] | s[1] | s[2]) % 8, need, (n + 31) // 32, args))

@@ -12,18 +12,7 @@ import torch
 from ... import _lib
 
 Strides = ctypes.c_int64 * 3
-_STRIDES: dict[tuple, ctypes.Array] = {}
-
-
-def strides3(t: torch.Tensor) -> ctypes.Array:
-    """The first three strides of a 4-dimensional tensor for the C ABI, which only reads them."""
-    key = t.stride()
-    s = _STRIDES.get(key)
-    if s is None:
-        if len(_STRIDES) > 4096:
-            _STRIDES.clear()
-        s = _STRIDES[key] = Strides(*key[:3])
-    return s
+_I, _I64 = ctypes.c_int, ctypes.c_int64  # arguments in the C ABI's own types are not converted again at each call
 
 
 def check_start(start: torch.Tensor, batch: int, device) -> int:
@@ -60,22 +49,26 @@ def kv_append(cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
     ``counts``: int32, sequence b has only ``counts[b]`` new tokens and the
     rest of its rows is padding.  A position outside the cache is not written
     and shows as 3 in ``_lib.device_status``."""
-    if k.shape != v.shape or k.dim() != 4 or k.shape[0] != cache.batch or k.shape[2:] != (cache.heads, cache.dim):
-        raise ValueError(f"expected k and v [{cache.batch}, tokens, {cache.heads}, {cache.dim}], "
-                         f"got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.dtype not in _lib.DTYPE_CODES or v.dtype != k.dtype:
-        raise TypeError(f"unsupported key/value dtypes {k.dtype}, {v.dtype}")
+    key = ("append", k.shape, v.shape, k.stride(), v.stride(), k.dtype, v.dtype)
+    call = cache.checked.get(key)
+    if call is None:
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != cache.batch or k.shape[2:] != (cache.heads, cache.dim):
+            raise ValueError(f"expected k and v [{cache.batch}, tokens, {cache.heads}, {cache.dim}], "
+                             f"got {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.dtype not in _lib.DTYPE_CODES or v.dtype != k.dtype:
+            raise TypeError(f"unsupported key/value dtypes {k.dtype}, {v.dtype}")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            return kv_append(cache, k.contiguous(), v.contiguous(), start, counts)
+        call = cache.remember(key, (_I(_lib.DTYPE_CODES[k.dtype]), _I64(cache.batch), _I64(k.shape[1]),
+                                    _I64(cache.heads), _I64(cache.dim), Strides(*k.stride()[:3]),
+                                    Strides(*v.stride()[:3])))
     dev = cache.device
     if k.device != dev or v.device != dev:
         raise RuntimeError("tensors on different devices")
     stride = check_start(start, cache.batch, dev)
-    if k.stride(3) != 1:
-        k = k.contiguous()
-    if v.stride(3) != 1:
-        v = v.contiguous()
-    _lib.launch(dev, _lib.load().gsq_kv_append, k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODES[k.dtype], cache.batch,
-                k.shape[1], cache.heads, cache.dim, strides3(k), strides3(v), start.data_ptr(), stride,
-                check_counts(counts, cache.batch, dev), cache.fmt, *cache.pointers, cache.length)
+    _lib.launch(dev, _lib.load().gsq_kv_append, k.data_ptr(), v.data_ptr(), *call, start.data_ptr(), stride,
+                None if counts is None else check_counts(counts, cache.batch, dev), cache.fmt, *cache.pointers,
+                cache.length)
 
 
 def kv_read(cache, start: torch.Tensor, tokens: int, *, counts: torch.Tensor | None = None,
@@ -90,9 +83,10 @@ def kv_read(cache, start: torch.Tensor, tokens: int, *, counts: torch.Tensor | N
         raise ValueError("negative token count")
     dev = cache.device
     stride = check_start(start, cache.batch, dev)
-    shape = (cache.batch, tokens, cache.heads, cache.dim)
-    k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+    k = torch.empty((cache.batch, tokens, cache.heads, cache.dim), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     _lib.launch(dev, _lib.load().gsq_kv_read, cache.fmt, *cache.pointers, cache.batch, cache.heads, cache.length,
-                cache.dim, start.data_ptr(), stride, check_counts(counts, cache.batch, dev), tokens, k.data_ptr(),
+                cache.dim, start.data_ptr(), stride,
+                None if counts is None else check_counts(counts, cache.batch, dev), tokens, k.data_ptr(),
                 v.data_ptr(), _lib.DTYPE_CODES[dtype])
     return k, v

@@ -13,10 +13,8 @@ from ... import _lib
 _WORKSPACE_BYTES: dict[tuple[int, int], int] = {}  # gsq_adjust_logits_workspace_size per shape: a pure function of it
 
 
-def _per_row(t: torch.Tensor | None, name: str, rows: int, dev) -> int | None:
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or t.shape != (rows,) or t.device != dev or not t.is_contiguous():
+def _per_row(t: torch.Tensor, name: str, rows: int, dev) -> int:
+    if t.dtype != torch.float32 or t.shape != (rows,) or t.device != dev or t.stride(0) != 1:
         raise ValueError(f"{name} must be {rows} contiguous float32 values on {dev}")
     return t.data_ptr()
 
@@ -42,7 +40,9 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
         raise ValueError(f"expected logits [rows, vocab], got {tuple(logits.shape)}")
     if logits.dtype not in _lib.DTYPE_CODES:
         raise TypeError(f"unsupported logits dtype {logits.dtype}")
-    dev = _lib.require_cuda(logits)
+    dev = logits.device
+    if dev.type != "cuda":
+        raise RuntimeError("gsq_b200 runs on CUDA tensors only (no CPU fallback)")
     rows, vocab = logits.shape
     words = (vocab + 31) // 32
     if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < vocab):
@@ -81,21 +81,22 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
         allowed = allowed.contiguous()
         allowed_ptr, allowed_stride = allowed.data_ptr(), words if allowed.dim() == 2 else 0
     if out is None:
-        out = torch.empty((rows, vocab), dtype=torch.float32, device=dev)
+        out = logits.new_empty((rows, vocab), dtype=torch.float32)
     elif out.shape != (rows, vocab) or out.dtype != torch.float32 or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous float32 tensor of the logits' shape and device")
-    nxt = torch.empty(rows, dtype=torch.int32, device=dev)
+    nxt = logits.new_empty(rows, dtype=torch.int32)
     lib = _lib.load()
     key = (rows, vocab)
     need = _WORKSPACE_BYTES.get(key)
     if need is None:
         need = _WORKSPACE_BYTES[key] = lib.gsq_adjust_logits_workspace_size(rows, vocab)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = out.new_empty(need // 4) if need else None  # this call's alone: the stream orders its next use
     _lib.launch(dev, lib.gsq_adjust_logits, logits.data_ptr(), _lib.DTYPE_CODES[logits.dtype],
                 max(logits.stride(0), vocab), rows, vocab, seen_ptr, counts_ptr,
-                _per_row(repetition, "repetition", rows, dev), _per_row(frequency, "frequency", rows, dev),
-                _per_row(presence, "presence", rows, dev), bias_ids.data_ptr() if biases else None,
-                bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
+                None if repetition is None else _per_row(repetition, "repetition", rows, dev),
+                None if frequency is None else _per_row(frequency, "frequency", rows, dev),
+                None if presence is None else _per_row(presence, "presence", rows, dev),
+                bias_ids.data_ptr() if biases else None, bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
                 nxt.data_ptr(), int(record), ws.data_ptr() if need else None, need)
     return out, nxt
 

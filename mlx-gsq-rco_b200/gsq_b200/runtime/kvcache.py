@@ -9,6 +9,8 @@ it back, ``kernels.cached_attention`` attends over it.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 KV_FORMATS = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}  # by gsq_kv_format: 0, 1
@@ -18,7 +20,7 @@ _CODE = {torch.int8: 0, torch.float8_e4m3fn: 1}
 class QuantizedKVCache:
     """A handle on the four tensors (not copied; all contiguous, on one CUDA device)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "batch", "heads", "length", "dim", "fmt", "device", "pointers")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "batch", "heads", "length", "dim", "fmt", "device", "pointers", "checked")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
         if k.dim() != 4 or k.shape[3] not in (128, 256):
@@ -39,7 +41,15 @@ class QuantizedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = tensors
         self.batch, self.heads, self.length, self.dim = k.shape
         self.fmt, self.device = _CODE[k.dtype], k.device
-        self.pointers = tuple(t.data_ptr() for t in tensors)
+        self.pointers = tuple(ctypes.c_void_p(t.data_ptr()) for t in tensors)
+        self.checked: dict[tuple, tuple] = {}  # shapes and strides of calls seen, with what the C ABI takes for them
+
+    def remember(self, key: tuple, call: tuple) -> tuple:
+        """Keeps what was derived from a call's shapes, strides and types (never from its data or addresses)."""
+        if len(self.checked) >= 1024:
+            self.checked.clear()
+        self.checked[key] = call
+        return call
 
     @classmethod
     def empty(cls, batch: int, heads: int, length: int, dim: int, fmt: str = "int8", device="cuda") -> QuantizedKVCache:
