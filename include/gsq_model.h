@@ -211,15 +211,12 @@ GSQ_API int gsq_cached_attention(const void* q, int dtype, const int64_t* q_stri
  *               [0, vocab) are skipped (padding)
  *   allowed     words like seen's, row r's at r * allowed_stride (0: one mask
  *               for all), bit set = allowed; or NULL
- * workspace: gsq_adjust_logits_workspace_size() bytes, 8-byte aligned, of any
- * content, for this call alone until it has completed. */
-GSQ_API size_t gsq_adjust_logits_workspace_size(int64_t rows, int64_t vocab);
+ * rows <= 65535, vocab <= 2^20.  No workspace. */
 GSQ_API int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
                               int32_t* seen, int32_t* counts, const float* repetition, const float* frequency,
                               const float* presence, const int32_t* bias_ids, const float* bias_values,
                               int64_t biases, const int32_t* allowed, int64_t allowed_stride, float* out,
-                              int32_t* next, int record, void* workspace, size_t workspace_bytes,
-                              gsq_stream_t stream);
+                              int32_t* next, int record, gsq_stream_t stream);
 
 /* The history of row r learns tokens[r * row_stride + 0 .. n): as output
  * (generated != 0: bit and count) or as prompt (bit only).  Tokens outside

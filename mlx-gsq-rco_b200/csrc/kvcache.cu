@@ -27,7 +27,7 @@ using namespace gsq;
 namespace {
 
 constexpr int KV_WARPS = 4;  // per CTA
-constexpr int KV_EACH = 2;   // vectors per warp
+constexpr int KV_EACH = 4;   // vectors per warp
 
 struct KvArgs {
   const void* src[2];     // k, v (append)
@@ -43,14 +43,12 @@ struct KvArgs {
   int* err;
 };
 
-// Position of vector (b, t) in the cache, or -1: past the sequence's count, or outside the cache.
-__device__ __forceinline__ int64_t kv_position(const KvArgs& a, int b, int t, bool* outside) {
-  *outside = false;
-  if (a.counts && t >= a.counts[b]) return -1;
-  const int64_t p = (int64_t)a.start[(int64_t)b * a.start_stride] + t;
-  if (p >= 0 && p < a.cap) return p;
-  *outside = true;
-  return -1;
+// Sequence b's first position and its tokens (past them: padding).
+struct KvSpan {
+  int start, count;
+};
+__device__ __forceinline__ KvSpan kv_span(const KvArgs& a, int b) {
+  return {a.start[(int64_t)b * a.start_stride], a.counts ? min(a.counts[b], a.tokens) : a.tokens};
 }
 
 // N consecutive values of T at p, as one or two vector loads where VEC (p 16-byte aligned, or 8-byte for 8 bytes).
@@ -91,7 +89,9 @@ __device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N
   // +-2^-21 around it have the same nearest code, that is the code, without a division; near a tie, or where the
   // reciprocal may leave the normal range, it is divided.
   uint32_t differ = scale > 1e-30f ? 0u : 1u;
-  const float inv = __frcp_rn(scale), up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));  // within 2^-23
+  const float up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
     if constexpr (FMT == KV_INT8) {
@@ -148,19 +148,22 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_append_kernel(const KvArgs a
   const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
   float f[KV_EACH][N];
   int64_t row[KV_EACH];  // of codes and scales, or -1
+  int t = first / (unsigned)a.heads, h = first % (unsigned)a.heads;
+  const KvSpan span = kv_span(a, b);
+  const T* src = static_cast<const T*>(a.src[which]) + b * a.sb[which] + lane * N;
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
     row[i] = -1;
-    const unsigned u = first + i;
-    if (u >= (unsigned)(a.tokens * a.heads)) continue;
-    const int t = u / (unsigned)a.heads, h = u % (unsigned)a.heads;
-    bool outside;
-    const int64_t p = kv_position(a, b, t, &outside);
-    if (outside && lane == 0 && a.err) atomicExch(a.err, DEV_CACHE_POSITION);
-    if (p < 0) continue;
-    row[i] = ((int64_t)b * a.heads + h) * a.cap + p;
-    load_n<T, N, VEC>(
-        static_cast<const T*>(a.src[which]) + b * a.sb[which] + t * a.st[which] + h * a.sh[which] + lane * N, f[i]);
+    if (t < span.count) {
+      const int64_t p = (int64_t)span.start + t;
+      if (p >= 0 && p < a.cap) {
+        row[i] = ((int64_t)b * a.heads + h) * a.cap + p;
+        load_n<T, N, VEC>(src + t * a.st[which] + h * a.sh[which], f[i]);
+      } else if (lane == 0 && a.err) {
+        atomicExch(a.err, DEV_CACHE_POSITION);
+      }
+    }
+    if (++h == a.heads) h = 0, t++;
   }
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
@@ -183,21 +186,22 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvArgs a) 
   const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
   uint32_t c[KV_EACH][N / 4];
   float scale[KV_EACH];
+  int t = first / (unsigned)a.heads, h = first % (unsigned)a.heads;
+  const KvSpan span = kv_span(a, b);
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
-    const unsigned u = first + i;
     scale[i] = 0.f;
 #pragma unroll
     for (int e = 0; e < N / 4; e++) c[i][e] = 0u;
-    if (u >= vectors) break;
-    bool outside;
-    const int64_t p = kv_position(a, b, u / (unsigned)a.heads, &outside);
-    if (p < 0) continue;
-    const int64_t row = ((int64_t)b * a.heads + u % (unsigned)a.heads) * a.cap + p;
-    scale[i] = a.scale[which][row];
-    const uint8_t* src = a.codes[which] + row * D + lane * N;
-    if constexpr (N == 8) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(src);
-    else c[i][0] = *reinterpret_cast<const uint32_t*>(src);
+    const int64_t p = (int64_t)span.start + t;
+    if (t < span.count && p >= 0 && p < a.cap) {
+      const int64_t row = ((int64_t)b * a.heads + h) * a.cap + p;
+      scale[i] = a.scale[which][row];
+      const uint8_t* src = a.codes[which] + row * D + lane * N;
+      if constexpr (N == 8) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(src);
+      else c[i][0] = *reinterpret_cast<const uint32_t*>(src);
+    }
+    if (++h == a.heads) h = 0, t++;
   }
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {

@@ -6,16 +6,17 @@
 // result is the formula's in any order of evaluation a host would use, and
 // ties go to the lowest token.
 //
-// Bound: HBM bytes, one read and one write of the rows.  A row is cut into
-// chunks of LG_CHUNK tokens, one CTA each, so that one row still fills the GPU
-// (248320 tokens: 122 CTAs).  A thread holds eight tokens, as two 16-byte
-// pieces where every row starts on such a boundary, else one by one in
-// neighbouring lanes.  The penalties run only where a token's seen bit is set
-// (some thousand of 248320 tokens), and only there the counts are read.  Biases
-// of a chunk are gathered into shared memory first, duplicates summed in list
-// order by one thread, so no atomic orders the sum.  Each CTA leaves its best
-// token; a second launch (one warp per row) takes the best of them and
-// records it.
+// Bound: HBM bytes, one read and one write of the rows.  A row belongs to one
+// cluster of up to 8 CTAs, each with a run of its tokens: one launch, in which
+// the CTAs' best tokens meet in distributed shared memory.  A thread takes
+// eight tokens at a time, as two 16-byte pieces where every row starts on such
+// a boundary, else one by one in neighbouring lanes.  The penalties run only
+// where a token's seen bit is set (some thousand of 248320 tokens), and only
+// there the counts are read.  Biased tokens are marked in a bit mask in shared
+// memory; the main pass leaves them without bias and mask and out of the
+// maximum, and a second pass over the list finishes them, each by the thread
+// of its first entry, which adds the token's biases in list order: no atomic
+// orders a sum.
 #include <cstdio>
 
 #include "gsq_common.cuh"
@@ -26,12 +27,14 @@ using namespace gsq;
 
 namespace {
 
-constexpr int LG_THREADS = 256;
-constexpr int LG_CHUNK = 8 * LG_THREADS;  // tokens per CTA
+constexpr int LG_THREADS = 1024;          // of a CTA, at most
+constexpr int LG_CLUSTER = 8;             // CTAs of a row, at most
+constexpr int64_t LG_VOCAB = 1ll << 20;   // tokens: the mask of a CTA's biased ones has a bit for each
 
 struct LogitsArgs {
   const void* logits;
-  int64_t row_stride, vocab, words, chunks;
+  int64_t row_stride, vocab, words;
+  int cluster, run;  // CTAs of a row, tokens of each (a multiple of 128)
   int32_t* seen;    // [rows, words] or null
   int32_t* counts;  // [rows, vocab]
   const float *repetition, *frequency, *presence;  // [rows] or null
@@ -42,7 +45,6 @@ struct LogitsArgs {
   int64_t allowed_stride;
   float* out;
   int32_t* next;
-  unsigned long long* best;  // [rows, chunks]
   int record;
 };
 
@@ -75,132 +77,6 @@ __device__ __forceinline__ void load4(const T* p, float* f) {
   }
 }
 
-// VEC: the rows of logits and out start on 16-byte (two-byte types: 8-byte) boundaries, and vocab % 4 == 0.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) {
-  __shared__ __align__(16) float bias[LG_CHUNK];
-  __shared__ unsigned long long part[LG_THREADS / 32];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int64_t row = blockIdx.y;
-  const int vocab = (int)a.vocab, c0 = blockIdx.x * LG_CHUNK;
-  const int tid = threadIdx.x, lane = tid & 31;
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const int32_t* seen_row = a.seen ? a.seen + row * a.words : nullptr;
-  const int32_t* allowed_row = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  // token e of this thread, and its bits of the masks (bit e), one word for 4 tokens of 8 lanes or 1 of 32
-  auto token = [&](int e) { return VEC ? c0 + e / 4 * (4 * LG_THREADS) + 4 * tid + e % 4 : c0 + e * LG_THREADS + tid; };
-  alignas(16) float z[8] = {};
-  uint32_t seen = 0, allowed = 0xffu;
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int v = token(4 * i);
-      if (v < vocab) {
-        load4(x + v, z + 4 * i);
-        if (seen_row) seen |= ((uint32_t)seen_row[v >> 5] >> (v & 31) & 15u) << 4 * i;
-        if (allowed_row) allowed &= ((uint32_t)allowed_row[v >> 5] >> (v & 31) & 15u) << 4 * i | 15u << 4 * (1 - i);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int v = token(e);
-      if (v < vocab) {
-        z[e] = to_f32(x[v]);
-        if (seen_row) seen |= ((uint32_t)seen_row[v >> 5] >> lane & 1u) << e;
-        if (allowed_row && !((uint32_t)allowed_row[v >> 5] >> lane & 1u)) allowed &= ~(1u << e);
-      }
-    }
-  }
-  if (a.biases) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) reinterpret_cast<float4*>(bias)[tid + i * LG_THREADS] = make_float4(0.f, 0.f, 0.f, 0.f);
-    __syncthreads();
-    const int32_t* ids = a.bias_ids + row * a.biases;
-    const float* val = a.bias_values + row * a.biases;
-    const int n = (int)a.biases;
-    for (int i = tid; i < n; i += LG_THREADS) {
-      const int id = ids[i];
-      if (id < c0 || id - c0 >= LG_CHUNK || id >= vocab) continue;
-      bool first = true;
-      for (int j = 0; j < i && first; j++) first = ids[j] != id;
-      if (!first) continue;
-      float s = 0.f;
-      for (int j = i; j < n; j++)
-        if (ids[j] == id) s = __fadd_rn(s, val[j]);
-      bias[id - c0] = s;
-    }
-    __syncthreads();
-  }
-  if (seen) {
-    const float rep = a.repetition ? a.repetition[row] : 1.f;
-    const float freq = a.frequency ? a.frequency[row] : 0.f;
-    const float pres = a.presence ? a.presence[row] : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      if (seen >> e & 1) {
-        float y = z[e];
-        y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-        const int32_t n = a.counts[row * vocab + token(e)];
-        if (n > 0) {
-          y = __fsub_rn(y, __fmul_rn(freq, (float)n));
-          y = __fsub_rn(y, pres);
-        }
-        z[e] = y;
-      }
-    }
-  }
-  if (a.biases) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = __fadd_rn(z[e], bias[token(e) - c0]);
-  }
-  if (allowed != 0xffu) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = allowed >> e & 1 ? z[e] : -INFINITY;
-  }
-  float* out = a.out + row * vocab;
-  // the thread's best token: tokens rise with e, so those past the end come after the others
-  if (c0 + LG_CHUNK > vocab) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = token(e) < vocab ? z[e] : -INFINITY;
-  }
-  float top = z[0];
-  bool nan = isnan(z[0]);
-#pragma unroll
-  for (int e = 1; e < 8; e++) {
-    top = fmaxf(top, z[e]);
-    nan = nan || isnan(z[e]);
-  }
-  int at = 0;
-  if (nan) {
-#pragma unroll
-    for (int e = 7; e >= 0; e--) at = isnan(z[e]) ? e : at;
-    top = __int_as_float(0x7fffffff);
-  } else {
-#pragma unroll
-    for (int e = 7; e >= 0; e--) at = z[e] == top ? e : at;
-  }
-  unsigned long long best = 0;
-  if (token(at) < vocab) best = (unsigned long long)order_key(top) << 32 | (uint32_t)~(uint32_t)token(at);
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-      if (token(4 * i) < vocab) *reinterpret_cast<float4*>(out + token(4 * i)) = *reinterpret_cast<const float4*>(z + 4 * i);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (token(e) < vocab) out[token(e)] = z[e];
-  }
-  best = warp_max(best);
-  if (lane == 0) part[tid >> 5] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < LG_THREADS / 32; w++) best = part[w] > best ? part[w] : best;
-    a.best[row * a.chunks + blockIdx.x] = best;
-  }
-}
-
 // The history of row r learns token v (bit and, for a generated token, count).
 __device__ __forceinline__ void remember(int32_t* seen, int32_t* counts, int64_t words, int64_t vocab, int64_t r,
                                          int64_t v, bool generated) {
@@ -208,21 +84,192 @@ __device__ __forceinline__ void remember(int32_t* seen, int32_t* counts, int64_t
   if (generated) atomicAdd(counts + r * vocab + v, 1);
 }
 
-__global__ void __launch_bounds__(32) pick_kernel(const LogitsArgs a) {
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// VEC: the rows of logits and out start on 16-byte (two-byte types: 8-byte) boundaries, and vocab % 4 == 0.
+// BIAS: there are biases; dynamic shared memory: the mask of biased tokens of the CTA's run.
+template <typename T, bool VEC, bool BIAS>
+__global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) {
+  extern __shared__ uint32_t biased[];
+  __shared__ unsigned long long part[LG_THREADS / 32], cta_best;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t row = blockIdx.x;
+  const int64_t row = blockIdx.y;
+  const int vocab = (int)a.vocab, lo = blockIdx.x * a.run, hi = min(vocab, lo + a.run);
+  const int tid = threadIdx.x, lane = tid & 31;
+  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
+  float* out = a.out + row * vocab;
+  const int32_t* seen_row = a.seen ? a.seen + row * a.words : nullptr;
+  const int32_t* allowed_row = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+  const int32_t* ids = BIAS ? a.bias_ids + row * a.biases : nullptr;
+  const int biases = (int)a.biases;
+  const float rep = a.repetition ? a.repetition[row] : 1.f;
+  const float freq = a.frequency ? a.frequency[row] : 0.f;
+  const float pres = a.presence ? a.presence[row] : 0.f;
+  if constexpr (BIAS) {
+    for (int i = tid; i < a.run / 32; i += blockDim.x) biased[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < biases; i += blockDim.x) {
+      const int id = ids[i];
+      if (id >= lo && id < hi) atomicOr(&biased[(id - lo) >> 5], 1u << (id & 31));  // lo % 32 == 0
+    }
+    __syncthreads();
+  }
+
   unsigned long long best = 0;
-  for (int64_t i = threadIdx.x; i < a.chunks; i += 32) {
-    const unsigned long long k = a.best[row * a.chunks + i];
+  float top = -INFINITY;  // the thread's best so far
+  int top_at = -1;
+  // Eight tokens of the thread and their mask words; the next eight are loaded while these are worked on.
+  struct Group {
+    alignas(16) float z[8];
+    uint32_t seen[VEC ? 2 : 8], allowed[VEC ? 2 : 8];
+  };
+  const int threads = blockDim.x, step = 8 * threads;
+  auto token = [&](int v0, int e) { return VEC ? v0 + e / 4 * (4 * threads) + 4 * tid + e % 4 : v0 + e * threads + tid; };
+  auto load = [&](int v0, Group& g) {
+    constexpr int N = VEC ? 2 : 8;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int v = token(v0, i * (8 / N));
+      const bool in = v < hi;
+      if constexpr (VEC) {
+        if (in) load4(x + v, g.z + 4 * i);
+        else g.z[4 * i] = g.z[4 * i + 1] = g.z[4 * i + 2] = g.z[4 * i + 3] = -INFINITY;
+      } else {
+        g.z[i] = in ? to_f32(x[v]) : -INFINITY;
+      }
+      g.seen[i] = in && seen_row ? (uint32_t)seen_row[v >> 5] >> (v & 31) : 0u;
+      g.allowed[i] = in && allowed_row ? (uint32_t)allowed_row[v >> 5] >> (v & 31) : ~0u;
+    }
+  };
+  Group next;
+  load(lo, next);
+  for (int v0 = lo; v0 < hi; v0 += step) {
+    Group g = next;
+    if (v0 + step < hi) load(v0 + step, next);
+    float (&z)[8] = g.z;
+    uint32_t seen = 0, hidden = 0, late = 0;  // bit e: seen, not allowed, biased
+    if constexpr (VEC) {
+      seen = (g.seen[0] & 15u) | (g.seen[1] & 15u) << 4;
+      hidden = (~g.allowed[0] & 15u) | (~g.allowed[1] & 15u) << 4;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        seen |= (g.seen[e] & 1u) << e;
+        hidden |= (~g.allowed[e] & 1u) << e;
+      }
+    }
+    if constexpr (BIAS) {
+#pragma unroll
+      for (int i = 0; i < (VEC ? 2 : 8); i++) {
+        const int v = token(v0, i * (VEC ? 4 : 1));
+        if (v < hi) late |= (biased[(v - lo) >> 5] >> (v & 31) & (VEC ? 15u : 1u)) << i * (VEC ? 4 : 1);
+      }
+    }
+    if (seen) {
+      int32_t n[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) n[e] = seen >> e & 1 ? a.counts[row * vocab + token(v0, e)] : 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (seen >> e & 1) {
+          z[e] = z[e] > 0.f ? __fdiv_rn(z[e], rep) : __fmul_rn(z[e], rep);
+          if (n[e] > 0) {
+            z[e] = __fsub_rn(z[e], __fmul_rn(freq, (float)n[e]));
+            z[e] = __fsub_rn(z[e], pres);
+          }
+        }
+      }
+    }
+    hidden &= ~late;
+    if (hidden) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) z[e] = hidden >> e & 1 ? -INFINITY : z[e];
+    }
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (token(v0, 4 * i) < hi)
+          *reinterpret_cast<float4*>(out + token(v0, 4 * i)) = *reinterpret_cast<const float4*>(z + 4 * i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (token(v0, e) < hi) out[token(v0, e)] = z[e];
+    }
+    // the thread's best token: they rise with e, and those past the end are -inf and come after the others
+    if (BIAS && late) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) z[e] = late >> e & 1 ? -INFINITY : z[e];
+    }
+    float m = z[0];
+    bool nan = isnan(z[0]);
+#pragma unroll
+    for (int e = 1; e < 8; e++) {
+      m = fmaxf(m, z[e]);
+      nan = nan || isnan(z[e]);
+    }
+    if (nan) {
+      int at = 0;
+#pragma unroll
+      for (int e = 7; e >= 0; e--) at = isnan(z[e]) ? e : at;
+      const unsigned long long k = 0xffffffffull << 32 | (uint32_t)~(uint32_t)token(v0, at);
+      best = k > best ? k : best;
+    } else if (m > top || top_at < 0) {
+      int at = 0;
+#pragma unroll
+      for (int e = 7; e >= 0; e--) at = z[e] == m ? e : at;
+      if (token(v0, at) < hi) {
+        top = m;
+        top_at = token(v0, at);
+      }
+    }
+  }
+  if (top_at >= 0) {
+    const unsigned long long k = (unsigned long long)order_key(top) << 32 | (uint32_t)~(uint32_t)top_at;
     best = k > best ? k : best;
   }
+  if constexpr (BIAS) {
+    __syncthreads();  // the main pass has written the biased tokens' values
+    const float* val = a.bias_values + row * a.biases;
+    for (int i = tid; i < biases; i += blockDim.x) {
+      const int id = ids[i];
+      if (id < lo || id >= hi) continue;
+      bool first = true;
+      for (int j = 0; j < i && first; j++) first = ids[j] != id;
+      if (!first) continue;
+      float s = 0.f;
+      for (int j = i; j < biases; j++)
+        if (ids[j] == id) s = __fadd_rn(s, val[j]);
+      float y = __fadd_rn(out[id], s);
+      if (allowed_row && !((uint32_t)allowed_row[id >> 5] >> (id & 31) & 1u)) y = -INFINITY;
+      out[id] = y;
+      const unsigned long long k = (unsigned long long)order_key(y) << 32 | (uint32_t)~(uint32_t)id;
+      best = k > best ? k : best;
+    }
+  }
   best = warp_max(best);
-  if (threadIdx.x == 0) {
+  if (lane == 0) part[tid >> 5] = best;
+  __syncthreads();
+  if (tid < 32) {
+    best = warp_max(tid < blockDim.x / 32 ? part[tid] : 0ull);
+    if (tid == 0) cta_best = best;
+  }
+  if (a.cluster > 1) cluster_sync_all();
+  if (blockIdx.x == 0 && tid == 0) {
+    for (int r = 1; r < a.cluster; r++) {
+      uint32_t remote;
+      unsigned long long k;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&cta_best)), "r"(r));
+      asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(remote) : "memory");
+      best = k > best ? k : best;
+    }
     const int32_t v = (int32_t)~(uint32_t)best;
     a.next[row] = v;
     if (a.record) remember(a.seen, a.counts, a.words, a.vocab, row, v, true);
   }
+  if (a.cluster > 1) cluster_sync_all();  // no CTA leaves before its best token is read
 }
 
 __global__ void __launch_bounds__(256) record_kernel(const int32_t* tokens, int64_t stride, int64_t rows, int64_t n,
@@ -247,31 +294,33 @@ int launched(cudaError_t rc, const char* what) {
   return fail(GSQ_ERR_CUDA, buf);
 }
 
-template <typename T>
-cudaError_t adjust_launch(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
-  return vec ? launch_pdl(adjust_kernel<T, true>, grid, dim3(LG_THREADS), 0, st, a)
-             : launch_pdl(adjust_kernel<T, false>, grid, dim3(LG_THREADS), 0, st, a);
+template <typename T, bool VEC, bool BIAS>
+cudaError_t adjust_launch(dim3 grid, size_t smem, cudaStream_t st, const LogitsArgs& a) {
+  // a CTA for each SM or fewer: all the threads there can be; else smaller ones, which divide more evenly
+  const dim3 block(grid.x * grid.y <= 148 ? LG_THREADS : grid.x * grid.y <= 296 ? LG_THREADS / 2 : LG_THREADS / 4);
+  return a.cluster > 1 ? launch_pdl_cluster(adjust_kernel<T, VEC, BIAS>, grid, block, a.cluster, st, smem, a)
+                       : launch_pdl(adjust_kernel<T, VEC, BIAS>, grid, block, smem, st, a);
 }
 
-int64_t chunks_of(int64_t vocab) { return (vocab + LG_CHUNK - 1) / LG_CHUNK; }
+template <typename T>
+cudaError_t adjust(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
+  const size_t smem = a.biases ? a.run / 8 : 0;
+  if (a.biases) return vec ? adjust_launch<T, true, true>(grid, smem, st, a) : adjust_launch<T, false, true>(grid, smem, st, a);
+  return vec ? adjust_launch<T, true, false>(grid, smem, st, a) : adjust_launch<T, false, false>(grid, smem, st, a);
+}
+
 bool al4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
 }  // namespace
 
 extern "C" {
 
-size_t gsq_adjust_logits_workspace_size(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || vocab <= 0) return 0;
-  return (size_t)rows * chunks_of(vocab) * sizeof(unsigned long long);
-}
-
 int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, int32_t* seen,
                       int32_t* counts, const float* repetition, const float* frequency, const float* presence,
                       const int32_t* bias_ids, const float* bias_values, int64_t biases, const int32_t* allowed,
-                      int64_t allowed_stride, float* out, int32_t* next, int record, void* workspace,
-                      size_t workspace_bytes, gsq_stream_t stream) {
+                      int64_t allowed_stride, float* out, int32_t* next, int record, gsq_stream_t stream) {
   if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return fail(GSQ_ERR_ARG, "gsq_adjust_logits: bad dtype");
-  if (rows < 0 || rows > 65535 || vocab <= 0 || vocab > (1ll << 30) || row_stride < vocab)
+  if (rows < 0 || rows > 65535 || vocab <= 0 || vocab > LG_VOCAB || row_stride < vocab)
     return fail(GSQ_ERR_SIZE, "gsq_adjust_logits: bad shape");
   if (biases < 0 || biases > 65536) return fail(GSQ_ERR_SIZE, "gsq_adjust_logits: bad bias count");
   if (rows == 0) return GSQ_OK;
@@ -282,15 +331,11 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
     return fail(GSQ_ERR_ARG, "gsq_adjust_logits: penalties and recording need a history");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2) || !al4(out) || !al4(next))
     return fail(GSQ_ERR_ALIGN, "gsq_adjust_logits: pointers not aligned to their type");
-  if (!workspace || workspace_bytes < gsq_adjust_logits_workspace_size(rows, vocab))
-    return fail(GSQ_ERR_WORKSPACE, "gsq_adjust_logits: workspace missing or too small");
-  if (reinterpret_cast<uintptr_t>(workspace) % 8) return fail(GSQ_ERR_ALIGN, "gsq_adjust_logits: workspace not 8-byte aligned");
   LogitsArgs a = {};
   a.logits = logits;
   a.row_stride = row_stride;
   a.vocab = vocab;
   a.words = (vocab + 31) / 32;
-  a.chunks = chunks_of(vocab);
   a.seen = seen;
   a.counts = counts;
   a.repetition = repetition;
@@ -303,18 +348,21 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
   a.allowed_stride = allowed_stride;
   a.out = out;
   a.next = next;
-  a.best = static_cast<unsigned long long*>(workspace);
   a.record = record;
+  // As many CTAs a row as fill the GPU once (six of them on an SM), so that a few rows get 8 and many get one; and
+  // no more than 2^18 tokens a CTA, whose mask of biased tokens is then at most 32 KB.
+  a.cluster = LG_CLUSTER;
+  while (a.cluster > 1 && rows * a.cluster > 148 * 6 && vocab <= (1ll << 18) * (a.cluster / 2)) a.cluster /= 2;
+  a.run = (int)((vocab + 128 * a.cluster - 1) / (128 * a.cluster) * 128);
+  const dim3 grid((unsigned)a.cluster, (unsigned)rows);
   cudaStream_t st = (cudaStream_t)stream;
-  const dim3 grid((unsigned)a.chunks, (unsigned)rows);
   const size_t size = dtype == DT_F32 ? 4 : 2;
   const bool vec = vocab % 4 == 0 && row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0 &&
                    reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  cudaError_t e = dtype == DT_F32   ? adjust_launch<float>(vec, grid, st, a)
-                  : dtype == DT_F16 ? adjust_launch<__half>(vec, grid, st, a)
-                                    : adjust_launch<__nv_bfloat16>(vec, grid, st, a);
-  if (e == cudaSuccess) e = launch_pdl(pick_kernel, dim3((unsigned)rows), dim3(32), 0, st, a);
-  return launched(e, "gsq_adjust_logits");
+  return launched(dtype == DT_F32   ? adjust<float>(vec, grid, st, a)
+                  : dtype == DT_F16 ? adjust<__half>(vec, grid, st, a)
+                                    : adjust<__nv_bfloat16>(vec, grid, st, a),
+                  "gsq_adjust_logits");
 }
 
 int gsq_record_tokens(const int32_t* tokens, int64_t row_stride, int64_t rows, int64_t n, int64_t vocab, int32_t* seen,

@@ -68,9 +68,7 @@ SIGNATURES = {
     "gsq_cached_attention_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "gsq_cached_attention": (_I, [_P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _P, _I64, _P, _P,
                                   _I64, _P, _P, ctypes.c_float, _P, _P, _SZ, _P]),
-    "gsq_adjust_logits_workspace_size": (_SZ, [_I64, _I64]),
-    "gsq_adjust_logits": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P, _I, _P,
-                               _SZ, _P]),
+    "gsq_adjust_logits": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P, _I, _P]),
     "gsq_record_tokens": (_I, [_P, _I64, _I64, _I64, _I64, _P, _P, _I, _P]),
 }
 

@@ -10,8 +10,6 @@ import torch
 
 from ... import _lib
 
-_WORKSPACE_BYTES: dict[tuple[int, int], int] = {}  # gsq_adjust_logits_workspace_size per shape: a pure function of it
-
 
 def _per_row(t: torch.Tensor, name: str, rows: int, dev) -> int:
     if t.dtype != torch.float32 or t.shape != (rows,) or t.device != dev or t.stride(0) != 1:
@@ -36,8 +34,8 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
     -inf where ``allowed`` (int32 words [rows, ceil(vocab / 32)], or [ceil(vocab
     / 32)] for all rows) has no bit.  ``out`` may be ``logits`` itself when it
     is contiguous fp32.  With ``record`` the history learns the tokens."""
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError(f"expected logits [rows, vocab], got {tuple(logits.shape)}")
+    if logits.dim() != 2 or not 0 < logits.shape[1] <= 1 << 20:
+        raise ValueError(f"expected logits [rows, vocab] with vocab at most 2^20, got {tuple(logits.shape)}")
     if logits.dtype not in _lib.DTYPE_CODES:
         raise TypeError(f"unsupported logits dtype {logits.dtype}")
     dev = logits.device
@@ -85,19 +83,13 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
     elif out.shape != (rows, vocab) or out.dtype != torch.float32 or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous float32 tensor of the logits' shape and device")
     nxt = logits.new_empty(rows, dtype=torch.int32)
-    lib = _lib.load()
-    key = (rows, vocab)
-    need = _WORKSPACE_BYTES.get(key)
-    if need is None:
-        need = _WORKSPACE_BYTES[key] = lib.gsq_adjust_logits_workspace_size(rows, vocab)
-    ws = out.new_empty(need // 4) if need else None  # this call's alone: the stream orders its next use
-    _lib.launch(dev, lib.gsq_adjust_logits, logits.data_ptr(), _lib.DTYPE_CODES[logits.dtype],
+    _lib.launch(dev, _lib.load().gsq_adjust_logits, logits.data_ptr(), _lib.DTYPE_CODES[logits.dtype],
                 max(logits.stride(0), vocab), rows, vocab, seen_ptr, counts_ptr,
                 None if repetition is None else _per_row(repetition, "repetition", rows, dev),
                 None if frequency is None else _per_row(frequency, "frequency", rows, dev),
                 None if presence is None else _per_row(presence, "presence", rows, dev),
                 bias_ids.data_ptr() if biases else None, bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
-                nxt.data_ptr(), int(record), ws.data_ptr() if need else None, need)
+                nxt.data_ptr(), int(record))
     return out, nxt
 
 
