@@ -10,13 +10,13 @@
 // cluster of up to 8 CTAs, each with a run of its tokens: one launch, in which
 // the CTAs' best tokens meet in distributed shared memory.  A thread takes
 // eight tokens at a time, as two 16-byte pieces where every row starts on such
-// a boundary, else one by one in neighbouring lanes.  The penalties run only
-// where a token's seen bit is set (some thousand of 248320 tokens), and only
-// there the counts are read.  Biased tokens are marked in a bit mask in shared
-// memory; the main pass leaves them without bias and mask and out of the
-// maximum, and a second pass over the list finishes them, each by the thread
-// of its first entry, which adds the token's biases in list order: no atomic
-// orders a sum.
+// a boundary, else one by one in neighbouring lanes, with the next eight on
+// their way.  That pass streams: it leaves the few tokens that the penalties or
+// a bias concern (some thousand of 248320) as they are, and out of the maximum.
+// A second pass gathers them from the bit masks into a queue for each warp and
+// works on them lane by lane, so that the scattered reads of their counts wait
+// together and not one after the other in the stream.  A token's biases are
+// added in list order by the thread that has the token: no atomic orders a sum.
 #include <cstdio>
 
 #include "gsq_common.cuh"
@@ -27,7 +27,8 @@ using namespace gsq;
 
 namespace {
 
-constexpr int LG_THREADS = 1024;          // of a CTA, at most
+constexpr int LG_THREADS = 512;           // of a CTA, at most
+constexpr int LG_QUEUE = 256;             // tokens of a warp's queue
 constexpr int LG_CLUSTER = 8;             // CTAs of a row, at most
 constexpr int64_t LG_VOCAB = 1ll << 20;   // tokens: the mask of a CTA's biased ones has a bit for each
 
@@ -64,19 +65,6 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   return k;
 }
 
-// Four tokens from v on, aligned for one load.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* f) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p);
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = to_f32(e[i]);
-  }
-}
-
 // The history of row r learns token v (bit and, for a generated token, count).
 __device__ __forceinline__ void remember(int32_t* seen, int32_t* counts, int64_t words, int64_t vocab, int64_t r,
                                          int64_t v, bool generated) {
@@ -89,10 +77,12 @@ __device__ __forceinline__ void cluster_sync_all() {
 }
 
 // VEC: the rows of logits and out start on 16-byte (two-byte types: 8-byte) boundaries, and vocab % 4 == 0.
-// BIAS: there are biases; dynamic shared memory: the mask of biased tokens of the CTA's run.
+// BIAS: there are biases. Dynamic shared memory: the warps' queues, with BIAS also the mask of the biased tokens of
+// the CTA's run.
 template <typename T, bool VEC, bool BIAS>
 __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) {
-  extern __shared__ uint32_t biased[];
+  extern __shared__ uint32_t queues[];
+  uint32_t* biased = queues + blockDim.x / 32 * LG_QUEUE;
   __shared__ unsigned long long part[LG_THREADS / 32], cta_best;
   pdl_launch_dependents();
   pdl_wait();
@@ -105,9 +95,6 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
   const int32_t* allowed_row = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
   const int32_t* ids = BIAS ? a.bias_ids + row * a.biases : nullptr;
   const int biases = (int)a.biases;
-  const float rep = a.repetition ? a.repetition[row] : 1.f;
-  const float freq = a.frequency ? a.frequency[row] : 0.f;
-  const float pres = a.presence ? a.presence[row] : 0.f;
   if constexpr (BIAS) {
     for (int i = tid; i < a.run / 32; i += blockDim.x) biased[i] = 0;
     __syncthreads();
@@ -121,66 +108,49 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
   unsigned long long best = 0;
   float top = -INFINITY;  // the thread's best so far
   int top_at = -1;
-  // Eight tokens of the thread and their mask words; the next eight are loaded while these are worked on.
+  // Eight tokens of the thread and their mask words, as they are loaded: the next eight, while these are worked on (any
+  // use would wait for them).
+  constexpr int PIECES = VEC ? 2 : 8;
   struct Group {
-    alignas(16) float z[8];
-    uint32_t seen[VEC ? 2 : 8], allowed[VEC ? 2 : 8];
+    alignas(16) T z[8];
+    uint32_t seen[PIECES], allowed[PIECES];
   };
   const int threads = blockDim.x, step = 8 * threads;
   auto token = [&](int v0, int e) { return VEC ? v0 + e / 4 * (4 * threads) + 4 * tid + e % 4 : v0 + e * threads + tid; };
   auto load = [&](int v0, Group& g) {
-    constexpr int N = VEC ? 2 : 8;
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const int v = token(v0, i * (8 / N));
-      const bool in = v < hi;
-      if constexpr (VEC) {
-        if (in) load4(x + v, g.z + 4 * i);
-        else g.z[4 * i] = g.z[4 * i + 1] = g.z[4 * i + 2] = g.z[4 * i + 3] = -INFINITY;
-      } else {
-        g.z[i] = in ? to_f32(x[v]) : -INFINITY;
+    for (int i = 0; i < PIECES; i++) {
+      const int v = token(v0, i * (8 / PIECES));
+      if (v < hi) {
+        if constexpr (!VEC) g.z[i] = x[v];
+        else if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(g.z)[i] = *reinterpret_cast<const uint4*>(x + v);
+        else reinterpret_cast<uint2*>(g.z)[i] = *reinterpret_cast<const uint2*>(x + v);
+        if (seen_row) g.seen[i] = seen_row[v >> 5];
+        if (allowed_row) g.allowed[i] = allowed_row[v >> 5];
       }
-      g.seen[i] = in && seen_row ? (uint32_t)seen_row[v >> 5] >> (v & 31) : 0u;
-      g.allowed[i] = in && allowed_row ? (uint32_t)allowed_row[v >> 5] >> (v & 31) : ~0u;
     }
   };
-  Group next;
+  Group next = {};
   load(lo, next);
   for (int v0 = lo; v0 < hi; v0 += step) {
-    Group g = next;
+    const Group g = next;
     if (v0 + step < hi) load(v0 + step, next);
-    float (&z)[8] = g.z;
-    uint32_t seen = 0, hidden = 0, late = 0;  // bit e: seen, not allowed, biased
-    if constexpr (VEC) {
-      seen = (g.seen[0] & 15u) | (g.seen[1] & 15u) << 4;
-      hidden = (~g.allowed[0] & 15u) | (~g.allowed[1] & 15u) << 4;
-    } else {
+    alignas(16) float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        seen |= (g.seen[e] & 1u) << e;
-        hidden |= (~g.allowed[e] & 1u) << e;
-      }
+    for (int e = 0; e < 8; e++) z[e] = token(v0, e) < hi ? to_f32(g.z[e]) : -INFINITY;
+    uint32_t late = 0, hidden = 0;  // bit e: seen or biased, not allowed
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      constexpr uint32_t MASK = VEC ? 15u : 1u;
+      const int v = token(v0, i * (8 / PIECES));
+      if (seen_row) late |= (g.seen[i] >> (v & 31) & MASK) << i * (8 / PIECES);
+      if (allowed_row) hidden |= (~g.allowed[i] >> (v & 31) & MASK) << i * (8 / PIECES);
     }
     if constexpr (BIAS) {
 #pragma unroll
       for (int i = 0; i < (VEC ? 2 : 8); i++) {
         const int v = token(v0, i * (VEC ? 4 : 1));
         if (v < hi) late |= (biased[(v - lo) >> 5] >> (v & 31) & (VEC ? 15u : 1u)) << i * (VEC ? 4 : 1);
-      }
-    }
-    if (seen) {
-      int32_t n[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) n[e] = seen >> e & 1 ? a.counts[row * vocab + token(v0, e)] : 0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        if (seen >> e & 1) {
-          z[e] = z[e] > 0.f ? __fdiv_rn(z[e], rep) : __fmul_rn(z[e], rep);
-          if (n[e] > 0) {
-            z[e] = __fsub_rn(z[e], __fmul_rn(freq, (float)n[e]));
-            z[e] = __fsub_rn(z[e], pres);
-          }
-        }
       }
     }
     hidden &= ~late;
@@ -199,7 +169,7 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
         if (token(v0, e) < hi) out[token(v0, e)] = z[e];
     }
     // the thread's best token: they rise with e, and those past the end are -inf and come after the others
-    if (BIAS && late) {
+    if (late) {
 #pragma unroll
       for (int e = 0; e < 8; e++) z[e] = late >> e & 1 ? -INFINITY : z[e];
     }
@@ -230,24 +200,70 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
     const unsigned long long k = (unsigned long long)order_key(top) << 32 | (uint32_t)~(uint32_t)top_at;
     best = k > best ? k : best;
   }
-  if constexpr (BIAS) {
-    __syncthreads();  // the main pass has written the biased tokens' values
-    const float* val = a.bias_values + row * a.biases;
-    for (int i = tid; i < biases; i += blockDim.x) {
-      const int id = ids[i];
-      if (id < lo || id >= hi) continue;
-      bool first = true;
-      for (int j = 0; j < i && first; j++) first = ids[j] != id;
-      if (!first) continue;
-      float s = 0.f;
-      for (int j = i; j < biases; j++)
-        if (ids[j] == id) s = __fadd_rn(s, val[j]);
-      float y = __fadd_rn(out[id], s);
-      if (allowed_row && !((uint32_t)allowed_row[id >> 5] >> (id & 31) & 1u)) y = -INFINITY;
-      out[id] = y;
-      const unsigned long long k = (unsigned long long)order_key(y) << 32 | (uint32_t)~(uint32_t)id;
-      best = k > best ? k : best;
+  if (BIAS || seen_row) {
+    __syncthreads();  // the values are written
+    uint32_t* queue = queues + (tid >> 5) * LG_QUEUE;
+    const float* val = BIAS ? a.bias_values + row * a.biases : nullptr;
+    const float rep = a.repetition ? a.repetition[row] : 1.f;
+    const float freq = a.frequency ? a.frequency[row] : 0.f;
+    const float pres = a.presence ? a.presence[row] : 0.f;
+    int queued = 0;
+    auto finish = [&]() {
+      __syncwarp();
+      for (int i = lane; i < queued; i += 32) {
+        const int v = queue[i];
+        float y = out[v];
+        if (seen_row && (uint32_t)seen_row[v >> 5] >> (v & 31) & 1u) {
+          const int32_t n = a.counts[row * vocab + v];
+          y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+          if (n > 0) {
+            y = __fsub_rn(y, __fmul_rn(freq, (float)n));
+            y = __fsub_rn(y, pres);
+          }
+        }
+        if (BIAS && biased[(v - lo) >> 5] >> (v & 31) & 1u) {
+          float s = 0.f;
+          for (int j = 0; j < biases; j++)
+            if (ids[j] == v) s = __fadd_rn(s, val[j]);
+          y = __fadd_rn(y, s);
+        }
+        if (allowed_row && !((uint32_t)allowed_row[v >> 5] >> (v & 31) & 1u)) y = -INFINITY;
+        out[v] = y;
+        const unsigned long long k = (unsigned long long)order_key(y) << 32 | (uint32_t)~(uint32_t)v;
+        best = k > best ? k : best;
+      }
+      __syncwarp();
+      queued = 0;
+    };
+    const int words = (hi - lo + 31) / 32, warps = blockDim.x / 32;
+    for (int w0 = (tid >> 5) * 32; w0 < words; w0 += 32 * warps) {
+      const int w = w0 + lane;
+      uint32_t bits = 0;
+      if (w < words) {
+        if (seen_row) bits = (uint32_t)seen_row[(lo >> 5) + w];
+        if constexpr (BIAS) bits |= biased[w];
+        if (hi - lo - 32 * w < 32) bits &= (1u << (hi - lo - 32 * w)) - 1;  // past the last token
+      }
+      // eight tokens of each word at a time: at most a queue full
+      while (__any_sync(0xffffffffu, bits)) {
+        const int mine = min(__popc(bits), 8);
+        int at = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, at, o);
+          if (lane >= o) at += u;
+        }
+        const int all = __shfl_sync(0xffffffffu, at, 31);
+        if (queued + all > LG_QUEUE) finish();
+        at += queued - mine;
+        for (int i = 0; i < mine; i++) {
+          queue[at + i] = lo + 32 * w + __ffs(bits) - 1;
+          bits &= bits - 1;
+        }
+        queued += all;
+      }
     }
+    finish();
   }
   best = warp_max(best);
   if (lane == 0) part[tid >> 5] = best;
@@ -295,18 +311,19 @@ int launched(cudaError_t rc, const char* what) {
 }
 
 template <typename T, bool VEC, bool BIAS>
-cudaError_t adjust_launch(dim3 grid, size_t smem, cudaStream_t st, const LogitsArgs& a) {
-  // a CTA for each SM or fewer: all the threads there can be; else smaller ones, which divide more evenly
-  const dim3 block(grid.x * grid.y <= 148 ? LG_THREADS : grid.x * grid.y <= 296 ? LG_THREADS / 2 : LG_THREADS / 4);
+cudaError_t adjust_launch(dim3 grid, dim3 block, size_t smem, cudaStream_t st, const LogitsArgs& a) {
   return a.cluster > 1 ? launch_pdl_cluster(adjust_kernel<T, VEC, BIAS>, grid, block, a.cluster, st, smem, a)
                        : launch_pdl(adjust_kernel<T, VEC, BIAS>, grid, block, smem, st, a);
 }
 
 template <typename T>
 cudaError_t adjust(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
-  const size_t smem = a.biases ? a.run / 8 : 0;
-  if (a.biases) return vec ? adjust_launch<T, true, true>(grid, smem, st, a) : adjust_launch<T, false, true>(grid, smem, st, a);
-  return vec ? adjust_launch<T, true, false>(grid, smem, st, a) : adjust_launch<T, false, false>(grid, smem, st, a);
+  // where there are few CTAs, large ones; many divide more evenly when they are small
+  const dim3 block(grid.x * grid.y <= 296 ? LG_THREADS : LG_THREADS / 2);
+  const size_t smem = block.x / 32 * LG_QUEUE * 4 + (a.biases ? a.run / 8 : 0);
+  if (a.biases)
+    return vec ? adjust_launch<T, true, true>(grid, block, smem, st, a) : adjust_launch<T, false, true>(grid, block, smem, st, a);
+  return vec ? adjust_launch<T, true, false>(grid, block, smem, st, a) : adjust_launch<T, false, false>(grid, block, smem, st, a);
 }
 
 bool al4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
@@ -350,7 +367,8 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
   a.next = next;
   a.record = record;
   // As many CTAs a row as fill the GPU once (six of them on an SM), so that a few rows get 8 and many get one; and
-  // no more than 2^18 tokens a CTA, whose mask of biased tokens is then at most 32 KB.
+  // no more than 2^18 tokens a CTA, whose mask of biased tokens is then at most 32 KB
+  // (and the queues 8, or with 2^17 tokens 16 + 16 KB).
   a.cluster = LG_CLUSTER;
   while (a.cluster > 1 && rows * a.cluster > 148 * 6 && vocab <= (1ll << 18) * (a.cluster / 2)) a.cluster /= 2;
   a.run = (int)((vocab + 128 * a.cluster - 1) / (128 * a.cluster) * 128);
