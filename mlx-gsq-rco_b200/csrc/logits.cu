@@ -10,13 +10,16 @@
 // cluster of up to 8 CTAs, each with a run of its tokens: one launch, in which
 // the CTAs' best tokens meet in distributed shared memory.  A thread takes
 // eight tokens at a time, as two 16-byte pieces where every row starts on such
-// a boundary, else one by one in neighbouring lanes, with the next eight on
-// their way.  That pass streams: it leaves the few tokens that the penalties or
+// a boundary, copied LG_STAGES - 1 steps ahead through shared memory (each
+// thread its own, so no barrier), else one by one in neighbouring lanes, one
+// step ahead in registers; the masks of the CTA's run are in shared memory from
+// the start.  That pass streams: it leaves the few tokens that the penalties or
 // a bias concern (some thousand of 248320) as they are, and out of the maximum.
 // A second pass gathers them from the bit masks into a queue for each warp and
 // works on them lane by lane, so that the scattered reads of their counts wait
 // together and not one after the other in the stream.  A token's biases are
 // added in list order by the thread that has the token: no atomic orders a sum.
+#include <atomic>
 #include <cstdio>
 
 #include "gsq_common.cuh"
@@ -29,6 +32,7 @@ namespace {
 
 constexpr int LG_THREADS = 512;           // of a CTA, at most
 constexpr int LG_QUEUE = 256;             // tokens of a warp's queue
+constexpr int LG_STAGES = 4;              // of a thread's eight tokens, on their way
 constexpr int LG_CLUSTER = 8;             // CTAs of a row, at most
 constexpr int64_t LG_VOCAB = 1ll << 20;   // tokens: the mask of a CTA's biased ones has a bit for each
 
@@ -72,85 +76,106 @@ __device__ __forceinline__ void remember(int32_t* seen, int32_t* counts, int64_t
   if (generated) atomicAdd(counts + r * vocab + v, 1);
 }
 
+// BYTES (8 or 16) of global memory to shared memory, asynchronously.
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // VEC: the rows of logits and out start on 16-byte (two-byte types: 8-byte) boundaries, and vocab % 4 == 0.
-// BIAS: there are biases. Dynamic shared memory: the warps' queues, with BIAS also the mask of the biased tokens of
-// the CTA's run.
-template <typename T, bool VEC, bool BIAS>
+// Dynamic shared memory: the masks of the CTA's run (tokens that the second pass finishes, allowed tokens), the warps'
+// queues, and with VEC the stages.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) {
-  extern __shared__ uint32_t queues[];
-  uint32_t* biased = queues + blockDim.x / 32 * LG_QUEUE;
+  extern __shared__ __align__(16) uint32_t smem[];
   __shared__ unsigned long long part[LG_THREADS / 32], cta_best;
   pdl_launch_dependents();
   pdl_wait();
   const int64_t row = blockIdx.y;
   const int vocab = (int)a.vocab, lo = blockIdx.x * a.run, hi = min(vocab, lo + a.run);
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, threads = blockDim.x, words = (max(hi - lo, 0) + 31) / 32;
+  uint32_t *late_mask = smem, *allowed_mask = smem + a.run / 32;
+  uint32_t* queue = smem + a.run / 16 + (tid >> 5) * LG_QUEUE;
   const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
   float* out = a.out + row * vocab;
   const int32_t* seen_row = a.seen ? a.seen + row * a.words : nullptr;
-  const int32_t* allowed_row = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  const int32_t* ids = BIAS ? a.bias_ids + row * a.biases : nullptr;
+  const int32_t* ids = a.biases ? a.bias_ids + row * a.biases : nullptr;
   const int biases = (int)a.biases;
-  if constexpr (BIAS) {
-    for (int i = tid; i < a.run / 32; i += blockDim.x) biased[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < biases; i += blockDim.x) {
-      const int id = ids[i];
-      if (id >= lo && id < hi) atomicOr(&biased[(id - lo) >> 5], 1u << (id & 31));  // lo % 32 == 0
+
+  // Eight tokens a step. token(v0, e): token e of this thread in the step that begins with v0.
+  const int step = 8 * threads;
+  auto token = [&](int v0, int e) { return VEC ? v0 + e / 4 * (4 * threads) + 4 * tid + e % 4 : v0 + e * threads + tid; };
+  constexpr int PIECE = 4 * sizeof(T);  // bytes of a copied piece
+  uint8_t* ring = reinterpret_cast<uint8_t*>(smem + a.run / 16 + threads / 32 * LG_QUEUE);
+  T next[VEC ? 1 : 8];
+  int ahead = lo, put = 0;
+  auto load = [&]() {  // the step `ahead`
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const int v = token(ahead, 4 * i);
+        if (v < hi) cp_async<PIECE>(ring + ((put * 2 + i) * threads + tid) * PIECE, x + v);
+      }
+      cp_async_commit();
+      put = put + 1 == LG_STAGES ? 0 : put + 1;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (token(ahead, e) < hi) next[e] = x[token(ahead, e)];
     }
-    __syncthreads();
+    ahead += step;
+  };
+#pragma unroll
+  for (int i = 0; i < (VEC ? LG_STAGES - 1 : 1); i++) load();
+
+  for (int w = tid; w < words; w += threads) {
+    late_mask[w] = seen_row ? (uint32_t)seen_row[(lo >> 5) + w] : 0u;  // lo % 32 == 0
+    allowed_mask[w] = a.allowed ? (uint32_t)a.allowed[row * a.allowed_stride + (lo >> 5) + w] : ~0u;
   }
+  if (biases) {
+    __syncthreads();
+    for (int i = tid; i < biases; i += threads) {
+      const int id = ids[i];
+      if (id >= lo && id < hi) atomicOr(&late_mask[(id - lo) >> 5], 1u << (id & 31));
+    }
+  }
+  __syncthreads();
 
   unsigned long long best = 0;
   float top = -INFINITY;  // the thread's best so far
-  int top_at = -1;
-  // Eight tokens of the thread and their mask words, as they are loaded: the next eight, while these are worked on (any
-  // use would wait for them).
-  constexpr int PIECES = VEC ? 2 : 8;
-  struct Group {
-    alignas(16) T z[8];
-    uint32_t seen[PIECES], allowed[PIECES];
-  };
-  const int threads = blockDim.x, step = 8 * threads;
-  auto token = [&](int v0, int e) { return VEC ? v0 + e / 4 * (4 * threads) + 4 * tid + e % 4 : v0 + e * threads + tid; };
-  auto load = [&](int v0, Group& g) {
-#pragma unroll
-    for (int i = 0; i < PIECES; i++) {
-      const int v = token(v0, i * (8 / PIECES));
-      if (v < hi) {
-        if constexpr (!VEC) g.z[i] = x[v];
-        else if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(g.z)[i] = *reinterpret_cast<const uint4*>(x + v);
-        else reinterpret_cast<uint2*>(g.z)[i] = *reinterpret_cast<const uint2*>(x + v);
-        if (seen_row) g.seen[i] = seen_row[v >> 5];
-        if (allowed_row) g.allowed[i] = allowed_row[v >> 5];
-      }
-    }
-  };
-  Group next = {};
-  load(lo, next);
+  int top_at = -1, get = 0;
   for (int v0 = lo; v0 < hi; v0 += step) {
-    const Group g = next;
-    if (v0 + step < hi) load(v0 + step, next);
+    alignas(16) T raw[8];
+    if constexpr (VEC) {
+      load();
+      cp_async_wait<LG_STAGES - 1>();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const uint8_t* p = ring + ((get * 2 + i) * threads + tid) * PIECE;
+        if constexpr (PIECE == 16) reinterpret_cast<uint4*>(raw)[i] = *reinterpret_cast<const uint4*>(p);
+        else reinterpret_cast<uint2*>(raw)[i] = *reinterpret_cast<const uint2*>(p);
+      }
+      get = get + 1 == LG_STAGES ? 0 : get + 1;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) raw[e] = next[e];
+      load();
+    }
     alignas(16) float z[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) z[e] = token(v0, e) < hi ? to_f32(g.z[e]) : -INFINITY;
-    uint32_t late = 0, hidden = 0;  // bit e: seen or biased, not allowed
+    for (int e = 0; e < 8; e++) z[e] = token(v0, e) < hi ? to_f32(raw[e]) : -INFINITY;
+    uint32_t late = 0, hidden = 0;  // bit e: for the second pass, not allowed
 #pragma unroll
-    for (int i = 0; i < PIECES; i++) {
-      constexpr uint32_t MASK = VEC ? 15u : 1u;
-      const int v = token(v0, i * (8 / PIECES));
-      if (seen_row) late |= (g.seen[i] >> (v & 31) & MASK) << i * (8 / PIECES);
-      if (allowed_row) hidden |= (~g.allowed[i] >> (v & 31) & MASK) << i * (8 / PIECES);
-    }
-    if constexpr (BIAS) {
-#pragma unroll
-      for (int i = 0; i < (VEC ? 2 : 8); i++) {
-        const int v = token(v0, i * (VEC ? 4 : 1));
-        if (v < hi) late |= (biased[(v - lo) >> 5] >> (v & 31) & (VEC ? 15u : 1u)) << i * (VEC ? 4 : 1);
+    for (int i = 0; i < (VEC ? 2 : 8); i++) {
+      constexpr int N = VEC ? 4 : 1;
+      const int v = token(v0, i * N);
+      if (v < hi) {
+        late |= (late_mask[(v - lo) >> 5] >> (v & 31) & ((1u << N) - 1)) << i * N;
+        hidden |= (~allowed_mask[(v - lo) >> 5] >> (v & 31) & ((1u << N) - 1)) << i * N;
       }
     }
     hidden &= ~late;
@@ -200,20 +225,20 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
     const unsigned long long k = (unsigned long long)order_key(top) << 32 | (uint32_t)~(uint32_t)top_at;
     best = k > best ? k : best;
   }
-  if (BIAS || seen_row) {
+  if (biases || seen_row) {
     __syncthreads();  // the values are written
-    uint32_t* queue = queues + (tid >> 5) * LG_QUEUE;
-    const float* val = BIAS ? a.bias_values + row * a.biases : nullptr;
+    const float* val = biases ? a.bias_values + row * a.biases : nullptr;
     const float rep = a.repetition ? a.repetition[row] : 1.f;
     const float freq = a.frequency ? a.frequency[row] : 0.f;
     const float pres = a.presence ? a.presence[row] : 0.f;
     int queued = 0;
     auto finish = [&]() {
       __syncwarp();
-      for (int i = lane; i < queued; i += 32) {
-        const int v = queue[i];
-        float y = out[v];
-        if (seen_row && (uint32_t)seen_row[v >> 5] >> (v & 31) & 1u) {
+      for (int i0 = 0; i0 < queued; i0 += 32) {
+        const bool mine = i0 + lane < queued;
+        const int v = mine ? (int)queue[i0 + lane] : -1;
+        float y = mine ? out[v] : 0.f;
+        if (mine && seen_row && (uint32_t)seen_row[v >> 5] >> (v & 31) & 1u) {
           const int32_t n = a.counts[row * vocab + v];
           y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
           if (n > 0) {
@@ -221,13 +246,28 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
             y = __fsub_rn(y, pres);
           }
         }
-        if (BIAS && biased[(v - lo) >> 5] >> (v & 31) & 1u) {
+        if (biases) {
+          // the list against the warp's tokens, 32 entries at a time, each token's sum in the list's order
           float s = 0.f;
-          for (int j = 0; j < biases; j++)
-            if (ids[j] == v) s = __fadd_rn(s, val[j]);
-          y = __fadd_rn(y, s);
+          bool any = false;
+          for (int j0 = 0; j0 < biases; j0 += 32) {
+            const int id = j0 + lane < biases ? ids[j0 + lane] : -1;
+            const float b = j0 + lane < biases ? val[j0 + lane] : 0.f;
+            unsigned here = __ballot_sync(0xffffffffu, id >= lo && id < hi);
+            while (here) {
+              const int l = __ffs(here) - 1;
+              here &= here - 1;
+              const float one = __shfl_sync(0xffffffffu, b, l);
+              if (__shfl_sync(0xffffffffu, id, l) == v) {
+                s = __fadd_rn(s, one);
+                any = true;
+              }
+            }
+          }
+          if (any) y = __fadd_rn(y, s);
         }
-        if (allowed_row && !((uint32_t)allowed_row[v >> 5] >> (v & 31) & 1u)) y = -INFINITY;
+        if (!mine) continue;
+        if (!(allowed_mask[(v - lo) >> 5] >> (v & 31) & 1u)) y = -INFINITY;
         out[v] = y;
         const unsigned long long k = (unsigned long long)order_key(y) << 32 | (uint32_t)~(uint32_t)v;
         best = k > best ? k : best;
@@ -235,15 +275,10 @@ __global__ void __launch_bounds__(LG_THREADS) adjust_kernel(const LogitsArgs a) 
       __syncwarp();
       queued = 0;
     };
-    const int words = (hi - lo + 31) / 32, warps = blockDim.x / 32;
-    for (int w0 = (tid >> 5) * 32; w0 < words; w0 += 32 * warps) {
+    for (int w0 = (tid >> 5) * 32; w0 < words; w0 += threads) {
       const int w = w0 + lane;
-      uint32_t bits = 0;
-      if (w < words) {
-        if (seen_row) bits = (uint32_t)seen_row[(lo >> 5) + w];
-        if constexpr (BIAS) bits |= biased[w];
-        if (hi - lo - 32 * w < 32) bits &= (1u << (hi - lo - 32 * w)) - 1;  // past the last token
-      }
+      uint32_t bits = w < words ? late_mask[w] : 0u;
+      if (w < words && hi - lo - 32 * w < 32) bits &= (1u << (hi - lo - 32 * w)) - 1;  // past the last token
       // eight tokens of each word at a time: at most a queue full
       while (__any_sync(0xffffffffu, bits)) {
         const int mine = min(__popc(bits), 8);
@@ -310,20 +345,29 @@ int launched(cudaError_t rc, const char* what) {
   return fail(GSQ_ERR_CUDA, buf);
 }
 
-template <typename T, bool VEC, bool BIAS>
-cudaError_t adjust_launch(dim3 grid, dim3 block, size_t smem, cudaStream_t st, const LogitsArgs& a) {
-  return a.cluster > 1 ? launch_pdl_cluster(adjust_kernel<T, VEC, BIAS>, grid, block, a.cluster, st, smem, a)
-                       : launch_pdl(adjust_kernel<T, VEC, BIAS>, grid, block, smem, st, a);
+template <typename T, bool VEC>
+cudaError_t adjust_launch(dim3 grid, cudaStream_t st, const LogitsArgs& a) {
+  // where there are few CTAs, large ones; many divide more evenly when they are small
+  const dim3 block(grid.x * grid.y <= 296 ? LG_THREADS : LG_THREADS / 2);
+  const size_t smem = a.run / 4 + block.x / 32 * LG_QUEUE * 4 + (VEC ? LG_STAGES * block.x * 8 * sizeof(T) : 0);
+  // (at most 2^18 tokens a CTA: 64 KB of masks)
+  auto kernel = adjust_kernel<T, VEC>;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  return a.cluster > 1 ? launch_pdl_cluster(kernel, grid, block, a.cluster, st, smem, a)
+                       : launch_pdl(kernel, grid, block, smem, st, a);
 }
 
 template <typename T>
 cudaError_t adjust(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
-  // where there are few CTAs, large ones; many divide more evenly when they are small
-  const dim3 block(grid.x * grid.y <= 296 ? LG_THREADS : LG_THREADS / 2);
-  const size_t smem = block.x / 32 * LG_QUEUE * 4 + (a.biases ? a.run / 8 : 0);
-  if (a.biases)
-    return vec ? adjust_launch<T, true, true>(grid, block, smem, st, a) : adjust_launch<T, false, true>(grid, block, smem, st, a);
-  return vec ? adjust_launch<T, true, false>(grid, block, smem, st, a) : adjust_launch<T, false, false>(grid, block, smem, st, a);
+  return vec ? adjust_launch<T, true>(grid, st, a) : adjust_launch<T, false>(grid, st, a);
 }
 
 bool al4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
@@ -366,11 +410,10 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
   a.out = out;
   a.next = next;
   a.record = record;
-  // As many CTAs a row as fill the GPU once (six of them on an SM), so that a few rows get 8 and many get one; and
-  // no more than 2^18 tokens a CTA, whose mask of biased tokens is then at most 32 KB
-  // (and the queues 8, or with 2^17 tokens 16 + 16 KB).
+  // As many CTAs a row as fill the GPU once (four of them on an SM), so that a few rows get 8 and many get one; and no
+  // more than 2^18 tokens a CTA.
   a.cluster = LG_CLUSTER;
-  while (a.cluster > 1 && rows * a.cluster > 148 * 6 && vocab <= (1ll << 18) * (a.cluster / 2)) a.cluster /= 2;
+  while (a.cluster > 1 && rows * a.cluster > 148 * 4 && vocab <= (1ll << 18) * (a.cluster / 2)) a.cluster /= 2;
   a.run = (int)((vocab + 128 * a.cluster - 1) / (128 * a.cluster) * 128);
   const dim3 grid((unsigned)a.cluster, (unsigned)rows);
   cudaStream_t st = (cudaStream_t)stream;
