@@ -19,8 +19,9 @@
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs.
 // Roles (20 warps): two softmax warpgroups that take the tiles in turn, one
-// row a thread; two that dequantise; one warp issues. S of the next two tiles
-// is issued before P V of this one, so that two tiles are in the softmax
+// row a thread; two that dequantise; one thread issues the products, one the
+// bulk copies of codes (a tile is one contiguous piece). S of the next two
+// tiles is issued before P V of this one, so that two tiles are in the softmax
 // while the tensor core works on their neighbours; what the two groups share
 // is each row's reference (the running maximum), passed from tile to tile.
 // The reference is followed lazily: O is rescaled only when it grows by more
@@ -36,15 +37,17 @@ namespace gsq {
 
 constexpr int AR_M = 128, AR_TILE = 64;
 constexpr int AR_GROUP = 4, AR_SOFTMAX = 2 * AR_GROUP, AR_DEQUANT = 8;  // warps
-constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four one issues, the others end its warpgroup
+constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four one issues products, one copies
 
 template <int D>
 struct ArGeom {
   static constexpr int ITEM = AR_TILE * D * 2;  // one K or V tile in fp16
-  static constexpr int STAGES = 6;
+  static constexpr int STAGES = D == 256 ? 5 : 6;
+  static constexpr int RAW = AR_TILE * D;       // its codes
+  static constexpr int RAWS = 3;
   static constexpr int SCALES = AR_SOFTMAX * 5 * AR_TILE * 4;
   static constexpr int STATE = 3 * AR_M * 4;    // references, and the two groups' sums
-  static constexpr int SMEM = 1024 + STAGES * ITEM + SCALES + STATE + 512;
+  static constexpr int SMEM = 1024 + STAGES * ITEM + RAWS * RAW + SCALES + STATE + 512;
   static constexpr int O = 0, Q = D, S = Q + D / 2, P = S + AR_TILE;  // TMEM columns
   static constexpr int COLS = 512;
   static_assert(P + AR_TILE <= COLS && SMEM <= 227 * 1024, "fits");
@@ -121,17 +124,17 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// MN-major operand, 128-byte swizzle: rows of 64 values, 8 rows (of K) 1024 bytes apart from the next 8, the next 64
-// values of MN `lbo` bytes on.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t lbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)(lbo >> 4) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
+// Shared-memory descriptors with 128-byte swizzle, of which only the low word depends on the address (in 16-byte units):
+// K-major (8 rows of 128 bytes 1024 bytes apart from the next 8), and MN-major (rows of 64 values, 8 rows of K 1024
+// bytes apart from the next 8, the next 64 values of MN `lbo` bytes on).
+constexpr uint32_t AR_DESC_HI = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint64_t ar_desc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(AR_DESC_HI));
   return d;
 }
+__device__ __forceinline__ uint32_t ar_k_major(uint32_t saddr) { return (saddr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t ar_mn_major(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
 // D = fp32, A = B = fp16, M = 128; B K-major or MN-major.
 __host__ __device__ constexpr uint32_t ar_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AR_M >> 4) << 24);
@@ -183,12 +186,12 @@ __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const S
   return m & below(s.len - p0);
 }
 
-// Scales of two positions of a tile a lane, as the softmax uses them: keys' scales, log2 of the values' and its
-// inverse in linear terms, in the warp's own copy.
+// Scales of two positions of a tile a lane, as the softmax uses them: the keys' times `factor`, log2 of the values' and
+// its inverse in linear terms, in the warp's own copy.
 struct ArZeros {
   uint32_t even, odd;  // bit i: the value scale of position 2i (2i + 1) is 0
 };
-__device__ __forceinline__ ArZeros ar_scales(float* ks, float2 k2, float2 v2) {
+__device__ __forceinline__ ArZeros ar_scales(float* ks, float factor, float2 k2, float2 v2) {
   const int lane = threadIdx.x & 31;
   // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of scale 0 has
   // no part in the output, but in the sum of weights: it is weighted with the largest scale of the tile, and that
@@ -205,23 +208,22 @@ __device__ __forceinline__ ArZeros ar_scales(float* ks, float2 k2, float2 v2) {
   }
   lx = v2.x > 0.f ? lx : v2.x == 0.f ? top : v2.x;  // NaN stays
   ly = v2.y > 0.f ? ly : v2.y == 0.f ? top : v2.y;
-  *reinterpret_cast<float2*>(ks + 2 * lane) = k2;
+  *reinterpret_cast<float2*>(ks + 2 * lane) = make_float2(k2.x * factor, k2.y * factor);
   *reinterpret_cast<float2*>(ks + AR_TILE + 2 * lane) = make_float2(lx, ly);
   *reinterpret_cast<float2*>(ks + 2 * AR_TILE + 2 * lane) = make_float2(exp2_approx(-lx), exp2_approx(-ly));
   return z;
 }
 
-// s: raw scores of a row -> t = factor * ks * s + log2 vs; -inf where a bit of `see` is off (EDGE). Returns the maximum.
+// s: raw scores of a row -> t = ks * s + log2 vs; -inf where a bit of `see` is off (EDGE). Returns the maximum.
 template <bool EDGE>
-__device__ __forceinline__ float ar_scores(float2 (&s)[AR_TILE / 2], const float* ks, float factor, uint64_t see) {
-  const float2 f2 = make_float2(factor, factor);
+__device__ __forceinline__ float ar_scores(float2 (&s)[AR_TILE / 2], const float* ks, uint64_t see) {
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int e = 0; e < AR_TILE; e += 4) {
     const float4 k4 = *reinterpret_cast<const float4*>(ks + e);
     const float4 v4 = *reinterpret_cast<const float4*>(ks + AR_TILE + e);
-    float2 x = fma2(mul2(s[e / 2], make_float2(k4.x, k4.y)), f2, make_float2(v4.x, v4.y));
-    float2 y = fma2(mul2(s[e / 2 + 1], make_float2(k4.z, k4.w)), f2, make_float2(v4.z, v4.w));
+    float2 x = fma2(s[e / 2], make_float2(k4.x, k4.y), make_float2(v4.x, v4.y));
+    float2 y = fma2(s[e / 2 + 1], make_float2(k4.z, k4.w), make_float2(v4.z, v4.w));
     if constexpr (EDGE) {
       x.x = see >> e & 1 ? x.x : -INFINITY;
       x.y = see >> (e + 1) & 1 ? x.y : -INFINITY;
@@ -269,10 +271,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
   using G = ArGeom<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* scales = reinterpret_cast<float*>(smem + G::STAGES * G::ITEM);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][64]
+  uint8_t* raw = smem + G::STAGES * G::ITEM;
+  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][64]
   float* refs = scales + G::SCALES / 4;                                   // [128], base-2 exponents
   float* sums = refs + AR_M;                                              // [group][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::STAGES * G::ITEM + G::SCALES + G::STATE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sums + 2 * AR_M);
   uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
   uint64_t* empty = full + G::STAGES;     // [STAGES] commit
   uint64_t* s_full = empty + G::STAGES;   // [group] commit
@@ -283,8 +286,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
   uint64_t* ref_done = q_full + 1;        // [32 rows] count 1: the references are those of one more tile
   uint64_t* sum_done = ref_done + 4;      // [32 rows] count 2: both groups' sums are there
   uint64_t* drained = sum_done + 4;       // commit
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
-  static_assert((2 * G::STAGES + 17) * 8 + 4 <= 512, "barriers");
+  uint64_t* raw_full = drained + 1;       // [RAWS] the copy
+  uint64_t* raw_empty = raw_full + G::RAWS;  // [RAWS] count AR_DEQUANT
+  int* raw_rows = reinterpret_cast<int*>(raw_empty + G::RAWS);  // [RAWS] positions in the stage
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_rows + G::RAWS);
+  static_assert((2 * G::STAGES + 17 + 2 * G::RAWS) * 8 + 4 * G::RAWS + 4 <= 512, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == AR_SOFTMAX + AR_DEQUANT) tmem_alloc(tmem_slot, G::COLS);
@@ -305,6 +311,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       mbar_init(&sum_done[i], 2);
     }
     mbar_init(drained, 1);
+    for (int i = 0; i < G::RAWS; i++) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], AR_DEQUANT);
+    }
     fence_mbar_init();
   }
   tc_fence_before();
@@ -337,18 +347,22 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     do {
       const int r = run.at.mb * AR_M + row;  // row of the unit's head
       const int i = r / a.group;
-      // Q: the row in fp16 (bf16: times a power of two), 16 dimensions in 8 columns; a half of it by each group
+      // Q: the row in fp16, 16 dimensions in 8 columns; a half of it by each group. bf16: times a power of two that
+      // fits the largest of the warp's rows, so that one factor serves them all (what a row 2^27 times smaller loses
+      // is far below the rounding of its neighbours' scores, and its own are as much smaller). Padding counts as 0.
+      const int r_load = i < run.at.span.count ? r : rows;
       int shift = 0;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         float amax = 0.f;
 #pragma unroll 4
         for (int d = 0; d < D; d += 8) {
           float f[8];
-          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r, d), f);
+          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r_load, d), f);
 #pragma unroll
           for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(f[e]));
         }
-        shift = q_shift(amax);
+        amax = amax <= 3.4e38f ? amax : 0.f;  // a row with an infinity is lost by itself
+        shift = q_shift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))));
       }
       const float up = (a.scale < 0.f ? -1.f : 1.f) * exp2_int(shift);
       const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);
@@ -358,7 +372,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 #pragma unroll
         for (int d = 0; d < 64; d += 8) {
           float f[8];
-          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r, 64 * c + d), f);
+          q8_values<T>(load_q8<T>(a, run.at.b, run.at.kh, r_load, 64 * c + d), f);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const __half2 h = __floats2half2_rn(f[2 * e] * up, f[2 * e + 1] * up);
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         const int p0 = (run.at.tile + tile - run0) * AR_TILE;
         cp_async_wait<0>();
         __syncwarp();  // this tile's are there, and the warp has read the last tile's
-        const ArZeros zeros = ar_scales(ks, *reinterpret_cast<const float2*>(ks + 3 * AR_TILE + 2 * lane),
+        const ArZeros zeros = ar_scales(ks, factor, *reinterpret_cast<const float2*>(ks + 3 * AR_TILE + 2 * lane),
                                         *reinterpret_cast<const float2*>(ks + 4 * AR_TILE + 2 * lane));
         __syncwarp();
         if (tile + 2 < run0 + run.len) fetch_scales(p0 + 2 * AR_TILE);
@@ -410,7 +424,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 
         const bool edge = p0 + AR_TILE > min(run.at.span.base, run.at.span.len);  // the same for all threads
         const uint64_t see = edge ? ar_visible(a, run.at.b, run.at.span, i, p0) : ~0ull;
-        const float top = edge ? ar_scores<true>(s, ks, factor, see) : ar_scores<false>(s, ks, factor, see);
+        const float top = edge ? ar_scores<true>(s, ks, see) : ar_scores<false>(s, ks, see);
         // the reference after the last tile, which the other group has set
         if (tile > run0) {
           ok = warp_wait(&ref_done[quarter], (uint32_t)((tile - 1) & 1), a.err);
@@ -516,7 +530,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       tc_fence_before();  // the loads of O come before the next unit's products (through q_full)
     } while (run.next(a));
   } else if (warp < AR_SOFTMAX + AR_DEQUANT) {
-    // ---------------- dequantise: items in the order K0, K1, K2, V0, K3, V1, .. of each run ----------------
+    // ---------------- dequantise ----------------
     // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
     // swizzled row. Rows of one lane differ by multiples of 8, so its swizzle is a constant.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -526,114 +540,118 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     constexpr int STEPS = AR_TILE / (8 * RPW);
     const int row = w * RPW + lane / LPR, chunk = lane % LPR;  // + 8 RPW per step
     const uint32_t dst = (uint32_t)(chunk / 8 * (AR_TILE * 128) + row * 128 + ((chunk % 8) ^ (row & 7)) * 16);
-    ArRun run;
-    run.begin(a, first, last);
-    int kpos = 0, vpos = 0;
-    bool more = true;
-    uint2 ahead[2][STEPS];
-    // Loads the next item's codes; zeros past the sequence's end.
-    auto load = [&](uint2 (&c)[STEPS]) {
-      if (!more) return;
-      const bool key = kpos < run.len && kpos - vpos < 3;
-      const int j = key ? kpos++ : vpos++;
-      const int p0 = (run.at.tile + j) * AR_TILE + row, left = run.at.span.len - p0;
-      const uint8_t* src = (key ? a.kc : a.vc) + (((int64_t)run.at.b * a.kv + run.at.kh) * a.cap + p0) * D + chunk * 8;
-#pragma unroll
-      for (int i = 0; i < STEPS; i++)
-        c[i] = i * 8 * RPW < left ? *reinterpret_cast<const uint2*>(src + (int64_t)i * 8 * RPW * D) : make_uint2(0u, 0u);
-      if (vpos == run.len) {
-        more = run.next(a);
-        kpos = vpos = 0;
-      }
-    };
     const int items = 2 * (last - first);
-    load(ahead[0]);
-    load(ahead[1]);
-    int stage = 0, use = 0;
-    for (int it = 0; it < items && ok; it += 2) {
+    int stage = 0, use = 0, rs = 0, ruse = 0;
+    for (int it = 0; it < items; it++) {
+      ok = warp_wait(&raw_full[rs], (uint32_t)(ruse & 1), a.err);
+      if (!ok) break;
+      const uint8_t* src = raw + rs * G::RAW + row * D + chunk * 8;
+      uint2 c[STEPS];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        if (use > 0) ok = ok && warp_wait(&empty[stage], (uint32_t)((use - 1) & 1), a.err);
-        if (!ok) break;
-        uint8_t* p = smem + stage * G::ITEM + dst;
+      for (int i = 0; i < STEPS; i++) c[i] = *reinterpret_cast<const uint2*>(src + i * 8 * RPW * D);
+      const int there = raw_rows[rs] - row;  // rows past the sequence's end: zeros
+      if (raw_rows[rs] < AR_TILE) {
 #pragma unroll
-        for (int i = 0; i < STEPS; i++) {
-          uint4 v;
-          codes_to_half2<FMT>(ahead[h][i].x, v.x, v.y);
-          codes_to_half2<FMT>(ahead[h][i].y, v.z, v.w);
-          *reinterpret_cast<uint4*>(p + i * 8 * RPW * 128) = v;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[stage]);
-        load(ahead[h]);  // after the arrival, which as a release waits for the loads before it
-        if (++stage == G::STAGES) {
-          stage = 0;
-          use++;
-        }
+        for (int i = 0; i < STEPS; i++)
+          if (i * 8 * RPW >= there) c[i] = make_uint2(0u, 0u);
       }
+      if (use > 0) {
+        ok = warp_wait(&empty[stage], (uint32_t)((use - 1) & 1), a.err);
+        if (!ok) break;
+      }
+      uint8_t* p = smem + stage * G::ITEM + dst;
+#pragma unroll
+      for (int i = 0; i < STEPS; i++) {
+        uint4 v;
+        codes_to_half2<FMT>(c[i].x, v.x, v.y);
+        codes_to_half2<FMT>(c[i].y, v.z, v.w);
+        *reinterpret_cast<uint4*>(p + i * 8 * RPW * 128) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[stage]);
+        mbar_arrive(&raw_empty[rs]);
+      }
+      if (++stage == G::STAGES) stage = 0, use++;
+      if (++rs == G::RAWS) rs = 0, ruse++;
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-    if (warp == AR_SOFTMAX + AR_DEQUANT) {
-    // ---------------- issue ----------------
     ArRun run;
-    run.begin(a, first, last);
-    if (lane == 0) ArList::note(a, blockIdx.x, first, run.at, total, ctas);
-    int stage = 0, use = 0, tile = 0, runs = 0;
-    auto next_item = [&]() {
-      if (++stage == G::STAGES) {
-        stage = 0;
-        use++;
-      }
-    };
-    // S of the CTA's tile t: into TMEM when the softmax has taken tile t - 1's
-    auto scores = [&](int t) {
-      ok = warp_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
-           (t == 0 || warp_wait(s_free, (uint32_t)((t - 1) & 1), a.err));
-      if (!ok) return;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t b = smem_u32(smem + stage * G::ITEM);
+    if (warp < AR_SOFTMAX + AR_DEQUANT + 2) run.begin(a, first, last);
+    if (warp == AR_SOFTMAX + AR_DEQUANT && lane == 0) {
+      // ---------------- issue the products: one thread ----------------
+      ArList::note(a, blockIdx.x, first, run.at, total, ctas);
+      int stage = 0, use = 0, tile = 0, runs = 0;
+      const uint32_t items = smem_u32(smem);
+      // S of the CTA's tile t: into TMEM when the softmax has taken tile t - 1's
+      auto scores = [&](int t) {
+        ok = mbar_wait_bounded(&full[stage], (uint32_t)(use & 1), a.err) &&
+             (t == 0 || mbar_wait_bounded(s_free, (uint32_t)((t - 1) & 1), a.err));
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t b = ar_k_major(items + stage * G::ITEM);
 #pragma unroll
         for (int k = 0; k < D / 16; k++)
-          tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, sw128_desc(b + k / 4 * (AR_TILE * 128) + k % 4 * 32),
+          tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, ar_desc(b + k / 4 * (AR_TILE * 128 / 16) + k % 4 * 2),
                         ar_idesc(AR_TILE, false), k != 0);
         tc_commit(&empty[stage]);
         tc_commit(&s_full[t & 1]);
-      }
-      __syncwarp();
-      next_item();
-    };
-    do {
-      ok = warp_wait(q_full, (uint32_t)(runs++ & 1), a.err);
-      if (!ok) break;
-      scores(tile);
-      if (ok && run.len > 1) scores(tile + 1);
-      for (int j = 0; j < run.len && ok; j++, tile++) {
-        if (j + 2 < run.len) scores(tile + 2);
-        ok = ok && warp_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
-             warp_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
+        if (++stage == G::STAGES) stage = 0, use++;
+      };
+      do {
+        ok = mbar_wait_bounded(q_full, (uint32_t)(runs++ & 1), a.err);
         if (!ok) break;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t b = smem_u32(smem + stage * G::ITEM);
+        scores(tile);
+        if (ok && run.len > 1) scores(tile + 1);
+        for (int j = 0; j < run.len && ok; j++, tile++) {
+          if (j + 2 < run.len) scores(tile + 2);
+          ok = ok && mbar_wait_bounded(&full[stage], (uint32_t)(use & 1), a.err) &&
+               mbar_wait_bounded(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = ar_mn_major(items + stage * G::ITEM, AR_TILE * 128);
+          const uint32_t p = tmem + G::P + (tile & 1) * (AR_TILE / 2);
 #pragma unroll
           for (int k = 0; k < AR_TILE / 16; k++)
-            tc_mma_f16_ts(tmem + G::O, tmem + G::P + (tile & 1) * (AR_TILE / 2) + 8 * k,
-                          sw128_mn_desc(b + k * 2048, AR_TILE * 128), ar_idesc(D, true), j + k != 0);
+            tc_mma_f16_ts(tmem + G::O, p + 8 * k, ar_desc(b + k * (2048 / 16)), ar_idesc(D, true), (j | k) != 0);
           tc_commit(&empty[stage]);
           tc_commit(&pv_done[tile & 1]);
+          if (++stage == G::STAGES) stage = 0, use++;
         }
-        __syncwarp();
-        next_item();
+      } while (ok && run.next(a));
+      // nothing may still write TMEM when it is given back
+      tc_commit(drained);
+      mbar_wait_bounded(drained, 0, a.err);
+    } else if (warp == AR_SOFTMAX + AR_DEQUANT + 1 && lane == 0) {
+      // ---------------- copy the codes: one thread; items in the order K0, K1, K2, V0, K3, V1, .. of each run --------
+      int rs = 0, ruse = 0, kpos = 0, vpos = 0;
+      const int items = 2 * (last - first);
+      for (int it = 0; it < items; it++) {
+        if (ruse > 0) {
+          ok = mbar_wait_bounded(&raw_empty[rs], (uint32_t)((ruse - 1) & 1), a.err);
+          if (!ok) break;
+        }
+        const bool key = kpos < run.len && kpos - vpos < 3;
+        const int p0 = (run.at.tile + (key ? kpos++ : vpos++)) * AR_TILE, n = min(run.at.span.len - p0, AR_TILE);
+        raw_rows[rs] = n;
+        mbar_arrive_expect_tx(&raw_full[rs], n * D);
+        bulk_g2s(raw + rs * G::RAW, (key ? a.kc : a.vc) + (((int64_t)run.at.b * a.kv + run.at.kh) * a.cap + p0) * D, n * D,
+                 &raw_full[rs]);
+        if (++rs == G::RAWS) rs = 0, ruse++;
+        if (vpos == run.len && it + 1 < items) {
+          run.next(a);
+          kpos = vpos = 0;
+        }
       }
-    } while (ok && run.next(a));
-    // nothing may still write TMEM when it is given back
-    if (lane == 0) tc_commit(drained);
-    __syncwarp();
-    warp_wait(drained, 0, a.err);
+      // no copy may still be under way when the CTA ends (after a wait that gave up, one may be)
+      for (int i = 0; i < G::RAWS; i++) {
+        const int uses = ruse + (i < rs ? 1 : 0);
+        if (uses > 0) mbar_wait_bounded(&raw_full[i], (uint32_t)((uses - 1) & 1), a.err);
+      }
     }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
