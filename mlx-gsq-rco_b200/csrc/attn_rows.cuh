@@ -140,30 +140,47 @@ __host__ __device__ constexpr uint32_t ar_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AR_M >> 4) << 24);
 }
 
-// Pairs of fp32 in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 c;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+// Pairs of fp32 in one register pair and one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float x, float y) {
+  f32x2 p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 halves(f32x2 p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 c;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c) : "l"(a), "l"(b));
   return c;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 c;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return c;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}\n"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
   return d;
 }
 
+// mbar_wait_bounded with the clock read every 64 tries only: a waiting warp leaves the issue slots to the others (the
+// waits were a quarter of this kernel's instructions).
+__device__ __forceinline__ bool ar_wait(uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; i++)
+      if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    if (clock64() - t0 > (1ll << 31)) {
+      if (err) atomicExch(err, DEV_WAIT_TIMEOUT);
+      return false;
+    }
+  }
+}
 // A bounded wait of a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, err));
+  return __all_sync(0xffffffffu, ar_wait(bar, parity, err));
 }
 
 // Which of positions p0 .. p0 + 63 token i of sequence b sees, as bits.
@@ -216,22 +233,23 @@ __device__ __forceinline__ ArZeros ar_scales(float* ks, float factor, float2 k2,
 
 // s: raw scores of a row -> t = ks * s + log2 vs; -inf where a bit of `see` is off (EDGE). Returns the maximum.
 template <bool EDGE>
-__device__ __forceinline__ float ar_scores(float2 (&s)[AR_TILE / 2], const float* ks, uint64_t see) {
+__device__ __forceinline__ float ar_scores(f32x2 (&s)[AR_TILE / 2], const float* ks, uint64_t see) {
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int e = 0; e < AR_TILE; e += 4) {
-    const float4 k4 = *reinterpret_cast<const float4*>(ks + e);
-    const float4 v4 = *reinterpret_cast<const float4*>(ks + AR_TILE + e);
-    float2 x = fma2(s[e / 2], make_float2(k4.x, k4.y), make_float2(v4.x, v4.y));
-    float2 y = fma2(s[e / 2 + 1], make_float2(k4.z, k4.w), make_float2(v4.z, v4.w));
+    const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + e);
+    const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(ks + AR_TILE + e);
+    s[e / 2] = fma2(s[e / 2], k4.x, v4.x);
+    s[e / 2 + 1] = fma2(s[e / 2 + 1], k4.y, v4.y);
+    float2 x = halves(s[e / 2]), y = halves(s[e / 2 + 1]);
     if constexpr (EDGE) {
       x.x = see >> e & 1 ? x.x : -INFINITY;
       x.y = see >> (e + 1) & 1 ? x.y : -INFINITY;
       y.x = see >> (e + 2) & 1 ? y.x : -INFINITY;
       y.y = see >> (e + 3) & 1 ? y.y : -INFINITY;
+      s[e / 2] = pair(x.x, x.y);
+      s[e / 2 + 1] = pair(y.x, y.y);
     }
-    s[e / 2] = x;
-    s[e / 2 + 1] = y;
     top[e / 4 % 2] = fmaxf(fmaxf(top[e / 4 % 2], x.x), x.y);
     top[2 + e / 4 % 2] = fmaxf(fmaxf(top[2 + e / 4 % 2], y.x), y.y);
   }
@@ -240,37 +258,36 @@ __device__ __forceinline__ float ar_scores(float2 (&s)[AR_TILE / 2], const float
 
 // Weights 2^(t + shift) in fp16, and the sum of the unrounded ones over their value scales.
 template <bool EDGE>
-__device__ __forceinline__ float ar_weights(const float2 (&t)[AR_TILE / 2], const float* inv, float shift, uint64_t see,
+__device__ __forceinline__ float ar_weights(const f32x2 (&t)[AR_TILE / 2], const float* inv, float shift, uint64_t see,
                                             uint32_t (&w)[AR_TILE / 2]) {
-  const float2 sh = make_float2(shift, shift);
-  float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+  const f32x2 sh = pair(shift, shift);
+  f32x2 acc0 = pair(0.f, 0.f), acc1 = acc0;
 #pragma unroll
   for (int e = 0; e < AR_TILE; e += 4) {
-    float2 x = add2(t[e / 2], sh), y = add2(t[e / 2 + 1], sh);
+    float2 x = halves(add2(t[e / 2], sh)), y = halves(add2(t[e / 2 + 1], sh));
     x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
     y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-    float4 i4 = *reinterpret_cast<const float4*>(inv + e);
+    ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(inv + e);
     if constexpr (EDGE) {  // a hidden position's scale may be NaN
-      i4.x = see >> e & 1 ? i4.x : 0.f;
-      i4.y = see >> (e + 1) & 1 ? i4.y : 0.f;
-      i4.z = see >> (e + 2) & 1 ? i4.z : 0.f;
-      i4.w = see >> (e + 3) & 1 ? i4.w : 0.f;
+      const float2 a = halves(i4.x), b = halves(i4.y);
+      i4.x = pair(see >> e & 1 ? a.x : 0.f, see >> (e + 1) & 1 ? a.y : 0.f);
+      i4.y = pair(see >> (e + 2) & 1 ? b.x : 0.f, see >> (e + 3) & 1 ? b.y : 0.f);
     }
-    acc0 = fma2(x, make_float2(i4.x, i4.y), acc0);
-    acc1 = fma2(y, make_float2(i4.z, i4.w), acc1);
+    acc0 = fma2(pair(x.x, x.y), i4.x, acc0);
+    acc1 = fma2(pair(y.x, y.y), i4.y, acc1);
     const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
     w[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
     w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
   }
-  acc0 = add2(acc0, acc1);
-  return acc0.x + acc0.y;
+  const float2 sum = halves(add2(acc0, acc1));
+  return sum.x + sum.y;
 }
 
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs a) {
   using G = ArGeom<D>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // (an offset: the pointer stays a shared one)
   uint8_t* raw = smem + G::STAGES * G::ITEM;
   float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][64]
   float* refs = scales + G::SCALES / 4;                                   // [128], base-2 exponents
@@ -414,10 +431,13 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         ok = warp_wait(&s_full[group], (uint32_t)((tile / 2) & 1), a.err);
         if (!ok) break;
         tc_fence_after();
-        float2 s[AR_TILE / 2];
-        tmem_ld32(lanes + G::S, reinterpret_cast<uint32_t*>(s));
-        tmem_ld32(lanes + G::S + 32, reinterpret_cast<uint32_t*>(s) + 32);
+        uint32_t s32[AR_TILE];
+        tmem_ld32(lanes + G::S, s32);
+        tmem_ld32(lanes + G::S + 32, s32 + 32);
         tmem_wait_ld();
+        f32x2 s[AR_TILE / 2];
+#pragma unroll
+        for (int e = 0; e < AR_TILE / 2; e++) s[e] = pair(__uint_as_float(s32[2 * e]), __uint_as_float(s32[2 * e + 1]));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
@@ -587,8 +607,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       const uint32_t items = smem_u32(smem);
       // S of the CTA's tile t: into TMEM when the softmax has taken tile t - 1's
       auto scores = [&](int t) {
-        ok = mbar_wait_bounded(&full[stage], (uint32_t)(use & 1), a.err) &&
-             (t == 0 || mbar_wait_bounded(s_free, (uint32_t)((t - 1) & 1), a.err));
+        ok = ar_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
+             (t == 0 || ar_wait(s_free, (uint32_t)((t - 1) & 1), a.err));
         if (!ok) return;
         tc_fence_after();
         const uint32_t b = ar_k_major(items + stage * G::ITEM);
@@ -601,14 +621,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         if (++stage == G::STAGES) stage = 0, use++;
       };
       do {
-        ok = mbar_wait_bounded(q_full, (uint32_t)(runs++ & 1), a.err);
+        ok = ar_wait(q_full, (uint32_t)(runs++ & 1), a.err);
         if (!ok) break;
         scores(tile);
         if (ok && run.len > 1) scores(tile + 1);
         for (int j = 0; j < run.len && ok; j++, tile++) {
           if (j + 2 < run.len) scores(tile + 2);
-          ok = ok && mbar_wait_bounded(&full[stage], (uint32_t)(use & 1), a.err) &&
-               mbar_wait_bounded(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
+          ok = ok && ar_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
+               ar_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
           if (!ok) break;
           tc_fence_after();
           const uint32_t b = ar_mn_major(items + stage * G::ITEM, AR_TILE * 128);
@@ -623,14 +643,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       } while (ok && run.next(a));
       // nothing may still write TMEM when it is given back
       tc_commit(drained);
-      mbar_wait_bounded(drained, 0, a.err);
+      ar_wait(drained, 0, a.err);
     } else if (warp == AR_SOFTMAX + AR_DEQUANT + 1 && lane == 0) {
       // ---------------- copy the codes: one thread; items in the order K0, K1, K2, V0, K3, V1, .. of each run --------
       int rs = 0, ruse = 0, kpos = 0, vpos = 0;
       const int items = 2 * (last - first);
       for (int it = 0; it < items; it++) {
         if (ruse > 0) {
-          ok = mbar_wait_bounded(&raw_empty[rs], (uint32_t)((ruse - 1) & 1), a.err);
+          ok = ar_wait(&raw_empty[rs], (uint32_t)((ruse - 1) & 1), a.err);
           if (!ok) break;
         }
         const bool key = kpos < run.len && kpos - vpos < 3;
@@ -648,7 +668,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       // no copy may still be under way when the CTA ends (after a wait that gave up, one may be)
       for (int i = 0; i < G::RAWS; i++) {
         const int uses = ruse + (i < rs ? 1 : 0);
-        if (uses > 0) mbar_wait_bounded(&raw_full[i], (uint32_t)((uses - 1) & 1), a.err);
+        if (uses > 0) ar_wait(&raw_full[i], (uint32_t)((uses - 1) & 1), a.err);
       }
     }
     __syncwarp();
