@@ -18,12 +18,14 @@
 //     score, and its value scale enters the weight as 2^(s + log2 vs - ref),
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs.
-// Roles (20 warps): two softmax warpgroups that take the tiles in turn, one
-// row a thread; two that dequantise; one thread issues the products, one the
-// bulk copies of codes (a tile is one contiguous piece). S of the next two
-// tiles is issued before P V of this one, so that two tiles are in the softmax
-// while the tensor core works on their neighbours; what the two groups share
-// is each row's reference (the running maximum), passed from tile to tile.
+// Roles (20 warps): two softmax warpgroups, one row a thread, that take the
+// two halves of every tile's columns; two that dequantise; one thread issues
+// the products, one the bulk copies of codes (a tile is one contiguous piece).
+// The groups pass each other the largest score of a row's half, so that both
+// follow the same reference (the running maximum). Half a tile a thread keeps
+// the softmax loop, which is unrolled over its scores, short enough for the
+// instruction caches: with whole tiles in turn a fifth of its time went into
+// instruction misses.
 // The reference is followed lazily: O is rescaled only when it grows by more
 // than 2^8, which weights of up to 2^14 in fp16 leave room for.
 // Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded
@@ -35,7 +37,7 @@
 
 namespace gsq {
 
-constexpr int AR_M = 128, AR_TILE = 64;
+constexpr int AR_M = 128, AR_TILE = 64, AR_HALF = AR_TILE / 2;
 constexpr int AR_GROUP = 4, AR_SOFTMAX = 2 * AR_GROUP, AR_DEQUANT = 8;  // warps
 constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four one issues products, one copies
 
@@ -45,8 +47,8 @@ struct ArGeom {
   static constexpr int STAGES = D == 256 ? 5 : 6;
   static constexpr int RAW = AR_TILE * D;       // its codes
   static constexpr int RAWS = 3;
-  static constexpr int SCALES = AR_SOFTMAX * 5 * AR_TILE * 4;
-  static constexpr int STATE = 3 * AR_M * 4;    // references, and the two groups' sums
+  static constexpr int SCALES = AR_SOFTMAX * 5 * AR_HALF * 4;
+  static constexpr int STATE = 6 * AR_M * 4;    // the two groups' maxima of two tiles, and their sums
   static constexpr int SMEM = 1024 + STAGES * ITEM + RAWS * RAW + SCALES + STATE + 512;
   static constexpr int O = 0, Q = D, S = Q + D / 2, P = S + AR_TILE;  // TMEM columns
   static constexpr int COLS = 512;
@@ -120,6 +122,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
       "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::GSQ_I8(r, 0), GSQ_I8(r, 8), GSQ_I8(r, 16),
       GSQ_I8(r, 24), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::GSQ_I8(r, 0),
+      GSQ_I8(r, 8), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -203,84 +210,27 @@ __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const S
   return m & below(s.len - p0);
 }
 
-// Scales of two positions of a tile a lane, as the softmax uses them: the keys' times `factor`, log2 of the values' and
-// its inverse in linear terms, in the warp's own copy.
-struct ArZeros {
-  uint32_t even, odd;  // bit i: the value scale of position 2i (2i + 1) is 0
-};
-__device__ __forceinline__ ArZeros ar_scales(float* ks, float factor, float2 k2, float2 v2) {
+// Scales of the warp's 32 positions, one a lane, as the softmax uses them: the key's times `factor`, log2 of the value's
+// and its inverse in linear terms, in the warp's own copy. Returns the positions (bits) whose value scale is 0.
+__device__ __forceinline__ uint32_t ar_scales(float* ks, float factor) {
   const int lane = threadIdx.x & 31;
+  const float k = ks[3 * AR_HALF + lane], v = ks[4 * AR_HALF + lane];
   // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of scale 0 has
-  // no part in the output, but in the sum of weights: it is weighted with the largest scale of the tile, and that
-  // weight left out of P.
-  float lx = v2.x > 0.f ? fmaxf(log2_approx(v2.x), -100.f) : -INFINITY;
-  float ly = v2.y > 0.f ? fmaxf(log2_approx(v2.y), -100.f) : -INFINITY;
-  const ArZeros z = {__ballot_sync(0xffffffffu, v2.x == 0.f), __ballot_sync(0xffffffffu, v2.y == 0.f)};
-  float top = -40.f;
-  if (z.even | z.odd) {
-    top = fmaxf(lx, ly);
+  // no part in the output, but in the sum of weights: it is weighted with the largest scale beside it, and that weight
+  // left out of P. NaN stays, with 1 / vs as 0, so that a row that does not see the position takes no harm.
+  float lv = v > 0.f ? fmaxf(log2_approx(v), -100.f) : -INFINITY;
+  const uint32_t zeros = __ballot_sync(0xffffffffu, v == 0.f);
+  if (zeros) {
+    float top = lv;
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top == -INFINITY) top = -40.f;
+    if (v == 0.f) lv = top == -INFINITY ? -40.f : top;
   }
-  lx = v2.x > 0.f ? lx : v2.x == 0.f ? top : v2.x;  // NaN stays
-  ly = v2.y > 0.f ? ly : v2.y == 0.f ? top : v2.y;
-  *reinterpret_cast<float2*>(ks + 2 * lane) = make_float2(k2.x * factor, k2.y * factor);
-  *reinterpret_cast<float2*>(ks + AR_TILE + 2 * lane) = make_float2(lx, ly);
-  *reinterpret_cast<float2*>(ks + 2 * AR_TILE + 2 * lane) = make_float2(exp2_approx(-lx), exp2_approx(-ly));
-  return z;
-}
-
-// s: raw scores of a row -> t = ks * s + log2 vs; -inf where a bit of `see` is off (EDGE). Returns the maximum.
-template <bool EDGE>
-__device__ __forceinline__ float ar_scores(f32x2 (&s)[AR_TILE / 2], const float* ks, uint64_t see) {
-  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-  for (int e = 0; e < AR_TILE; e += 4) {
-    const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + e);
-    const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(ks + AR_TILE + e);
-    s[e / 2] = fma2(s[e / 2], k4.x, v4.x);
-    s[e / 2 + 1] = fma2(s[e / 2 + 1], k4.y, v4.y);
-    float2 x = halves(s[e / 2]), y = halves(s[e / 2 + 1]);
-    if constexpr (EDGE) {
-      x.x = see >> e & 1 ? x.x : -INFINITY;
-      x.y = see >> (e + 1) & 1 ? x.y : -INFINITY;
-      y.x = see >> (e + 2) & 1 ? y.x : -INFINITY;
-      y.y = see >> (e + 3) & 1 ? y.y : -INFINITY;
-      s[e / 2] = pair(x.x, x.y);
-      s[e / 2 + 1] = pair(y.x, y.y);
-    }
-    top[e / 4 % 2] = fmaxf(fmaxf(top[e / 4 % 2], x.x), x.y);
-    top[2 + e / 4 % 2] = fmaxf(fmaxf(top[2 + e / 4 % 2], y.x), y.y);
-  }
-  return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-}
-
-// Weights 2^(t + shift) in fp16, and the sum of the unrounded ones over their value scales.
-template <bool EDGE>
-__device__ __forceinline__ float ar_weights(const f32x2 (&t)[AR_TILE / 2], const float* inv, float shift, uint64_t see,
-                                            uint32_t (&w)[AR_TILE / 2]) {
-  const f32x2 sh = pair(shift, shift);
-  f32x2 acc0 = pair(0.f, 0.f), acc1 = acc0;
-#pragma unroll
-  for (int e = 0; e < AR_TILE; e += 4) {
-    float2 x = halves(add2(t[e / 2], sh)), y = halves(add2(t[e / 2 + 1], sh));
-    x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-    y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-    ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(inv + e);
-    if constexpr (EDGE) {  // a hidden position's scale may be NaN
-      const float2 a = halves(i4.x), b = halves(i4.y);
-      i4.x = pair(see >> e & 1 ? a.x : 0.f, see >> (e + 1) & 1 ? a.y : 0.f);
-      i4.y = pair(see >> (e + 2) & 1 ? b.x : 0.f, see >> (e + 3) & 1 ? b.y : 0.f);
-    }
-    acc0 = fma2(pair(x.x, x.y), i4.x, acc0);
-    acc1 = fma2(pair(y.x, y.y), i4.y, acc1);
-    const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
-    w[e / 2] = *reinterpret_cast<const uint32_t*>(&h0);
-    w[e / 2 + 1] = *reinterpret_cast<const uint32_t*>(&h1);
-  }
-  const float2 sum = halves(add2(acc0, acc1));
-  return sum.x + sum.y;
+  const bool nan = isnan(v);
+  ks[lane] = k * factor;
+  ks[AR_HALF + lane] = nan ? v : lv;
+  ks[2 * AR_HALF + lane] = nan ? 0.f : exp2_approx(-lv);
+  return zeros;
 }
 
 template <typename T, int FMT, int D>
@@ -289,19 +239,19 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // (an offset: the pointer stays a shared one)
   uint8_t* raw = smem + G::STAGES * G::ITEM;
-  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][64]
-  float* refs = scales + G::SCALES / 4;                                   // [128], base-2 exponents
-  float* sums = refs + AR_M;                                              // [group][128]
+  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][32]
+  float* tops = scales + G::SCALES / 4;   // [tile & 1][group][128]: largest scores, to base 2
+  float* sums = tops + 4 * AR_M;          // [group][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sums + 2 * AR_M);
   uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
   uint64_t* empty = full + G::STAGES;     // [STAGES] commit
-  uint64_t* s_full = empty + G::STAGES;   // [group] commit
-  uint64_t* s_free = s_full + 2;          // count AR_GROUP
-  uint64_t* p_full = s_free + 1;          // [group] count AR_GROUP
-  uint64_t* pv_done = p_full + 2;         // [group] commit
+  uint64_t* s_full = empty + G::STAGES;   // commit
+  uint64_t* s_free = s_full + 1;          // count AR_SOFTMAX
+  uint64_t* p_full = s_free + 1;          // [tile & 1] count AR_SOFTMAX
+  uint64_t* pv_done = p_full + 2;         // [tile & 1] commit
   uint64_t* q_full = pv_done + 2;         // count AR_SOFTMAX
-  uint64_t* ref_done = q_full + 1;        // [32 rows] count 1: the references are those of one more tile
-  uint64_t* sum_done = ref_done + 4;      // [32 rows] count 2: both groups' sums are there
+  uint64_t* top_done = q_full + 1;        // [32 rows] count 2: both groups' maxima are there
+  uint64_t* sum_done = top_done + 4;      // [32 rows] count 2: both groups' sums are there
   uint64_t* drained = sum_done + 4;       // commit
   uint64_t* raw_full = drained + 1;       // [RAWS] the copy
   uint64_t* raw_empty = raw_full + G::RAWS;  // [RAWS] count AR_DEQUANT
@@ -316,15 +266,15 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       mbar_init(&full[i], AR_DEQUANT);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(s_free, AR_GROUP);
+    mbar_init(s_full, 1);
+    mbar_init(s_free, AR_SOFTMAX);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], AR_GROUP);
+      mbar_init(&p_full[i], AR_SOFTMAX);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, AR_SOFTMAX);
     for (int i = 0; i < 4; i++) {
-      mbar_init(&ref_done[i], 1);
+      mbar_init(&top_done[i], 2);
       mbar_init(&sum_done[i], 2);
     }
     mbar_init(drained, 1);
@@ -352,12 +302,10 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     if (threadIdx.x == 0) a.joints[blockIdx.x].parts = 0;
   } else if (warp < AR_SOFTMAX) {
     // ---------------- softmax: thread = row ----------------
-    // of 96 registers a thread at the launch (480 in all): 136 for each group here, 80 for each that dequantises, 48
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const int group = warp / AR_GROUP, quarter = warp % AR_GROUP, row = threadIdx.x % AR_M;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     const int rows = a.n * a.group;
-    float* ks = scales + warp * 5 * AR_TILE;
+    float* ks = scales + warp * 5 * AR_HALF;
     ArRun run;
     run.begin(a, first, last);
     int tile = 0, runs = 0;  // of the CTA
@@ -404,69 +352,78 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       if (lane == 0) mbar_arrive(q_full);
 
       const int64_t row0 = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap;
-      // Scales of this group's coming tile, copied while the last one is worked on (loads into registers would be
-      // waited for at the next arrival on a barrier); 0 past the end
-      auto fetch_scales = [&](int p0) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          const int p = p0 + (c & 1) * 32 + lane;
-          const bool in = p < run.at.span.len;
-          cp_async4_zfill(ks + (3 + c / 2) * AR_TILE + (c & 1) * 32 + lane, (c < 2 ? a.ks : a.vs) + (in ? row0 + p : 0), in);
-        }
+      // Scales of the coming half tile, copied while the last one is worked on (loads into registers would be waited
+      // for at the next arrival on a barrier); 0 past the end
+      auto fetch_scales = [&](int p) {
+        const bool in = p < run.at.span.len;
+        cp_async4_zfill(ks + 3 * AR_HALF + lane, a.ks + (in ? row0 + p : 0), in);
+        cp_async4_zfill(ks + 4 * AR_HALF + lane, a.vs + (in ? row0 + p : 0), in);
         cp_async_commit();
       };
       const int run0 = tile;  // the run's first tile
-      if ((tile & 1) != group) tile++;
-      if (tile < run0 + run.len) fetch_scales((run.at.tile + tile - run0) * AR_TILE);
+      fetch_scales(run.at.tile * AR_TILE + group * AR_HALF + lane);
 
-      float ref = -INFINITY, sum = 0.f;  // of the row, as this group knows them
-      for (; tile < run0 + run.len; tile += 2) {
-        const int p0 = (run.at.tile + tile - run0) * AR_TILE;
+      float ref = -INFINITY, sum = 0.f;  // of the row; the sum of this group's half
+      for (; tile < run0 + run.len; tile++) {
+        const int p0 = (run.at.tile + tile - run0) * AR_TILE + group * AR_HALF;
         cp_async_wait<0>();
-        __syncwarp();  // this tile's are there, and the warp has read the last tile's
-        const ArZeros zeros = ar_scales(ks, factor, *reinterpret_cast<const float2*>(ks + 3 * AR_TILE + 2 * lane),
-                                        *reinterpret_cast<const float2*>(ks + 4 * AR_TILE + 2 * lane));
+        __syncwarp();  // this half's are there, and the warp has read the last one's
+        const uint32_t zeros = ar_scales(ks, factor);
         __syncwarp();
-        if (tile + 2 < run0 + run.len) fetch_scales(p0 + 2 * AR_TILE);
-        ok = warp_wait(&s_full[group], (uint32_t)((tile / 2) & 1), a.err);
+        if (tile + 1 < run0 + run.len) fetch_scales(p0 + AR_TILE + lane);
+        ok = warp_wait(s_full, (uint32_t)(tile & 1), a.err);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s32[AR_TILE];
-        tmem_ld32(lanes + G::S, s32);
-        tmem_ld32(lanes + G::S + 32, s32 + 32);
+        uint32_t s[AR_HALF];
+        tmem_ld32(lanes + G::S + group * AR_HALF, s);
         tmem_wait_ld();
-        f32x2 s[AR_TILE / 2];
-#pragma unroll
-        for (int e = 0; e < AR_TILE / 2; e++) s[e] = pair(__uint_as_float(s32[2 * e]), __uint_as_float(s32[2 * e + 1]));
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
 
-        const bool edge = p0 + AR_TILE > min(run.at.span.base, run.at.span.len);  // the same for all threads
-        const uint64_t see = edge ? ar_visible(a, run.at.b, run.at.span, i, p0) : ~0ull;
-        const float top = edge ? ar_scores<true>(s, ks, see) : ar_scores<false>(s, ks, see);
-        // the reference after the last tile, which the other group has set
-        if (tile > run0) {
-          ok = warp_wait(&ref_done[quarter], (uint32_t)((tile - 1) & 1), a.err);
-          if (!ok) break;
-          const float now = refs[row];
-          if (now != ref) {
-            if (ref != -INFINITY) sum *= exp2_approx(ref - now);
-            ref = now;
+        // t = ks * s + log2 vs, and the row's maximum over both halves
+        f32x2 t[AR_HALF / 2];
+#pragma unroll
+        for (int e = 0; e < AR_HALF; e += 4) {
+          const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + e);
+          const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(ks + AR_HALF + e);
+          t[e / 2] = fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), k4.x, v4.x);
+          t[e / 2 + 1] = fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), k4.y, v4.y);
+        }
+        if (p0 + AR_HALF > min(run.at.span.base, run.at.span.len)) {  // the same for all threads
+          const uint32_t see = (uint32_t)ar_visible(a, run.at.b, run.at.span, i, p0);
+#pragma unroll
+          for (int e = 0; e < AR_HALF / 2; e++) {
+            const float2 x = halves(t[e]);
+            t[e] = pair(see >> 2 * e & 1 ? x.x : -INFINITY, see >> (2 * e + 1) & 1 ? x.y : -INFINITY);
           }
         }
+        float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < AR_HALF / 2; e++) {
+          const float2 x = halves(t[e]);
+          m[e % 4] = fmaxf(fmaxf(m[e % 4], x.x), x.y);
+        }
+        float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        float* mine = tops + (tile & 1) * 2 * AR_M + row;
+        mine[group * AR_M] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&top_done[quarter]);
+        ok = warp_wait(&top_done[quarter], (uint32_t)(tile & 1), a.err);
+        if (!ok) break;
+        top = fmaxf(top, mine[(1 - group) * AR_M]);
         const bool grow = top > ref + 8.f || (ref == -INFINITY && top > ref);
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? top : ref;
           const float f = ref == next || ref == -INFINITY ? 1.f : exp2_approx(ref - next);  // no weight yet: 0, or NaN
           sum *= f;
           if (tile > run0) {
-            // O holds this unit's tiles so far: wait for the last of them and rescale it
+            // O holds this unit's tiles so far: wait for the last of them and rescale it, each group half its columns
             ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += 32) {
               uint32_t o[32];
               tmem_ld32(lanes + G::O + c, o);
               tmem_wait_ld();
@@ -478,40 +435,45 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           }
           ref = next;
         }
-        refs[row] = ref;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ref_done[quarter]);
 
-        // weights 2^(t - ref + 6), at most 2^14
-        uint32_t w[AR_TILE / 2];
+        // weights 2^(t - ref + 6), at most 2^14, in fp16; and the sum of the unrounded ones over their value scales
         const float lift = 6.f - (ref == -INFINITY ? 0.f : ref);
-        sum += edge ? ar_weights<true>(s, ks + 2 * AR_TILE, lift, see, w)
-                    : ar_weights<false>(s, ks + 2 * AR_TILE, lift, see, w);
-        if (zeros.even | zeros.odd) {
+        const f32x2 lift2 = pair(lift, lift);
+        f32x2 acc0 = pair(0.f, 0.f), acc1 = acc0;
+        uint32_t w[AR_HALF / 2];
 #pragma unroll
-          for (int e = 0; e < AR_TILE / 2; e++)
-            w[e] &= (zeros.even >> e & 1 ? 0u : 0xffffu) | (zeros.odd >> e & 1 ? 0u : 0xffff0000u);
+        for (int e = 0; e < AR_HALF / 2; e += 2) {
+          float2 x = halves(add2(t[e], lift2)), y = halves(add2(t[e + 1], lift2));
+          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          y = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+          const ulonglong2 i4 = *reinterpret_cast<const ulonglong2*>(ks + 2 * AR_HALF + 2 * e);
+          acc0 = fma2(pair(x.x, x.y), i4.x, acc0);
+          acc1 = fma2(pair(y.x, y.y), i4.y, acc1);
+          const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
+          w[e] = *reinterpret_cast<const uint32_t*>(&h0);
+          w[e + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
-        if (tile >= 2) {  // this group's last P has been read
-          ok = warp_wait(&pv_done[group], (uint32_t)((tile / 2 - 1) & 1), a.err);
+        const float2 added = halves(add2(acc0, acc1));
+        sum += added.x + added.y;
+        if (zeros) {
+#pragma unroll
+          for (int e = 0; e < AR_HALF / 2; e++)
+            w[e] &= (zeros >> 2 * e & 1 ? 0u : 0xffffu) | (zeros >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
+        }
+        if (tile >= 2) {  // the P of tile - 2 has been read
+          ok = warp_wait(&pv_done[tile & 1], (uint32_t)((tile / 2 - 1) & 1), a.err);
           if (!ok) break;
         }
-        tmem_st32(lanes + G::P + group * (AR_TILE / 2), w);
+        tmem_st16(lanes + G::P + (tile & 1) * (AR_TILE / 2) + group * (AR_HALF / 2), w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[group]);
+        if (lane == 0) mbar_arrive(&p_full[tile & 1]);
       }
       if (!ok) break;
 
       // ---- the unit's (or its part's) result: the columns' halves by the two groups ----
-      const int end = run0 + run.len - 1;  // the run's last tile
-      tile = end + 1;
-      ok = warp_wait(&ref_done[quarter], (uint32_t)(end & 1), a.err);
-      if (!ok) break;
-      const float now = refs[row];
-      if (now != ref && ref != -INFINITY) sum *= exp2_approx(ref - now);
-      ref = now;
+      const int end = tile - 1;  // the run's last tile
       sums[group * AR_M + row] = sum;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sum_done[quarter]);
@@ -553,7 +515,6 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     // ---------------- dequantise ----------------
     // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
     // swizzled row. Rows of one lane differ by multiples of 8, so its swizzle is a constant.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     const int w = warp - AR_SOFTMAX;
     constexpr int LPR = D / 8;               // lanes per row
     constexpr int RPW = 32 / LPR;            // rows per warp and step
@@ -597,7 +558,6 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       if (++rs == G::RAWS) rs = 0, ruse++;
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     ArRun run;
     if (warp < AR_SOFTMAX + AR_DEQUANT + 2) run.begin(a, first, last);
     if (warp == AR_SOFTMAX + AR_DEQUANT && lane == 0) {
@@ -617,16 +577,15 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, ar_desc(b + k / 4 * (AR_TILE * 128 / 16) + k % 4 * 2),
                         ar_idesc(AR_TILE, false), k != 0);
         tc_commit(&empty[stage]);
-        tc_commit(&s_full[t & 1]);
+        tc_commit(s_full);
         if (++stage == G::STAGES) stage = 0, use++;
       };
       do {
         ok = ar_wait(q_full, (uint32_t)(runs++ & 1), a.err);
         if (!ok) break;
         scores(tile);
-        if (ok && run.len > 1) scores(tile + 1);
         for (int j = 0; j < run.len && ok; j++, tile++) {
-          if (j + 2 < run.len) scores(tile + 2);
+          if (j + 1 < run.len) scores(tile + 1);
           ok = ok && ar_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
                ar_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
           if (!ok) break;
@@ -645,7 +604,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       tc_commit(drained);
       ar_wait(drained, 0, a.err);
     } else if (warp == AR_SOFTMAX + AR_DEQUANT + 1 && lane == 0) {
-      // ---------------- copy the codes: one thread; items in the order K0, K1, K2, V0, K3, V1, .. of each run --------
+      // ---------------- copy the codes: one thread; items in the order K0, K1, V0, K2, V1, .. of each run --------
       int rs = 0, ruse = 0, kpos = 0, vpos = 0;
       const int items = 2 * (last - first);
       for (int it = 0; it < items; it++) {
@@ -653,7 +612,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           ok = ar_wait(&raw_empty[rs], (uint32_t)((ruse - 1) & 1), a.err);
           if (!ok) break;
         }
-        const bool key = kpos < run.len && kpos - vpos < 3;
+        const bool key = kpos < run.len && kpos - vpos < 2;
         const int p0 = (run.at.tile + (key ? kpos++ : vpos++)) * AR_TILE, n = min(run.at.span.len - p0, AR_TILE);
         raw_rows[rs] = n;
         mbar_arrive_expect_tx(&raw_full[rs], n * D);
