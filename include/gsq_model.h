@@ -161,6 +161,18 @@ GSQ_API int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const
                         int64_t start_stride, const int32_t* counts, int64_t tokens, void* k, void* v, int dtype,
                         gsq_stream_t stream);
 
+/* gsq_kv_append as the attention layer of the model needs it, from its
+ * projection: qkv [batch * tokens, qkv_stride] fp32, per row as in
+ * gsq_attn_decode (nq times 256 query and 256 gate values, then keys, then
+ * values; heads 256 wide).  Queries and keys are RMS-normalised per head and
+ * rotated as there, at positions start + t; the queries go to q [batch,
+ * tokens, nq, 256] rounded to fp16, keys and values into the cache.
+ * batch * tokens <= 65535. */
+GSQ_API int gsq_qkv_append(const float* qkv, int64_t qkv_stride, int64_t batch, int64_t tokens, int64_t nq,
+                           int64_t nkv, const float* q_norm_w, const float* k_norm_w, float eps, int64_t rot,
+                           float theta, const int32_t* start, int64_t start_stride, void* q, int fmt, void* k_codes,
+                           void* v_codes, float* k_scale, float* v_scale, int64_t cap, gsq_stream_t stream);
+
 /* Attention of n new tokens of each sequence, whose keys and values are in
  * the cache already (gsq_kv_append with the same start and counts):
  *

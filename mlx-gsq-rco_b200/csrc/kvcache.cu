@@ -230,6 +230,83 @@ __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvArgs a) 
   }
 }
 
+// The attention layer's step between its projection and its attention (heads 256 wide): queries and keys normalised and
+// rotated, queries rounded to fp16, keys and values quantised into the cache. One warp per vector: first the queries,
+// then keys and values in turn. The vector passes through shared memory once, for the rotation's pairs.
+struct QkvArgs {
+  const float* qkv;
+  int64_t stride;
+  const float *qw, *kw;
+  float eps, theta;
+  int rot, nq, nkv, tokens;
+  const int32_t* start;
+  int64_t start_stride;
+  __half* q;
+  uint8_t* codes[2];
+  float* scale[2];
+  int64_t cap;
+  int* err;
+};
+
+template <int FMT>
+__global__ void __launch_bounds__(32 * KV_WARPS) qkv_append_kernel(const QkvArgs a) {
+  constexpr int D = 256, N = D / 32;
+  __shared__ __align__(16) float vec[KV_WARPS][D];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int v = blockIdx.x * KV_WARPS + warp;  // 0 .. nq - 1: queries; then k0, v0, k1, v1, ..
+  if (v >= a.nq + 2 * a.nkv) return;
+  const int64_t row = blockIdx.y;  // sequence and token
+  const int b = (int)(row / a.tokens), t = (int)(row % a.tokens);
+  const bool query = v < a.nq;
+  const int h = query ? v : (v - a.nq) / 2, which = query ? 0 : (v - a.nq) % 2;
+  const float* src = a.qkv + row * a.stride +
+                     (query ? (int64_t)h * 2 * D : (int64_t)a.nq * 2 * D + ((int64_t)which * a.nkv + h) * D) + lane * N;
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) f[i] = src[i];
+  const int64_t p = (int64_t)a.start[(int64_t)b * a.start_stride] + t;
+  if (query || which == 0) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++) ss = fmaf(f[i], f[i], ss);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float inv = rsqrtf(ss / D + a.eps);
+    const float* w = (query ? a.qw : a.kw) + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; i++) vec[warp][lane * N + i] = f[i] = f[i] * inv * w[i];
+    __syncwarp();
+    const int half = a.rot / 2;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int d = lane * N + i;
+      if (d < a.rot) {
+        const float ang = (float)p * powf(a.theta, -2.f * (float)(d % half) / (float)a.rot);
+        float sn, cs;
+        sincosf(ang, &sn, &cs);
+        f[i] = f[i] * cs + (d < half ? -vec[warp][d + half] : vec[warp][d - half]) * sn;
+      }
+    }
+  }
+  if (query) {
+    alignas(16) __half2 q[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) q[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    *reinterpret_cast<uint4*>(a.q + (row * a.nq + h) * D + lane * N) = *reinterpret_cast<const uint4*>(q);
+  } else if (p >= 0 && p < a.cap) {
+    uint32_t code[N / 4];
+    float scale;
+    quantise<FMT, N>(f, code, scale);
+    const int64_t at = ((int64_t)b * a.nkv + h) * a.cap + p;
+    store_codes<N>(a.codes[which] + at * D + lane * N, code);
+    if (lane == 0) a.scale[which][at] = scale;
+  } else if (lane == 0 && a.err) {
+    atomicExch(a.err, DEV_CACHE_POSITION);
+  }
+}
+
 int fail(int code, const char* msg) { return set_last_error(code, msg); }
 
 int launched(cudaError_t rc, const char* what) {
@@ -368,6 +445,45 @@ int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* 
                                        : (dim == 256 ? read_launch<KV_FP8, 256>(dtype, grid, st, a)
                                                      : read_launch<KV_FP8, 128>(dtype, grid, st, a));
   return launched(e, "gsq_kv_read");
+}
+
+int gsq_qkv_append(const float* qkv, int64_t qkv_stride, int64_t batch, int64_t tokens, int64_t nq, int64_t nkv,
+                   const float* q_norm_w, const float* k_norm_w, float eps, int64_t rot, float theta,
+                   const int32_t* start, int64_t start_stride, void* q, int fmt, void* k_codes, void* v_codes,
+                   float* k_scale, float* v_scale, int64_t cap, gsq_stream_t stream) {
+  int rc = kv_check("gsq_qkv_append", fmt, k_codes, v_codes, k_scale, v_scale, batch, nkv, 256, cap);
+  if (rc) return rc;
+  if (tokens < 0 || batch * tokens > 65535) return fail(GSQ_ERR_SIZE, "gsq_qkv_append: at most 65535 tokens in all");
+  if (nq <= 0 || nq > 65535 || qkv_stride < 512 * nq + 512 * nkv)
+    return fail(GSQ_ERR_SIZE, "gsq_qkv_append: bad head count or stride");
+  if (rot < 0 || rot > 256 || rot % 2) return fail(GSQ_ERR_SIZE, "gsq_qkv_append: bad rotary width");
+  if (batch == 0 || tokens == 0) return GSQ_OK;
+  if (!qkv || !q_norm_w || !k_norm_w || !start || !q) return fail(GSQ_ERR_ARG, "gsq_qkv_append: null pointer");
+  if (!al16(q)) return fail(GSQ_ERR_ALIGN, "gsq_qkv_append: q not 16-byte aligned");
+  QkvArgs a = {};
+  a.qkv = qkv;
+  a.stride = qkv_stride;
+  a.qw = q_norm_w;
+  a.kw = k_norm_w;
+  a.eps = eps;
+  a.theta = theta;
+  a.rot = (int)rot;
+  a.nq = (int)nq;
+  a.nkv = (int)nkv;
+  a.tokens = (int)tokens;
+  a.start = start;
+  a.start_stride = start_stride;
+  a.q = static_cast<__half*>(q);
+  a.codes[0] = static_cast<uint8_t*>(k_codes);
+  a.codes[1] = static_cast<uint8_t*>(v_codes);
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.cap = cap;
+  a.err = device_error_word();
+  const dim3 grid((unsigned)((nq + 2 * nkv + KV_WARPS - 1) / KV_WARPS), (unsigned)(batch * tokens));
+  return launched(launch_pdl(fmt == KV_INT8 ? qkv_append_kernel<KV_INT8> : qkv_append_kernel<KV_FP8>, grid,
+                             dim3(32 * KV_WARPS), 0, (cudaStream_t)stream, a),
+                  "gsq_qkv_append");
 }
 
 }  // extern "C"

@@ -65,6 +65,8 @@ SIGNATURES = {
                                    _I, _I64, _P]),
     "gsq_kv_append": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _I, _P, _P, _P, _P, _I64, _P]),
     "gsq_kv_read": (_I, [_I, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I, _P]),
+    "gsq_qkv_append": (_I, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, ctypes.c_float, _I64, ctypes.c_float, _P, _I64, _P,
+                            _I, _P, _P, _P, _P, _I64, _P]),
     "gsq_cached_attention_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "gsq_cached_attention": (_I, [_P, _I, _P, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _P, _I64, _P, _P,
                                   _I64, _P, _P, ctypes.c_float, _P, _P, _SZ, _P]),

@@ -23,6 +23,10 @@ SwiGLU FFN 17408, vocab 248320.  Here the same model runs on B200:
     add + RMSNorm, SiLU-mul, the gated-DeltaNet block (conv, norms, gates,
     recurrence, gated norm) and the single-token attention step; prefill
     attention uses torch's scaled-dot-product attention;
+  * with ``kv_format`` the attention layers keep an 8-bit cache instead
+    (``QuantizedKVCache``) and attend over it in prompts and decode alike
+    (``gsq_qkv_append``, ``gsq_cached_attention``), and a prompt can go on
+    where the last one or a decode ended (``extend``);
   * a decode step (embedding gather -> 64 layers -> LM head -> argmax ->
     next id) reads its token and position from device buffers, so it is
     captured once as a CUDA graph and replayed per token.
@@ -43,7 +47,8 @@ import torch.nn.functional as F
 
 from .. import _lib
 from ..parallel.tp import reduce_partials
-from ..runtime.kernels import packed_embedding, quantized_matvec
+from ..runtime.kernels import adjust_logits, cached_attention, packed_embedding, quantized_matvec, record_tokens
+from ..runtime.kvcache import QuantizedKVCache
 from ..runtime.store import PackedWeight
 
 
@@ -403,7 +408,7 @@ class Qwen35:
     as with ``group``."""
 
     def __init__(self, weights: dict, cfg: Qwen35Config, device, max_len: int = 2304, group=None,
-                 max_batch: int = 1, reduce_group=None):
+                 max_batch: int = 1, reduce_group=None, kv_format: str | None = None):
         cfg.check()
         if max_batch < 1:
             raise ValueError("max_batch must be at least 1")
@@ -443,8 +448,11 @@ class Qwen35:
                 L["o"] = _Packed([w[p + "attn_output.weight"]])
                 L["q_norm"] = w[p + "attn_q_norm.weight"].float().contiguous()
                 L["k_norm"] = w[p + "attn_k_norm.weight"].float().contiguous()
-                L["k_cache"] = torch.zeros(max_batch, max_len, nkv, hd, device=self.dev)
-                L["v_cache"] = torch.zeros(max_batch, max_len, nkv, hd, device=self.dev)
+                if kv_format is None:
+                    L["k_cache"] = torch.zeros(max_batch, max_len, nkv, hd, device=self.dev)
+                    L["v_cache"] = torch.zeros(max_batch, max_len, nkv, hd, device=self.dev)
+                else:  # handles on the first so many sequences, by their number
+                    L["kv"] = {max_batch: QuantizedKVCache.empty(max_batch, nkv, max_len, hd, kv_format, self.dev)}
             self.layers.append(L)
         self.world = dist.get_world_size(group) if group is not None else 1
         self.reduce_group = reduce_group if reduce_group is not None and dist.get_world_size(reduce_group) > 1 \
@@ -483,6 +491,7 @@ class Qwen35:
         self.cur_id = torch.zeros(max_batch, dtype=torch.int32, device=self.dev)  # tokens to feed next (decode)
         self.n_pos = 0  # host copy of the position (prefill bookkeeping)
         self._graph = None
+        self._logits_control: dict | None = None
         inv = cfg.rope_theta ** (-torch.arange(0, cfg.rotary_dim, 2, dtype=torch.float32) / cfg.rotary_dim)
         self._inv_freq = inv.to(self.dev)
 
@@ -532,9 +541,15 @@ class Qwen35:
             if L["linear"]:
                 L["conv_state"][1:batch].copy_(L["conv_state"][0:1].expand(batch - 1, -1, -1))
                 L["state"][1:batch].copy_(L["state"][0:1].expand(batch - 1, -1, -1, -1))
+            elif "kv" in L:
+                L["kv"][self.max_batch].copy_sequence(0, slice(1, batch), n)
             else:
                 for key in ("k_cache", "v_cache"):
                     L[key][1:batch, :n].copy_(L[key][0:1, :n].expand(batch - 1, -1, -1, -1))
+        if self._logits_control is not None and self._logits_control["history"] is not None:
+            h = self._logits_control["history"]
+            for t in (h.seen, h.counts):
+                t[1:batch].copy_(t[0:1].expand(batch - 1, -1))
         self.cur_id[1:batch].copy_(self.cur_id[0:1].expand(batch - 1))
         self.batch = batch
         self._graph = None
@@ -583,9 +598,26 @@ class Qwen35:
         x1, x2 = x[..., :rot // 2], x[..., rot // 2:rot]
         return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin, x[..., rot:]], dim=-1)
 
+    def _attn_cached(self, L, p: torch.Tensor, batch: int) -> torch.Tensor:
+        """Attention over the 8-bit cache: p's rows are the tokens of
+        ``batch`` sequences at the device position and after it."""
+        cfg, rows = self.cfg, p.shape[0]
+        nq, nkv, hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        kv = L["kv"].get(batch)
+        if kv is None:
+            kv = L["kv"][batch] = L["kv"][self.max_batch].sequences(batch)
+        q = torch.empty(batch, rows // batch, nq, hd, dtype=torch.float16, device=self.dev)
+        _lib.launch(kv.device, _lib.load().gsq_qkv_append, p.data_ptr(), p.stride(0), batch, rows // batch, nq, nkv,
+                    L["q_norm"].data_ptr(), L["k_norm"].data_ptr(), self.eps, cfg.rotary_dim, cfg.rope_theta,
+                    self.pos.data_ptr(), 0, q.data_ptr(), kv.fmt, *kv.pointers, kv.length)
+        gate = p[:, :nq * 2 * hd].unflatten(1, (nq, 2, hd))[:, :, 1].unflatten(0, (batch, -1))
+        return cached_attention(q, kv, self.pos, gate=gate).reshape(rows, nq * hd)
+
     def _attn_prefill(self, L, p: torch.Tensor, pos0: int) -> torch.Tensor:
         cfg, T = self.cfg, p.shape[0]
         nq, nkv, hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        if "kv" in L:
+            return self._attn_cached(L, p, 1)
         if pos0 != 0:
             raise NotImplementedError("multi-token calls start at position 0 (prefill of an empty cache)")
         qg = p[:, :nq * 2 * hd].reshape(T, nq, 2 * hd)
@@ -608,6 +640,8 @@ class Qwen35:
     def _attn_decode(self, L, p: torch.Tensor) -> torch.Tensor:
         """One decode token of each of the batch's p.shape[0] sequences."""
         cfg, B = self.cfg, p.shape[0]
+        if "kv" in L:
+            return self._attn_cached(L, p, B)
         nq, nkv, hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         out = torch.empty(B, nq * hd, dtype=torch.float16, device=self.dev)
         _lib.check(_lib.load().gsq_attn_decode_batch(p.data_ptr(), nq, nkv, L["q_norm"].data_ptr(),
@@ -641,25 +675,75 @@ class Qwen35:
         return delta
 
     # ---- public ----
+    def control_logits(self, *, history=None, repetition=None, frequency=None, presence=None, bias_ids=None,
+                       bias_values=None, allowed=None) -> None:
+        """Adjusts the logits of prefill, extend and every decode step before
+        the next token is taken (``adjust_logits``, same arguments): row b of
+        each tensor (up to max_batch rows, on the model's device) is for
+        sequence b. A ``history`` learns the prompt and the chosen tokens
+        (tokens given to ``decode_step`` are the caller's to record); the
+        tensors may be changed in place between steps, replays of a captured
+        graph included. Without arguments: plain logits again."""
+        given = dict(history=history, repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
+                     bias_values=bias_values, allowed=allowed)
+        if history is not None and history.rows < self.max_batch:
+            raise ValueError(f"the history must have {self.max_batch} rows")
+        self._logits_control = given if any(t is not None for t in given.values()) else None
+        self._graph = None
+
+    def _adjusted(self, logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(logits, next tokens) of the first sequences' rows of logits."""
+        c, rows = self._logits_control, logits.shape[0]
+        if c is None:
+            return logits, torch.argmax(logits, dim=-1).to(torch.int32)
+        rest = {k: t if t is None or (k == "allowed" and t.dim() == 1) else t[:rows]
+                for k, t in c.items() if k != "history"}
+        return adjust_logits(logits, history=c["history"], record=c["history"] is not None, **rest)
+
+    def _prompt(self, ids: torch.Tensor) -> torch.Tensor:
+        """Runs ids through sequence 0 from the current position; returns the last token's logits."""
+        cfg, T = self.cfg, ids.numel()
+        ids = ids.reshape(-1).to(self.dev)
+        x = packed_embedding(ids, self.embed.data, qtype=self.embed.quantization_type,
+                             vocab_size=cfg.vocab_size, dimensions=cfg.hidden_size, dtype=torch.float32)
+        x = x.reshape(T, cfg.hidden_size).contiguous()
+        delta = self._layers(x, self.n_pos)
+        last = x[T - 1:].clone()
+        hf = rmsnorm(last, delta[T - 1:].contiguous(), self.out_norm, self.eps)
+        if self._logits_control is not None and self._logits_control["history"] is not None:
+            record_tokens(self._logits_control["history"], ids.to(torch.int32)[None], generated=False)
+        logits, token = self._adjusted(self.lm_head(hf))
+        self.cur_id[:1].copy_(token)
+        self.n_pos += T
+        self.pos.fill_(self.n_pos)
+        return logits[0]
+
     def prefill(self, ids: torch.Tensor) -> torch.Tensor:
         """Runs a prompt from position 0 (the caches are reset); returns the
         last token's logits (fp32, vocab) and sets the next token to their
         argmax."""
         self.reset()
-        cfg, T = self.cfg, ids.numel()
-        if T > self.max_len:
+        if ids.numel() > self.max_len:
             raise ValueError("prompt longer than the cache")
-        x = packed_embedding(ids.reshape(-1).to(self.dev), self.embed.data, qtype=self.embed.quantization_type,
-                             vocab_size=cfg.vocab_size, dimensions=cfg.hidden_size, dtype=torch.float32)
-        x = x.reshape(T, cfg.hidden_size).contiguous()
-        delta = self._layers(x, 0)
-        last = x[T - 1:].clone()
-        hf = rmsnorm(last, delta[T - 1:].contiguous(), self.out_norm, self.eps)
-        logits = self.lm_head(hf)[0]
-        self.cur_id[:1].copy_(torch.argmax(logits).to(torch.int32).reshape(1))
-        self.pos.fill_(T)
-        self.n_pos = T
-        return logits
+        if self._logits_control is not None and self._logits_control["history"] is not None:
+            h = self._logits_control["history"]
+            h.seen[:1].zero_()
+            h.counts[:1].zero_()
+        return self._prompt(ids)
+
+    def extend(self, ids: torch.Tensor) -> torch.Tensor:
+        """Runs more prompt tokens from the current position of a single
+        sequence (the next turn after a decode, or a long prompt in parts);
+        returns as ``prefill``. Needs an 8-bit cache (``kv_format``)."""
+        if not all(L["linear"] or "kv" in L for L in self.layers):
+            raise NotImplementedError("only a model with a kv_format attends from a later position")
+        if self.batch != 1:
+            raise ValueError("a prompt extends a single sequence")
+        if ids.numel() == 0:
+            raise ValueError("no tokens")
+        if self.n_pos + ids.numel() > self.max_len:
+            raise ValueError("prompt longer than the cache")
+        return self._prompt(ids)
 
     def _decode_body(self) -> torch.Tensor:
         cfg, B = self.cfg, self.batch
@@ -669,8 +753,8 @@ class Qwen35:
         x = x.reshape(B, cfg.hidden_size)
         delta = self._layers(x, None)
         hf = rmsnorm(x, delta, self.out_norm, self.eps)
-        logits = self.lm_head(hf)
-        ids.copy_(torch.argmax(logits, dim=-1).to(torch.int32))
+        logits, tokens = self._adjusted(self.lm_head(hf))
+        ids.copy_(tokens)
         self.pos.add_(1)
         return logits
 
@@ -737,7 +821,7 @@ class Qwen35:
 
 
 def build_qwen35_head_split(weights: dict, cfg: Qwen35Config | None = None, device="cuda", max_len: int = 2304,
-                            group=None, max_batch: int = 1) -> Qwen35:
+                            group=None, max_batch: int = 1, kv_format: str | None = None) -> Qwen35:
     """The model split by heads over the ranks of ``group``: this rank's
     weights and configuration from ``head_split_weights``, the blocks'
     partial outputs summed over the ranks (``Qwen35``'s ``reduce_group``).
@@ -746,13 +830,16 @@ def build_qwen35_head_split(weights: dict, cfg: Qwen35Config | None = None, devi
     world = dist.get_world_size(group) if group is not None else 1
     rank = dist.get_rank(group) if group is not None else 0
     local, local_cfg = head_split_weights(weights, cfg, world, rank)
-    return Qwen35(local, local_cfg, device, max_len=max_len, max_batch=max_batch, reduce_group=group)
+    return Qwen35(local, local_cfg, device, max_len=max_len, max_batch=max_batch, reduce_group=group,
+                  kv_format=kv_format)
 
 
 def build_qwen35(weights: dict, cfg: Qwen35Config | None = None, device="cuda", max_len: int = 2304,
-                 group=None, max_batch: int = 1) -> Qwen35:
+                 group=None, max_batch: int = 1, kv_format: str | None = None) -> Qwen35:
     """The model from GGUF-named weights (``qwen35.py:104-152``): packed
     projections as ``PackedWeight`` on the device, plain tensors as arrays;
     ``group``: split every packed projection over the group's ranks;
-    ``max_batch``: sequences a batched decode can hold (``fork``)."""
-    return Qwen35(weights, cfg or Qwen35Config(), device, max_len=max_len, group=group, max_batch=max_batch)
+    ``max_batch``: sequences a batched decode can hold (``fork``);
+    ``kv_format``: an 8-bit key/value cache, "int8" or "fp8" (None: fp32)."""
+    return Qwen35(weights, cfg or Qwen35Config(), device, max_len=max_len, group=group, max_batch=max_batch,
+                  kv_format=kv_format)

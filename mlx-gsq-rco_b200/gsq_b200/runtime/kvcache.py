@@ -64,6 +64,10 @@ class QuantizedKVCache:
     def nbytes(self) -> int:
         return 2 * self.k.numel() + 8 * self.k_scale.numel()
 
+    def sequences(self, count: int) -> QuantizedKVCache:
+        """A handle on the first ``count`` sequences of the same tensors."""
+        return QuantizedKVCache(self.k[:count], self.v[:count], self.k_scale[:count], self.v_scale[:count])
+
     def copy_sequence(self, source: int, targets: slice, length: int) -> None:
         """The first ``length`` positions of sequence ``source`` into the sequences ``targets``."""
         for t in (self.k.view(torch.int8), self.v.view(torch.int8), self.k_scale, self.v_scale):
