@@ -137,8 +137,8 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
     return fail(GSQ_ERR_SIZE, "gsq_cached_attention: too much work for one call");
   for (int i = 0; i < 3; i++)
     if (q_strides[i] % 8) return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: rows of q not 16-byte aligned");
-  if (!al(q, 16) || !al(out, 16) || !al(gate, 4))
-    return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: q or out not 16-byte aligned, or gate not aligned");
+  if (!al(q, 16) || !al(out, 16) || !words_aligned({start, counts, tree, gate}))
+    return fail(GSQ_ERR_ALIGN, "gsq_cached_attention: q or out not 16-byte aligned, or 4-byte values not aligned");
   AttnArgs a = {};
   a.q = q;
   a.qb = q_strides[0];

@@ -6,9 +6,17 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <utility>
 
 namespace gsq {
+
+// Whether all of the pointers (null ones count) are aligned for their 4-byte values.
+static inline bool words_aligned(std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+  return bits % 4 == 0;
+}
 
 // Launch with programmatic stream serialization (PDL): the kernel may begin
 // while the previous kernel of the stream finishes; it synchronises with

@@ -381,6 +381,7 @@ int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_
   if (tokens < 0 || tokens * heads > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_append: bad token count");
   if (batch == 0 || tokens == 0) return GSQ_OK;
   if (!k || !v || !start || !k_strides || !v_strides) return fail(GSQ_ERR_ARG, "gsq_kv_append: null pointer");
+  if (!words_aligned({start, counts})) return fail(GSQ_ERR_ALIGN, "gsq_kv_append: start or counts not aligned");
   const int64_t size = dtype == DT_F32 ? 4 : 2;
   KvArgs a = {};
   a.src[0] = k;
@@ -424,7 +425,8 @@ int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* 
   if (tokens < 0 || tokens * heads > (1ll << 30)) return fail(GSQ_ERR_SIZE, "gsq_kv_read: bad token count");
   if (batch == 0 || tokens == 0) return GSQ_OK;
   if (!k || !v || !start) return fail(GSQ_ERR_ARG, "gsq_kv_read: null pointer");
-  if (!al16(k) || !al16(v)) return fail(GSQ_ERR_ALIGN, "gsq_kv_read: outputs not 16-byte aligned");
+  if (!al16(k) || !al16(v) || !words_aligned({start, counts}))
+    return fail(GSQ_ERR_ALIGN, "gsq_kv_read: outputs not 16-byte aligned, or start or counts not aligned");
   KvArgs a = {};
   a.dst[0] = k;
   a.dst[1] = v;
@@ -459,7 +461,8 @@ int gsq_qkv_append(const float* qkv, int64_t qkv_stride, int64_t batch, int64_t 
   if (rot < 0 || rot > 256 || rot % 2) return fail(GSQ_ERR_SIZE, "gsq_qkv_append: bad rotary width");
   if (batch == 0 || tokens == 0) return GSQ_OK;
   if (!qkv || !q_norm_w || !k_norm_w || !start || !q) return fail(GSQ_ERR_ARG, "gsq_qkv_append: null pointer");
-  if (!al16(q)) return fail(GSQ_ERR_ALIGN, "gsq_qkv_append: q not 16-byte aligned");
+  if (!al16(q) || !words_aligned({qkv, q_norm_w, k_norm_w, start}))
+    return fail(GSQ_ERR_ALIGN, "gsq_qkv_append: q not 16-byte aligned, or 4-byte values not aligned");
   QkvArgs a = {};
   a.qkv = qkv;
   a.stride = qkv_stride;

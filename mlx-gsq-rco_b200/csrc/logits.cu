@@ -370,7 +370,6 @@ cudaError_t adjust(bool vec, dim3 grid, cudaStream_t st, const LogitsArgs& a) {
   return vec ? adjust_launch<T, true>(grid, st, a) : adjust_launch<T, false>(grid, st, a);
 }
 
-bool al4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
 }  // namespace
 
@@ -390,7 +389,8 @@ int gsq_adjust_logits(const void* logits, int dtype, int64_t row_stride, int64_t
   if (!seen != !counts) return fail(GSQ_ERR_ARG, "gsq_adjust_logits: seen and counts come together");
   if (!seen && (repetition || frequency || presence || record))
     return fail(GSQ_ERR_ARG, "gsq_adjust_logits: penalties and recording need a history");
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2) || !al4(out) || !al4(next))
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == DT_F32 ? 4 : 2) ||
+      !words_aligned({seen, counts, repetition, frequency, presence, bias_ids, bias_values, allowed, out, next}))
     return fail(GSQ_ERR_ALIGN, "gsq_adjust_logits: pointers not aligned to their type");
   LogitsArgs a = {};
   a.logits = logits;
@@ -432,6 +432,8 @@ int gsq_record_tokens(const int32_t* tokens, int64_t row_stride, int64_t rows, i
     return fail(GSQ_ERR_SIZE, "gsq_record_tokens: bad shape");
   if (rows == 0 || n == 0) return GSQ_OK;
   if (!tokens || !seen || !counts) return fail(GSQ_ERR_ARG, "gsq_record_tokens: null pointer");
+  if (!words_aligned({tokens, seen, counts}))
+    return fail(GSQ_ERR_ALIGN, "gsq_record_tokens: pointers not aligned to their type");
   const int64_t blocks = (rows * n + 255) / 256;
   return launched(launch_pdl(record_kernel, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0,
                              (cudaStream_t)stream, tokens, row_stride, rows, n, vocab, (vocab + 31) / 32, seen, counts,

@@ -88,8 +88,8 @@ def adjust_logits(logits: torch.Tensor, *, history=None, repetition: torch.Tenso
                 None if repetition is None else _per_row(repetition, "repetition", rows, dev),
                 None if frequency is None else _per_row(frequency, "frequency", rows, dev),
                 None if presence is None else _per_row(presence, "presence", rows, dev),
-                bias_ids.data_ptr() if biases else None, bias_values.data_ptr() if biases else None, biases, allowed_ptr, allowed_stride, out.data_ptr(),
-                nxt.data_ptr(), int(record))
+                bias_ids.data_ptr() if biases else None, bias_values.data_ptr() if biases else None, biases, allowed_ptr,
+                allowed_stride, out.data_ptr(), nxt.data_ptr(), int(record))
     return out, nxt
 
 

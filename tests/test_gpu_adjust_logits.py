@@ -243,3 +243,46 @@ def test_refusals():
         TokenHistory(h.seen[:, :1], h.counts)
     got, nxt = adjust_logits(z[:0])
     assert got.shape == (0, 64) and nxt.shape == (0,)
+
+
+@pytest.mark.parametrize("rows,vocab,share", [(40, 9001, 0.05), (80, 32000, 0.5), (300, 4097, 1.0), (149, 131, 1.0),
+                                              (2, 1 << 20, 0.3)])
+def test_many_rows_and_dense_histories(rows, vocab, share):
+    """More rows than clusters fit at once; histories up to every token; the largest vocabulary; many biases."""
+    g = torch.Generator().manual_seed(rows)
+    z = 3 * torch.randn(rows, vocab, generator=g)
+    seen, counts, h = history(rows, vocab, 5, share)
+    if share == 1.0:
+        seen[:], counts[counts == 0] = True, 3
+        h = TokenHistory(words(seen).to(DEV), counts.to(DEV))
+    rep, freq, pres = 1 + torch.rand(rows, generator=g), torch.rand(rows, generator=g), torch.rand(rows, generator=g) - .5
+    many = 700
+    ids = torch.stack([torch.randperm(max(vocab, many), generator=g)[:many] for _ in range(rows)]).int()
+    values = torch.randn(rows, many, generator=g)
+    allowed = torch.rand(rows, vocab, generator=g) < 0.7
+    allowed[:, 0] = True
+    # no id comes twice: the sums are the values, and one indexed add does them all
+    want = formula(z, seen, counts, rep, freq, pres)
+    inside = ids < vocab
+    r = torch.arange(rows)[:, None].expand_as(ids)[inside]
+    want[r, ids[inside].long()] += values[inside]
+    want = torch.where(allowed, want, torch.full_like(want, -float("inf")))
+    d = lambda t: t.to(DEV)  # noqa: E731
+    got, nxt = adjust_logits(d(z), history=h, repetition=d(rep), frequency=d(freq), presence=d(pres), bias_ids=d(ids),
+                             bias_values=d(values), allowed=d(words(allowed)), record=True)
+    assert torch.equal(got.cpu(), want) and torch.equal(nxt.cpu(), lowest_best(want))
+    counts[torch.arange(rows), nxt.cpu().long()] += 1
+    seen[torch.arange(rows), nxt.cpu().long()] = True
+    assert torch.equal(h.counts.cpu(), counts) and torch.equal(h.seen.cpu(), words(seen))
+
+
+def test_a_full_list_of_biases():
+    vocab, many = 70000, 65536
+    g = torch.Generator().manual_seed(6)
+    ids = torch.randperm(vocab, generator=g)[None, :many].int()
+    values = torch.randn(1, many, generator=g)
+    z = torch.randn(1, vocab, generator=g)
+    want = z.clone()
+    want[0, ids[0].long()] += values[0]
+    got, nxt = adjust_logits(z.to(DEV), bias_ids=ids.to(DEV), bias_values=values.to(DEV))
+    assert torch.equal(got.cpu(), want) and int(nxt) == int(want.argmax())

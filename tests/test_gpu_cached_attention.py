@@ -338,6 +338,68 @@ def test_captured_and_on_another_stream(n):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,fmt", [(128, "fp8"), (256, "int8")])
+@pytest.mark.parametrize("n,group", [(1, 6), (2, 6), (1, 16), (8, 1), (3, 7)])
+@pytest.mark.parametrize("with_tree", [False, True])
+def test_long_caches_of_ragged_batches(dtype, dim, fmt, n, group, with_tree):
+    """Caches past 8192 positions are split over the GPU at any tile: with padding, starts outside, a gate, few heads."""
+    start, counts, cap = [0, 8192, -2, 137, 9000, 5000], [n, n, n, max(n - 1, 0), n, 0], 8205
+    b, kv = len(start), 2
+    used = [min(max(s + c, 0), cap) for s, c in zip(start, counts)]
+    cache = filled(b, kv, cap, dim, fmt, 31, used)
+    q = queries(b, n, kv * group, dim, dtype, 32)
+    gate = torch.randn(q.shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    parents = random_tree(n, 3)
+    see = visible(b, n, cap, start, counts, [ancestors(parents)] * b if with_tree else None)
+    want, bound = formula(q, cache, see, gate)
+    got = cached_attention(q, cache, i32(*start), counts=i32(*counts), gate=gate,
+                           tree=tree_mask(parents, DEV) if with_tree else None)
+    check(got, want, bound)
+    assert not got[~see.any(-1)].any()
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("batch,kv", [(1, 1), (3, 7), (10, 4), (37, 2), (75, 4), (2, 150)])
+@pytest.mark.parametrize("n", [1, 9])
+def test_any_number_of_sequences_and_heads(dim, batch, kv, n):
+    """From one head of one sequence to more of them than CTAs run at once; lengths differ along the batch."""
+    cap = 300
+    start = [(37 * b) % (cap - n) for b in range(batch)]
+    cache = filled(batch, kv, cap, dim, "int8", 33, [s + n for s in start])
+    q = queries(batch, n, kv, dim, torch.float16, 34)
+    want, bound = formula(q, cache, visible(batch, n, cap, start, None, None))
+    check(cached_attention(q, cache, i32(*start)), want, bound)
+
+
+@pytest.mark.parametrize("cap", [8192, 8193])
+@pytest.mark.parametrize("n", [1, 3])
+def test_both_ways_to_split_a_cache(cap, n):
+    cache = filled(2, 2, cap, 256, "fp8", 35)
+    q = queries(2, n, 12, 256, torch.float16, 36)
+    start = [cap - n, 4000]
+    want, bound = formula(q, cache, visible(2, n, cap, start, None, None))
+    check(cached_attention(q, cache, i32(*start)), want, bound)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("cap", [130, 9000])
+def test_starts_at_the_ends_of_int32(n, cap):
+    cache = filled(4, 1, cap, 128, "int8", 37)
+    q = queries(4, n, 2, 128, torch.float16, 38)
+    start = [2 ** 31 - 1, -2 ** 31, 2 ** 30, -1]
+    want, bound = formula(q, cache, visible(4, n, cap, start, None, None))
+    check(cached_attention(q, cache, i32(*start)), want, bound)
+
+
+def test_a_shared_start_and_counts_past_the_rows():
+    cache = filled(3, 2, 90, 128, "fp8", 39)
+    for n in (2, 20):
+        q = queries(3, n, 4, 128, torch.float16, 40)
+        want, bound = formula(q, cache, visible(3, n, 90, [33] * 3, [n, n, 0], None))
+        check(cached_attention(q, cache, i32(33), counts=i32(n, n + 7, -5)), want, bound)
+
+
 def test_tree_mask_words():
     assert tree_mask([-1, 0, 0, 1, -1], "cpu").flatten().tolist() == [1, 3, 5, 11, 16]
     w = tree_mask(torch.arange(-1, 39), "cpu")

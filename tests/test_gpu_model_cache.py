@@ -262,7 +262,8 @@ def test_the_step_from_projection_to_cache(fmt, rot, b, t, nq, nkv, pad):
     assert ((q.double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2 * off * size).all()
     keys = x[..., 512 * nq:512 * nq + hd * nkv].view(b, t, nkv, hd)
     vals = x[..., 512 * nq + hd * nkv:].view(b, t, nkv, hd)
-    for codes, scales, (want, size) in ((kv.k, kv.k_scale, rotated(keys, kw)), (kv.v, kv.v_scale, (vals, vals.abs() * 0))):
+    exact = (vals, torch.zeros_like(vals))
+    for codes, scales, (want, size) in ((kv.k, kv.k_scale, rotated(keys, kw)), (kv.v, kv.v_scale, exact)):
         for i in range(b):
             p = int(start[i])
             c, s = codes[i, :, p:p + t].double(), scales[i, :, p:p + t, None].double()
