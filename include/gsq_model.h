@@ -134,8 +134,10 @@ GSQ_API int gsq_attn_decode_batch(const float* qkv, int64_t nq, int64_t nkv, con
  * and a stored vector is code * scale.  With a = max|x| over the vector and
  * m = 127 (int8) or 448 (e4m3), scale = a * (1/m) and code = the nearest (ties
  * to even) of x / scale, with 1/m, scale and the quotient each rounded to fp32
- * (scale downwards where m * scale would pass fp32's range).  A zero vector has scale 0; a vector with an Inf
- * or NaN has scale NaN and reads back as NaN.
+ * (scale downwards where m * scale would pass fp32's range).  A zero vector has
+ * scale 0; a vector with an Inf or NaN has scale NaN and codes 0, and reads
+ * back as NaN.  Codes that a caller writes by other means must not be e4m3's
+ * NaN (0x7f, 0xff) in a position that some row of a call sees.
  * dim is 128 or 256; the codes are 16-byte aligned.
  *
  * Sequence b's new tokens begin at position start[b * start_stride] (device

@@ -29,7 +29,8 @@ struct AttnArgs {
   int* err;             // device error word
   float *part, *stat;   // [2 * ctas][rows8][dim], [2 * ctas][rows8][2] (max in base 2, sum)
   struct Joint* joints;  // [ctas], for the joining launch
-  int cluster;           // CTAs per unit (token kernel by units)
+  int cluster, blocks;   // token kernel by units: CTAs per unit, units (of 16 rows each, or 8) per key/value head
+  int joins;             // CTAs that join one unit's parts (row-block kernel)
 };
 
 // Cached positions and new tokens of sequence b. Caches hold at most 2^30 positions, so a start past that sees all of

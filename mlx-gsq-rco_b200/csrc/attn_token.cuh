@@ -1,5 +1,5 @@
 // Attention over the quantised cache for few rows per key/value head (n *
-// group <= 16: single tokens, small trees).
+// group <= 16: single tokens, small trees; more as several units of 16).
 //
 // Bound: HBM bytes of the cache, each read once.  At 6.5 TB/s an SM receives
 // about 23 codes a cycle, so what is done per code has to stay small:
@@ -11,13 +11,12 @@
 //     token's 1 to 8 heads need, where the query as the 16-row operand (or
 //     128 rows of tcgen05) would be mostly padding;
 //   - each warp runs its own softmax over its own 16 positions of a tile of
-//     128, so no barrier or exchange between warps interrupts the stream; the
-//     eight are joined once per unit of work.
+//     64, so no barrier or exchange between warps interrupts the stream; the
+//     four are joined once per unit of work.
 // Every warp copies its own 16 rows of K and V through a private ring
 // (cp.async, positions past the end filled with zeros), with 16-byte units
 // exchanged by the row so that all shared loads are 16 bytes and free of
-// conflicts.  The long axis is split evenly over the CTAs (TileList); a unit
-// that falls into several CTAs is joined by a second launch.
+// conflicts.
 //
 // Weights p are rounded to fp16 (2^-11 each) for the second product; the sum
 // of weights is of the unrounded ones, in fp32.  The values' scales differ by
@@ -26,7 +25,7 @@
 // range, whatever the scales.
 //
 // The work is divided in one of two ways.  UNITS: one cluster of 1 to 8 CTAs
-// for a sequence's head, whose CTAs take a share of its positions each and are
+// for up to 16 rows of a sequence's head, whose CTAs take a share of its positions each and are
 // joined through distributed shared memory; one launch, no scratch.  Else the
 // tiles of all units are split evenly over the CTAs, and a unit that falls
 // into several is joined by a second launch: for long caches, where units of
@@ -152,16 +151,18 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
   float* stat = reinterpret_cast<float*>(smem + G::RING);  // [warp][row][m, l]
   uint2* qfrag = reinterpret_cast<uint2*>(smem + G::RING + G::STAT);
 
-  int first, last;
+  int first, last, r0 = 0, rows = a.n * a.group;  // rows of the unit, from r0 on
   Place get = {};
   if constexpr (UNITS) {
     const int unit = blockIdx.x / a.cluster, rank = blockIdx.x % a.cluster;  // rank == %cluster_ctarank
-    get.b = unit / a.kv;
-    get.kh = unit % a.kv;
+    get.b = unit / (a.kv * a.blocks);
+    get.kh = unit / a.blocks % a.kv;
+    r0 = unit % a.blocks * G::ROWS;
+    rows = min(rows - r0, G::ROWS);
     get.span = seq_span(a, get.b);
     get.tiles = AtShape::tiles(a, get.span, 0);
     if (get.tiles == 0) {  // the whole cluster
-      if (rank == 0) zero_unit<T, D>(a, get.b, get.kh, 0, a.n * a.group);
+      if (rank == 0) zero_unit<T, D>(a, get.b, get.kh, r0, r0 + rows);
       return;
     }
     get.tile = first = rank * get.tiles / a.cluster;
@@ -178,7 +179,6 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
     if (threadIdx.x == 0) AtList::note(a, blockIdx.x, first, get, total, ctas);
   }
   Place use = get;
-  const int rows = a.n * a.group;
 
   // A warp's 16 positions of K and V, copied STEP rows at a time, a 16-byte unit a lane.
   constexpr int U = D / 16, STEP = 32 / U;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int c = 0; c < 2 * CH; c++)
-        raw[x][c] = load_q8<T>(a, use.b, use.kh, 8 * x + g, 64 * (c / 2) + 16 * t + 8 * (c % 2));
+        raw[x][c] = load_q8<T>(a, use.b, use.kh, r0 + 8 * x + g, 64 * (c / 2) + 16 * t + 8 * (c % 2));
   };
   fetch_q();
 
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
       for (int c = 0; c < 2; c++) {
         const int r = 8 * x + 2 * t + c;  // this lane's columns of the score tile; their shift is held by lanes 4r'
         factor[x][c] = a.scale * 1.4426950408889634f * exp2_int(-__shfl_sync(0xffffffffu, shift, 4 * (2 * t + c)));
-        lim[x][c] = r / a.group;
+        lim[x][c] = (r0 + r) / a.group;
         m[x][c] = -INFINITY;
         l[x][c] = 0.f;
       }
@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
 #pragma unroll
           for (int i = 0; i < PIECES; i++) {
             const int r = 8 * x + 2 * tt + c;
-            gate[x][c][i] = r < rows ? load_gate2(a, b, kh, r, 16 * (warp + i * AT_WARPS) + 2 * jj) : make_float2(0.f, 0.f);
+            gate[x][c][i] =
+                r < rows ? load_gate2(a, b, kh, r0 + r, 16 * (warp + i * AT_WARPS) + 2 * jj) : make_float2(0.f, 0.f);
           }
     }
 #pragma unroll
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           const float2 s = *reinterpret_cast<const float2*>(stat + (w * G::ROWS + r) * 2);
           sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);
         }
-        const bool none = sum == 0.f || r / a.group >= span.count;
+        const bool none = sum == 0.f || (r0 + r) / a.group >= span.count;
         const float inv = none ? 0.f : 0x1p-15f / sum;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           if (whole) {
             const float f0 = a.gate ? inv * sigmoid(gate[x][c][i].x) : inv;
             const float f1 = a.gate ? inv * sigmoid(gate[x][c][i].y) : inv;
-            store_row2<T>(a, b, kh, r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
+            store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
           } else if constexpr (UNITS) {
             *reinterpret_cast<float2*>(result(x) + (2 * tt + c) * D + d) = make_float2(v0, v1);
             if (piece == 0 && jj == 0) *reinterpret_cast<float2*>(unit_stat + r * 2) = make_float2(top, sum);
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           s[k] = ld_cluster2(unit_stat + r * 2, k);
           v[k] = ld_cluster2(result(r / 8) + r % 8 * D + d, k);
         }
-        float2 gate2 = a.gate ? load_gate2(a, b, kh, r, d) : make_float2(0.f, 0.f);
+        float2 gate2 = a.gate ? load_gate2(a, b, kh, r0 + r, d) : make_float2(0.f, 0.f);
         float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++)
@@ -542,10 +543,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           x = fmaf(v[k].x, f, x);
           y = fmaf(v[k].y, f, y);
         }
-        const bool none = sum == 0.f || r / a.group >= span.count;
+        const bool none = sum == 0.f || (r0 + r) / a.group >= span.count;
         const float inv = none ? 0.f : 0x1p-15f / sum;
         const float f0 = a.gate ? inv * sigmoid(gate2.x) : inv, f1 = a.gate ? inv * sigmoid(gate2.y) : inv;
-        store_row2<T>(a, b, kh, r, d, none ? 0.f : x * f0, none ? 0.f : y * f1);
+        store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : x * f0, none ? 0.f : y * f1);
       }
       cluster_sync_all();  // no CTA leaves while another may read its shared memory
       return;
@@ -555,8 +556,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
 }
 
 // Joins the partial results of the units that fell into several CTAs, in CTA order, and writes zeros for the rows
-// that no tile reaches. CTA (c, y): the unit that CTA c noted, its rows y, y + gridDim.y, ..; a row's parts over the
-// eight warps, D / 32 values a lane.
+// that no tile reaches. CTAs (c, 0 ..): the unit that CTA c noted. 1 to 8 of their warps take a row together, each some
+// of its parts, D / 32 values a lane: as many as there are for the rows, since what bounds this is the chain of loads
+// along the parts.
 template <typename T, int D, typename Shape>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   constexpr int NV = D / 32;
@@ -574,47 +576,49 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
   }
   const Joint j = a.joints[blockIdx.x];
   if (j.parts == 0) return;
-  const int r0 = j.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS);
-  // few parts: a warp has a row to itself
-  const bool alone = j.parts <= 4;
-  const int step = alone ? 1 : 8;
-  for (int r = alone ? blockIdx.y * 8 + warp : blockIdx.y; r < count; r += alone ? gridDim.y * 8 : gridDim.y) {
+  const int r0 = j.mb * Shape::ROWS, count = min(rows - r0, Shape::ROWS), warps = 8 * gridDim.y;
+  int share = 1;
+  while (share < 8 && 2 * share * count <= warps && 4 * share <= j.parts) share *= 2;
+  for (int base = 0; base < count; base += warps / share) {  // the same for the whole CTA
+    const int r = base + (blockIdx.y * 8 + warp) / share;
+    const bool live = r < count;
     float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < j.parts; i += 32) {
-      const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)j.slot(i) * a.rows8 + r) * 2);
-      add_stat(top, sum, s.x, s.y);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-      add_stat(top, sum, __shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o));
     float o[NV] = {};
-#pragma unroll 4
-    for (int i = alone ? 0 : warp; i < j.parts; i += step) {
-      const int64_t at = (int64_t)j.slot(i) * a.rows8 + r;
-      const float f = part_factor(a.stat[at * 2], top);
+    if (live) {
+      for (int i = lane; i < j.parts; i += 32) {
+        const float2 s = *reinterpret_cast<const float2*>(a.stat + ((int64_t)j.slot(i) * a.rows8 + r) * 2);
+        add_stat(top, sum, s.x, s.y);
+      }
 #pragma unroll
-      for (int e = 0; e < NV; e += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + lane * NV + e);
-        o[e] = fmaf(v.x, f, o[e]);
-        o[e + 1] = fmaf(v.y, f, o[e + 1]);
-        o[e + 2] = fmaf(v.z, f, o[e + 2]);
-        o[e + 3] = fmaf(v.w, f, o[e + 3]);
+      for (int x = 16; x; x >>= 1)
+        add_stat(top, sum, __shfl_xor_sync(0xffffffffu, top, x), __shfl_xor_sync(0xffffffffu, sum, x));
+#pragma unroll 8
+      for (int i = warp % share; i < j.parts; i += share) {
+        const int64_t at = (int64_t)j.slot(i) * a.rows8 + r;
+        const float f = part_factor(a.stat[at * 2], top);
+#pragma unroll
+        for (int e = 0; e < NV; e += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(a.part + at * D + lane * NV + e);
+          o[e] = fmaf(v.x, f, o[e]);
+          o[e + 1] = fmaf(v.y, f, o[e + 1]);
+          o[e + 2] = fmaf(v.z, f, o[e + 2]);
+          o[e + 3] = fmaf(v.w, f, o[e + 3]);
+        }
       }
     }
-    if (!alone) {
+    if (share > 1) {
 #pragma unroll
       for (int e = 0; e < NV; e += 4)
         *reinterpret_cast<float4*>(&acc[warp][lane * NV + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       __syncthreads();
-      if (warp == 0) {
+      if (warp % share == 0) {
+        for (int w = 1; w < share; w++)
 #pragma unroll
-        for (int w = 1; w < 8; w++)
-#pragma unroll
-          for (int e = 0; e < NV; e++) o[e] += acc[w][lane * NV + e];
+          for (int e = 0; e < NV; e++) o[e] += acc[warp + w][lane * NV + e];
       }
       __syncthreads();
-      if (warp) continue;
     }
+    if (!live || warp % share) continue;
     const bool none = sum == 0.f || (r0 + r) / a.group >= j.count;
     const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll

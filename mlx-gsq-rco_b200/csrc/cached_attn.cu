@@ -24,34 +24,66 @@ constexpr int SMS = 148;
 struct Plan {
   int nt;           // 8-row tiles of the token kernel; 0: the row-block kernel
   int cluster;      // token kernel by units: CTAs of a unit; 0: tiles split evenly
+  int blocks;       // and its units per key/value head
+  int joins;        // row-block kernel: CTAs that join one unit's parts
   int ctas, rows8;
   int64_t tiles;    // at most, over all sequences at full length
   size_t workspace;
 };
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Token kernel by units of up to 16 rows: as many CTAs for each unit, up to 8, as fill `most` slots.
+void plan_units(Plan& p, int64_t units, int64_t most) {
+  p.cluster = 1;
+  while (p.cluster < 8 && units * p.cluster * 2 <= most) p.cluster *= 2;
+  p.ctas = (int)(units * p.cluster);
+}
+
 // Up to 16 rows per key/value head the token kernel reads the cache once at the memory's rate; its tensor-core tiles
-// and registers hold two groups of eight rows. From there on the row-block kernel.
+// and registers hold two groups of eight rows.  By units up to 8192 positions: 64 sequences of 2304 take 53 us and one
+// takes 14, against 67 and 17 with the tiles split evenly and joined by a second launch.  Units of longer caches may
+// differ by more than the CTA slots even out, and few units of one need more than 8 CTAs each.
+//
+// More rows: the row-block kernel; or, of caches up to 8192 positions, several units of 16 rows for the token kernel,
+// which read the cache again (from L2).  A tile of 64 positions takes a CTA about as long in either, 1.0 us at 128
+// dimensions and 1.7 at 256.  In these terms a wave of the token kernel's CTAs costs 5 and its tiles; the row-block
+// kernel 8, 1 for every 32 rows (queries loaded, results stored), its tiles, and the joining launch 1 for every 1200
+// rows of parts.  Measured with 4 heads of 256 (us, token kernel and row blocks): one sequence, 42 rows, 1900
+// positions 18 and 21; 128 rows, 700 positions 16 and 25; 24 rows, 8000 positions 32 and 26; 8 sequences of 2000
+// positions, 24 rows 26 and 37, 96 rows 64 and 48.  Past 256 rows the row blocks are full.
 Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, int64_t cap) {
   Plan p = {};
-  const int64_t rows = n * (heads / kv);
-  if (rows <= 16) {
+  const int64_t rows = n * (heads / kv), cached = batch * kv;  // heads in the cache
+  p.blocks = 1;
+  if (rows > 16) {
+    const int64_t units = cached * ceil_div(rows, AR_M), tiles = ceil_div(cap, AR_TILE);
+    p.rows8 = AR_M;
+    p.tiles = units * tiles;
+    p.ctas = (int)std::min<int64_t>(p.tiles, SMS);
+    p.joins = units <= 8 ? 32 : 16;  // few units are in many parts each: 1 unit of 125, 128 rows 42 us with 32, 52 with 16
+    if (rows <= 256 && cap <= 8192) {
+      Plan t = {};
+      t.nt = 2;
+      t.rows8 = 16;
+      t.blocks = (int)ceil_div(rows, 16);
+      t.tiles = cached * t.blocks * tiles;
+      plan_units(t, cached * t.blocks, SMS * 2);
+      const int64_t full = std::min<int64_t>(rows, AR_M), parts = ceil_div(p.ctas, units);
+      if (ceil_div(t.ctas, SMS * 2) * (5 + ceil_div(tiles, t.cluster)) <=
+          8 + full / 32 + ceil_div(p.tiles, p.ctas) + (parts > 1 ? parts * full / 1200 : 0))
+        return t;
+    }
+  } else {
     p.nt = rows <= 8 ? 1 : 2;
     p.rows8 = 8 * p.nt;
-    p.tiles = batch * kv * ((cap + AT_TILE - 1) / AT_TILE);
-  } else {
-    p.rows8 = AR_M;
-    p.tiles = batch * kv * ((rows + AR_M - 1) / AR_M) * ((cap + AR_TILE - 1) / AR_TILE);
-  }
-  const int64_t most = p.nt == 0 ? SMS : SMS * (dim == 128 && p.nt == 1 ? 3 : 2);  // CTAs that run at once
-  p.ctas = (int)(p.tiles < most ? p.tiles : most);
-  // By units where that fills the GPU's `most` CTA slots, or the cache is short. Units of a long cache may differ by
-  // more than the slots even out, and few units of one need more than 8 CTAs each.
-  if (p.nt && cap <= 8192) {
-    const int64_t units = batch * kv;
-    p.cluster = 1;
-    while (p.cluster < 8 && units * p.cluster * 2 <= most) p.cluster *= 2;
-    p.ctas = (int)(units * p.cluster);
-    return p;
+    p.tiles = cached * ceil_div(cap, AT_TILE);
+    const int64_t most = SMS * (dim == 128 && p.nt == 1 ? 3 : 2);  // CTAs that run at once
+    if (cap <= 8192) {
+      plan_units(p, cached, most);
+      return p;
+    }
+    p.ctas = (int)std::min<int64_t>(p.tiles, most);
   }
   p.workspace = (size_t)2 * p.ctas * p.rows8 * (dim + 2) * sizeof(float) + p.ctas * sizeof(Joint);
   return p;
@@ -91,7 +123,7 @@ cudaError_t rows_launch(cudaStream_t st, const AttnArgs& a) {
   if (e == cudaSuccess)
     e = launch_pdl(attn_rows_kernel<T, FMT, D>, dim3((unsigned)a.ctas), dim3(AR_THREADS), smem, st, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, 16), dim3(256), 0, st, a);
+  return launch_pdl(attn_join_kernel<T, D, ArShape>, dim3((unsigned)a.ctas, a.joins), dim3(256), 0, st, a);
 }
 
 template <typename T, int FMT, int D>
@@ -179,6 +211,8 @@ int gsq_cached_attention(const void* q, int dtype, const int64_t* q_strides, int
   a.stat = a.part + (size_t)2 * a.ctas * a.rows8 * dim;
   a.joints = reinterpret_cast<Joint*>(a.stat + (size_t)2 * a.ctas * a.rows8 * 2);
   a.cluster = plan.cluster;
+  a.blocks = plan.blocks;
+  a.joins = plan.joins;
   a.err = device_error_word();
   cudaError_t e = dtype == DT_F16 ? attend<__half>(fmt, plan, st, a) : attend<__nv_bfloat16>(fmt, plan, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();

@@ -34,7 +34,7 @@ constexpr int LG_THREADS = 512;           // of a CTA, at most
 constexpr int LG_QUEUE = 256;             // tokens of a warp's queue
 constexpr int LG_STAGES = 4;              // of a thread's eight tokens, on their way
 constexpr int LG_CLUSTER = 8;             // CTAs of a row, at most
-constexpr int64_t LG_VOCAB = 1ll << 20;   // tokens: the mask of a CTA's biased ones has a bit for each
+constexpr int64_t LG_VOCAB = 1ll << 20;   // tokens at most: 2^18 a CTA, whose masks fit its shared memory
 
 struct LogitsArgs {
   const void* logits;
