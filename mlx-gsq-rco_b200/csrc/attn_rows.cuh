@@ -19,13 +19,22 @@
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs.
 // Roles (20 warps): two softmax warpgroups, one row a thread, that take the
-// two halves of every tile's columns; two that dequantise; one thread issues
-// the products, one the bulk copies of codes (a tile is one contiguous piece).
+// two halves of every tile's columns; two that dequantise; one warp issues the
+// products, one thread the bulk copies of codes (a tile is one contiguous
+// piece), one warp prepares the tile's scales.  S has two tiles in TMEM, and
+// P takes the place of the scores it comes from, so the next tile's scores are
+// there when the softmax is through with one.
 // The groups pass each other the largest score of a row's half, so that both
 // follow the same reference (the running maximum). Half a tile a thread keeps
 // the softmax loop, which is unrolled over its scores, short enough for the
 // instruction caches: with whole tiles in turn a fifth of its time went into
 // instruction misses.
+// Measured (777 rows of 6 heads on each of 4, after 23224 positions of 256):
+// 566 us, 796 TFLOP/s, 48 % of the tensor core's measured rate; about 2500
+// cycles a tile, of which the softmax warps are busy 2000 (their instructions
+// depend on one another, and two of them share an issue slot with dequantising
+// warps).  Products issued by one lane with values of its own: 634; scales
+// prepared by every softmax warp: 610.
 // The reference is followed lazily: O is rescaled only when it grows by more
 // than 2^8, which weights of up to 2^14 in fp16 leave room for.
 // Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded
@@ -47,22 +56,22 @@ struct ArGeom {
   static constexpr int STAGES = D == 256 ? 5 : 6;
   static constexpr int RAW = AR_TILE * D;       // its codes
   static constexpr int RAWS = 3;
-  static constexpr int SCALES = AR_SOFTMAX * 5 * AR_HALF * 4;
+  static constexpr int SCALES = 2 * (6 * AR_HALF + 4) * 4;  // of two tiles, with a mask for each half
   static constexpr int STATE = 6 * AR_M * 4;    // the two groups' maxima of two tiles, and their sums
   static constexpr int SMEM = 1024 + STAGES * ITEM + RAWS * RAW + SCALES + STATE + 512;
-  static constexpr int O = 0, Q = D, S = Q + D / 2, P = S + AR_TILE;  // TMEM columns
+  static constexpr int O = 0, Q = D, S = Q + D / 2;  // TMEM columns; S: two tiles
   static constexpr int COLS = 512;
-  static_assert(P + AR_TILE <= COLS && SMEM <= 227 * 1024, "fits");
+  static_assert(S + 2 * AR_TILE <= COLS && SMEM <= 227 * 1024, "fits");
 };
 
 struct ArShape {  // blocks of 128 rows; with a causal mask an early block sees fewer positions
   static constexpr int ROWS = AR_M;
-  __device__ static int blocks(const AttnArgs& a) { return (a.n * a.group + AR_M - 1) / AR_M; }
+  __device__ static int blocks(const AttnArgs& a) { return (a.n * a.group + ROWS - 1) / ROWS; }
   __device__ static int tiles(const AttnArgs& a, const SeqSpan& s, int mb) {
-    if (mb * AR_M / a.group >= s.count) return 0;
+    if (mb * ROWS / a.group >= s.count) return 0;
     int len = s.len;
     if (!a.tree) {
-      const int last = min(((mb + 1) * AR_M - 1) / a.group, s.count - 1);
+      const int last = min(((mb + 1) * ROWS - 1) / a.group, s.count - 1);
       len = min(max(s.base + last + 1, 0), (int)a.cap);
     }
     return (len + AR_TILE - 1) / AR_TILE;
@@ -146,6 +155,13 @@ __host__ __device__ constexpr uint32_t ar_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(AR_M >> 4) << 24);
 }
 
+// One lane of the warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
+}
+
 // Pairs of fp32 in one register pair and one instruction.
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pair(float x, float y) {
@@ -161,6 +177,11 @@ __device__ __forceinline__ float2 halves(f32x2 p) {
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   f32x2 c;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c) : "l"(a), "l"(b));
+  return c;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 c;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c) : "l"(a), "l"(b));
   return c;
 }
 __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
@@ -189,6 +210,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, ar_wait(bar, parity, err));
 }
 
+// The two warps of 32 rows meet (hardware barriers 1 .. 4, in a fraction of an mbarrier's time). It has no limit, so a
+// warp that gives up still meets the other as often as that one will wait.
+__device__ __forceinline__ void ar_meet(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
+
 // Which of positions p0 .. p0 + 63 token i of sequence b sees, as bits.
 __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const SeqSpan& s, int i, int p0) {
   if (i >= s.count) return 0;
@@ -209,11 +234,10 @@ __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const S
   return m & below(s.len - p0);
 }
 
-// Scales of the warp's 32 positions, one a lane, as the softmax uses them: the key's times `factor`, log2 of the value's
-// and its inverse in linear terms, in the warp's own copy. Returns the positions (bits) whose value scale is 0.
-__device__ __forceinline__ uint32_t ar_scales(float* ks, float factor) {
+// Scales of 32 positions, one a lane, as the softmax uses them: the key's times `factor`, log2 of the value's and its
+// inverse in linear terms, in 96 floats at `out`. Returns the positions (bits) whose value scale is 0.
+__device__ __forceinline__ uint32_t ar_scales(float k, float v, float factor, float* out) {
   const int lane = threadIdx.x & 31;
-  const float k = ks[3 * AR_HALF + lane], v = ks[4 * AR_HALF + lane];
   // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of scale 0 has
   // no part in the output, but in the sum of weights: it is weighted with the largest scale beside it, and that weight
   // left out of P. NaN stays, with 1 / vs as 0, so that a row that does not see the position takes no harm.
@@ -226,9 +250,9 @@ __device__ __forceinline__ uint32_t ar_scales(float* ks, float factor) {
     if (v == 0.f) lv = top == -INFINITY ? -40.f : top;
   }
   const bool nan = isnan(v);
-  ks[lane] = k * factor;
-  ks[AR_HALF + lane] = nan ? v : lv;
-  ks[2 * AR_HALF + lane] = nan ? 0.f : exp2_approx(-lv);
+  out[lane] = k * factor;
+  out[AR_HALF + lane] = nan ? v : lv;
+  out[2 * AR_HALF + lane] = nan ? 0.f : exp2_approx(-lv);
   return zeros;
 }
 
@@ -238,26 +262,24 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // (an offset: the pointer stays a shared one)
   uint8_t* raw = smem + G::STAGES * G::ITEM;
-  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [softmax warp][ks | log2 vs | 1 / vs | next ks | next vs][32]
+  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [tile & 1][half][ks | log2 vs | 1 / vs][32], masks
   float* tops = scales + G::SCALES / 4;   // [tile & 1][group][128]: largest scores, to base 2
   float* sums = tops + 4 * AR_M;          // [group][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sums + 2 * AR_M);
   uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
   uint64_t* empty = full + G::STAGES;     // [STAGES] commit
-  uint64_t* s_full = empty + G::STAGES;   // commit
-  uint64_t* s_free = s_full + 1;          // count AR_SOFTMAX
-  uint64_t* p_full = s_free + 1;          // [tile & 1] count AR_SOFTMAX
+  uint64_t* s_full = empty + G::STAGES;   // [tile & 1] commit, and the tile's scales
+  uint64_t* p_full = s_full + 2;          // [tile & 1] count AR_SOFTMAX
   uint64_t* pv_done = p_full + 2;         // [tile & 1] commit
   uint64_t* q_full = pv_done + 2;         // count AR_SOFTMAX
-  uint64_t* top_done = q_full + 1;        // [32 rows] count 2: both groups' maxima are there
-  uint64_t* sum_done = top_done + 4;      // [32 rows] count 2: both groups' sums are there
+  uint64_t* sum_done = q_full + 1;      // [32 rows] count 2: both groups' sums are there
   uint64_t* drained = sum_done + 4;       // commit
   uint64_t* raw_full = drained + 1;       // [RAWS] the copy
   uint64_t* raw_empty = raw_full + G::RAWS;  // [RAWS] count AR_DEQUANT
   int* raw_rows = reinterpret_cast<int*>(raw_empty + G::RAWS);  // [RAWS] positions in the stage
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_rows + G::RAWS);
-  static_assert((2 * G::STAGES + 17 + 2 * G::RAWS) * 8 + 4 * G::RAWS + 4 <= 512, "barriers");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert((2 * G::STAGES + 12 + 2 * G::RAWS) * 8 + 4 * G::RAWS + 4 <= 512, "barriers");
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == AR_SOFTMAX + AR_DEQUANT) tmem_alloc(tmem_slot, G::COLS);
   if (threadIdx.x == 0) {
@@ -265,15 +287,13 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       mbar_init(&full[i], AR_DEQUANT);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, AR_SOFTMAX);
     for (int i = 0; i < 2; i++) {
+      mbar_init(&s_full[i], 2);
       mbar_init(&p_full[i], AR_SOFTMAX);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, AR_SOFTMAX);
     for (int i = 0; i < 4; i++) {
-      mbar_init(&top_done[i], 2);
       mbar_init(&sum_done[i], 2);
     }
     mbar_init(drained, 1);
@@ -304,10 +324,9 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     const int group = warp / AR_GROUP, quarter = warp % AR_GROUP, row = threadIdx.x % AR_M;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16);
     const int rows = a.n * a.group;
-    float* ks = scales + warp * 5 * AR_HALF;
     ArRun run;
     run.begin(a, first, last);
-    int tile = 0, runs = 0;  // of the CTA
+    int tile = 0, runs = 0, met = 0;  // of the CTA
     do {
       const int r = run.at.mb * AR_M + row;  // row of the unit's head
       const int i = r / a.group;
@@ -329,7 +348,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         shift = q_shift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))));
       }
       const float up = (a.scale < 0.f ? -1.f : 1.f) * exp2_int(shift);
-      const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);
+      const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);  // fp16: with the keys' scales
+      const f32x2 factor2 = pair(factor, factor);
 #pragma unroll 1
       for (int c = group * (D / 128); c < (group + 1) * (D / 128); c++) {
         uint32_t w[32];
@@ -350,35 +370,20 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
 
-      const int64_t row0 = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap;
-      // Scales of the coming half tile, copied while the last one is worked on (loads into registers would be waited
-      // for at the next arrival on a barrier); 0 past the end
-      auto fetch_scales = [&](int p) {
-        const bool in = p < run.at.span.len;
-        cp_async4_zfill(ks + 3 * AR_HALF + lane, a.ks + (in ? row0 + p : 0), in);
-        cp_async4_zfill(ks + 4 * AR_HALF + lane, a.vs + (in ? row0 + p : 0), in);
-        cp_async_commit();
-      };
       const int run0 = tile;  // the run's first tile
-      fetch_scales(run.at.tile * AR_TILE + group * AR_HALF + lane);
 
       float ref = -INFINITY, sum = 0.f;  // of the row; the sum of this group's half
       for (; tile < run0 + run.len; tile++) {
         const int p0 = (run.at.tile + tile - run0) * AR_TILE + group * AR_HALF;
-        cp_async_wait<0>();
-        __syncwarp();  // this half's are there, and the warp has read the last one's
-        const uint32_t zeros = ar_scales(ks, factor);
-        __syncwarp();
-        if (tile + 1 < run0 + run.len) fetch_scales(p0 + AR_TILE + lane);
-        ok = warp_wait(s_full, (uint32_t)(tile & 1), a.err);
+        ok = warp_wait(&s_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
         if (!ok) break;
         tc_fence_after();
+        const float* ks = scales + (tile & 1) * (6 * AR_HALF + 4) + group * 3 * AR_HALF;
+        const uint32_t zeros = reinterpret_cast<const uint32_t*>(scales)[(tile & 1) * (6 * AR_HALF + 4) + 6 * AR_HALF + group];
+        const uint32_t scores = lanes + G::S + (tile & 1) * AR_TILE + group * AR_HALF;
         uint32_t s[AR_HALF];
-        tmem_ld32(lanes + G::S + group * AR_HALF, s);
+        tmem_ld32(scores, s);
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
 
         // t = ks * s + log2 vs, and the row's maximum over both halves
         f32x2 t[AR_HALF / 2];
@@ -386,8 +391,14 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         for (int e = 0; e < AR_HALF; e += 4) {
           const ulonglong2 k4 = *reinterpret_cast<const ulonglong2*>(ks + e);
           const ulonglong2 v4 = *reinterpret_cast<const ulonglong2*>(ks + AR_HALF + e);
-          t[e / 2] = fma2(pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), k4.x, v4.x);
-          t[e / 2 + 1] = fma2(pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), k4.y, v4.y);
+          f32x2 x = pair(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+          f32x2 y = pair(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
+          if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            x = mul2(x, factor2);
+            y = mul2(y, factor2);
+          }
+          t[e / 2] = fma2(x, k4.x, v4.x);
+          t[e / 2 + 1] = fma2(y, k4.y, v4.y);
         }
         if (p0 + AR_HALF > min(run.at.span.base, run.at.span.len)) {  // the same for all threads
           const uint32_t see = (uint32_t)ar_visible(a, run.at.b, run.at.span, i, p0);
@@ -406,10 +417,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
         float* mine = tops + (tile & 1) * 2 * AR_M + row;
         mine[group * AR_M] = top;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&top_done[quarter]);
-        ok = warp_wait(&top_done[quarter], (uint32_t)(tile & 1), a.err);
-        if (!ok) break;
+        ar_meet(quarter);
+        met++;
         top = fmaxf(top, mine[(1 - group) * AR_M]);
         const bool grow = top > ref + 8.f || (ref == -INFINITY && top > ref);
         if (__any_sync(0xffffffffu, grow)) {
@@ -459,11 +468,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           for (int e = 0; e < AR_HALF / 2; e++)
             w[e] &= (zeros >> 2 * e & 1 ? 0u : 0xffffu) | (zeros >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
         }
-        if (tile >= 2) {  // the P of tile - 2 has been read
-          ok = warp_wait(&pv_done[tile & 1], (uint32_t)((tile / 2 - 1) & 1), a.err);
-          if (!ok) break;
-        }
-        tmem_st16(lanes + G::P + (tile & 1) * (AR_TILE / 2) + group * (AR_HALF / 2), w);
+        tmem_st16(scores, w);  // over the first half of the scores that they come from
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -510,6 +515,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * AR_M + row) * 2) = make_float2(ref, sum);
       tc_fence_before();  // the loads of O come before the next unit's products (through q_full)
     } while (run.next(a));
+    for (; met < last - first; met++) ar_meet(quarter);
   } else if (warp < AR_SOFTMAX + AR_DEQUANT) {
     // ---------------- dequantise ----------------
     // A warp takes whole rows (D = 256: one, a lane 8 codes; D = 128: two), 8 codes becoming one 16-byte chunk of the
@@ -558,49 +564,64 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     }
   } else {
     ArRun run;
-    if (warp < AR_SOFTMAX + AR_DEQUANT + 2) run.begin(a, first, last);
-    if (warp == AR_SOFTMAX + AR_DEQUANT && lane == 0) {
-      // ---------------- issue the products: one thread ----------------
-      ArList::note(a, blockIdx.x, first, run.at, total, ctas);
+    if (warp < AR_SOFTMAX + AR_DEQUANT + 3) run.begin(a, first, last);
+    if (warp == AR_SOFTMAX + AR_DEQUANT) {
+      // ---------------- issue the products: one warp, one of its lanes. All values are the warp's (broadcast where
+      // the compiler cannot see it), so that operands and descriptors are built in uniform registers: with one lane's
+      // own values the issue of a tile's products took 2300 cycles, longer than the products ----------------
+      if (lane == 0) ArList::note(a, blockIdx.x, first, run.at, total, ctas);
+      const bool leader = elect_one();
       int stage = 0, use = 0, tile = 0, runs = 0;
-      const uint32_t items = smem_u32(smem);
-      // S of the CTA's tile t: into TMEM when the softmax has taken tile t - 1's
+      const uint32_t items = smem_u32(smem), tm = __shfl_sync(0xffffffffu, tmem, 0);
+      auto wait = [&](uint64_t* bar, int parity) {
+        return __all_sync(0xffffffffu, ar_wait(bar, (uint32_t)(parity & 1), a.err)) != 0;
+      };
+      // S of the CTA's tile t, where the weights of tile t - 2 were
       auto scores = [&](int t) {
-        ok = ar_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
-             (t == 0 || ar_wait(s_free, (uint32_t)((t - 1) & 1), a.err));
+        ok = wait(&full[stage], use) && (t < 2 || wait(&pv_done[t & 1], t / 2 - 1));
         if (!ok) return;
         tc_fence_after();
-        const uint32_t b = ar_k_major(items + stage * G::ITEM);
+        const uint32_t b = ar_k_major(items + stage * G::ITEM), d = tm + G::S + (t & 1) * AR_TILE;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < D / 16; k++)
-          tc_mma_f16_ts(tmem + G::S, tmem + G::Q + 8 * k, ar_desc(b + k / 4 * (AR_TILE * 128 / 16) + k % 4 * 2),
-                        ar_idesc(AR_TILE, false), k != 0);
-        tc_commit(&empty[stage]);
-        tc_commit(s_full);
+          for (int k = 0; k < D / 16; k++)
+            tc_mma_f16_ts(d, tm + G::Q + 8 * k, ar_desc(b + k / 4 * (AR_TILE * 128 / 16) + k % 4 * 2),
+                                ar_idesc(AR_TILE, false), k != 0);
+          tc_commit(&empty[stage]);
+          tc_commit(&s_full[t & 1]);
+        }
+        __syncwarp();
         if (++stage == G::STAGES) stage = 0, use++;
       };
-      do {
-        ok = ar_wait(q_full, (uint32_t)(runs++ & 1), a.err);
+      bool more = true;
+      while (more) {
+        const int len = __shfl_sync(0xffffffffu, run.len, 0);
+        ok = wait(q_full, runs++);
         if (!ok) break;
         scores(tile);
-        for (int j = 0; j < run.len && ok; j++, tile++) {
-          if (j + 1 < run.len) scores(tile + 1);
-          ok = ok && ar_wait(&full[stage], (uint32_t)(use & 1), a.err) &&
-               ar_wait(&p_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
+        if (ok && len > 1) scores(tile + 1);
+        for (int j = 0; j < len && ok; j++, tile++) {
+          ok = wait(&full[stage], use) && wait(&p_full[tile & 1], tile / 2);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = ar_mn_major(items + stage * G::ITEM, AR_TILE * 128);
-          const uint32_t p = tmem + G::P + (tile & 1) * (AR_TILE / 2);
+          const uint32_t b = ar_mn_major(items + stage * G::ITEM, AR_TILE * 128), p = tm + G::S + (tile & 1) * AR_TILE;
+          if (leader) {
 #pragma unroll
-          for (int k = 0; k < AR_TILE / 16; k++)
-            tc_mma_f16_ts(tmem + G::O, p + 8 * k, ar_desc(b + k * (2048 / 16)), ar_idesc(D, true), (j | k) != 0);
-          tc_commit(&empty[stage]);
-          tc_commit(&pv_done[tile & 1]);
+            for (int k = 0; k < AR_TILE / 16; k++)  // (weights of 32 positions in 16 columns, the others' 32 columns on)
+              tc_mma_f16_ts(tm + G::O, p + k / 2 * AR_HALF + k % 2 * 8, ar_desc(b + k * (2048 / 16)),
+                                  ar_idesc(D, true), (j | k) != 0);
+            tc_commit(&empty[stage]);
+            tc_commit(&pv_done[tile & 1]);
+          }
+          __syncwarp();
           if (++stage == G::STAGES) stage = 0, use++;
+          if (j + 2 < len) scores(tile + 2);
         }
-      } while (ok && run.next(a));
+        more = __all_sync(0xffffffffu, ok && run.next(a)) != 0;
+      }
       // nothing may still write TMEM when it is given back
-      tc_commit(drained);
+      if (leader) tc_commit(drained);
+      __syncwarp();
       ar_wait(drained, 0, a.err);
     } else if (warp == AR_SOFTMAX + AR_DEQUANT + 1 && lane == 0) {
       // ---------------- copy the codes: one thread; items in the order K0, K1, V0, K2, V1, .. of each run --------
@@ -627,6 +648,42 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       for (int i = 0; i < G::RAWS; i++) {
         const int uses = ruse + (i < rs ? 1 : 0);
         if (uses > 0) ar_wait(&raw_full[i], (uint32_t)((uses - 1) & 1), a.err);
+      }
+    } else if (warp == AR_SOFTMAX + AR_DEQUANT + 2) {
+      // ---------------- the tiles' scales: two positions a lane, loaded a tile ahead ----------------
+      const float factor =
+          std::is_same<T, __half>::value ? fabsf(a.scale) * 1.4426950408889634f : 1.f;  // bf16: a row's own, later
+      float k[2], v[2];
+      int j = 0;
+      auto load = [&]() {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int p = (run.at.tile + j) * AR_TILE + h * AR_HALF + lane;
+          const bool in = p < run.at.span.len;
+          const int64_t at = ((int64_t)run.at.b * a.kv + run.at.kh) * a.cap + p;
+          k[h] = in ? a.ks[at] : 0.f;
+          v[h] = in ? a.vs[at] : 0.f;
+        }
+      };
+      load();
+      for (int t = 0; t < last - first; t++) {
+        if (t >= 2) {  // the softmax is through with tile t - 2
+          ok = warp_wait(&pv_done[t & 1], (uint32_t)((t / 2 - 1) & 1), a.err);
+          if (!ok) break;
+        }
+        float* out = scales + (t & 1) * (6 * AR_HALF + 4);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t zeros = ar_scales(k[h], v[h], factor, out + h * 3 * AR_HALF);
+          if (lane == 0) reinterpret_cast<uint32_t*>(out)[6 * AR_HALF + h] = zeros;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_full[t & 1]);
+        if (++j == run.len) {
+          j = 0;
+          if (!run.next(a)) break;
+        }
+        load();
       }
     }
     __syncwarp();
