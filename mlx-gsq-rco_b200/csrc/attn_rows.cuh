@@ -30,11 +30,12 @@
 // instruction caches: with whole tiles in turn a fifth of its time went into
 // instruction misses.
 // Measured (777 rows of 6 heads on each of 4, after 23224 positions of 256):
-// 566 us, 796 TFLOP/s, 48 % of the tensor core's measured rate; about 2500
+// 566 us, 796 TFLOP/s, 48 % of the tensor core's measured rate; about 2300
 // cycles a tile, of which the softmax warps are busy 2000 (their instructions
 // depend on one another, and two of them share an issue slot with dequantising
-// warps).  Products issued by one lane with values of its own: 634; scales
-// prepared by every softmax warp: 610.
+// warps).  With all rows seeing all positions 476 us; there, products issued
+// by one lane with values of its own took 562, and scales prepared by each
+// softmax warp for itself 542.
 // The reference is followed lazily: O is rescaled only when it grows by more
 // than 2^8, which weights of up to 2^14 in fp16 leave room for.
 // Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded

@@ -33,15 +33,18 @@ struct Plan {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Token kernel by units of up to 16 rows: as many CTAs for each unit, up to 8, as fill `most` slots.
-void plan_units(Plan& p, int64_t units, int64_t most) {
+// Token kernel by units of up to 16 rows: as many CTAs for each unit, up to 8, as fill `most` slots; twice as many where
+// a CTA would still have more than 64 tiles, since units of unlike length then even out (64 sequences, 4 heads of 256:
+// up to 8000 positions 154 us and with twice as many CTAs 101, all of 8000 169 and 175; up to 2304 positions, 36 tiles,
+// 49 and 42, but all of 2304 54 and 63).
+void plan_units(Plan& p, int64_t units, int64_t most, int64_t tiles) {
   p.cluster = 1;
-  while (p.cluster < 8 && units * p.cluster * 2 <= most) p.cluster *= 2;
+  while (p.cluster < 8 && units * p.cluster * (tiles > 64 * p.cluster ? 1 : 2) <= most) p.cluster *= 2;
   p.ctas = (int)(units * p.cluster);
 }
 
 // Up to 16 rows per key/value head the token kernel reads the cache once at the memory's rate; its tensor-core tiles
-// and registers hold two groups of eight rows.  By units up to 8192 positions: 64 sequences of 2304 take 53 us and one
+// and registers hold two groups of eight rows.  By units up to 8192 positions: 64 ragged sequences of 2304 take 53 us and one
 // takes 14, against 67 and 17 with the tiles split evenly and joined by a second launch.  Units of longer caches may
 // differ by more than the CTA slots even out, and few units of one need more than 8 CTAs each.
 //
@@ -68,7 +71,7 @@ Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, i
       t.rows8 = 16;
       t.blocks = (int)ceil_div(rows, 16);
       t.tiles = cached * t.blocks * tiles;
-      plan_units(t, cached * t.blocks, SMS * 2);
+      plan_units(t, cached * t.blocks, SMS * 2, tiles);
       const int64_t full = std::min<int64_t>(rows, AR_M), parts = ceil_div(p.ctas, units);
       if (ceil_div(t.ctas, SMS * 2) * (5 + ceil_div(tiles, t.cluster)) <=
           8 + full / 32 + ceil_div(p.tiles, p.ctas) + (parts > 1 ? parts * full / 1200 : 0))
@@ -80,7 +83,7 @@ Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, i
     p.tiles = cached * ceil_div(cap, AT_TILE);
     const int64_t most = SMS * (dim == 128 && p.nt == 1 ? 3 : 2);  // CTAs that run at once
     if (cap <= 8192) {
-      plan_units(p, cached, most);
+      plan_units(p, cached, most, ceil_div(cap, AT_TILE));
       return p;
     }
     p.ctas = (int)std::min<int64_t>(p.tiles, most);
