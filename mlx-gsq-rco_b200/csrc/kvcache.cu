@@ -11,7 +11,9 @@
 // Bound: HBM bytes (input + D + 4 a vector), or the launch for one token.
 // One warp per vector: the whole vector sits in the warp's registers (D / 32
 // values a lane), so nothing is read twice; a warp takes KV_EACH vectors, all
-// loaded before the first is worked on.
+// loaded before the first is worked on.  Measured with 8 x 1999 tokens of 4
+// heads of 256, bf16: append 33 us (98 MB, 3.0 TB/s: instructions), read 15 us
+// of e4m3 (6.5 TB/s: HBM), 18 us of int8.
 #include <cuda_fp8.h>
 
 #include <cstdio>
@@ -85,36 +87,35 @@ __device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N
   scale = __fmul_rn(m, 1.f / M);
   if (m > 1e38f) scale = fminf(scale, __fdiv_rd(3.402823466e38f, M));  // M * scale stays finite
   if (top >= 0x7f800000u) scale = __int_as_float(0x7fffffff);
-  // code = nearest of fl(x / scale). x * (1 / scale) is within 2^-22 of that quotient, so where both ends of
-  // +-2^-21 around it have the same nearest code, that is the code, without a division; near a tie, or where the
-  // reciprocal may leave the normal range, it is divided.
-  uint32_t differ = scale > 1e-30f ? 0u : 1u;
-  float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));  // within 2^-23
-  const float up = inv * (1.f + 0x1p-21f), down = inv * (1.f - 0x1p-21f);
+  // The quotient correctly rounded, by Markstein's theorem: with y the correctly rounded reciprocal and q within one
+  // unit of x / scale, q + (x - q scale) y rounds to it. q is x times the reciprocal in two parts, neither negative, so
+  // that a zero keeps its sign. The remainder is exact as long as q scale does not underflow, which for scales from
+  // 2^-60 on only concerns quotients of code 0. (A product with the reciprocal alone, rounded both ways, and a division
+  // where the codes differed, took 38 us where this takes 33: 39 % of bf16 vectors hold a tie of int8, such as a value
+  // half as large as the largest.)
+  if (scale >= 0x1p-60f) {  // the same for the warp
+    const float y = __frcp_rn(scale);
+    const float high = __uint_as_float(__float_as_uint(y) - (fmaf(-scale, y, 1.f) < 0.f ? 1u : 0u));
+    const float low = fmaf(-scale, high, 1.f) * y;
+    const f32x2 high2 = pair(high, high), low2 = pair(low, low), minus2 = pair(-y, -y), scale2 = pair(scale, scale);
+    auto quotient = [&](float a, float b) {
+      const f32x2 x = pair(a, b), q = fma2(x, high2, mul2(x, low2));
+      return fma2(fma2(q, scale2, pair(-a, -b)), minus2, q);
+    };
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    if constexpr (FMT == KV_INT8) {
-      constexpr float R = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest integer, ties to even
-      uint32_t u[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        u[e] = __float_as_uint(fmaf(f[i + e], up, R));
-        differ |= u[e] ^ __float_as_uint(fmaf(f[i + e], down, R));
+    for (int i = 0; i < N; i += 4) {
+      const f32x2 a = quotient(f[i], f[i + 1]), b = quotient(f[i + 2], f[i + 3]);
+      if constexpr (FMT == KV_INT8) {
+        const f32x2 R = pair(12582912.f, 12582912.f);  // 1.5 * 2^23: a sum's low bits are the nearest integer, ties to even
+        const float2 u = halves(add2(a, R)), v = halves(add2(b, R));
+        code[i / 4] = __byte_perm(__byte_perm(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040),
+                                  __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040), 0x5410);
+      } else {
+        const uint32_t u = __nv_cvt_float2_to_fp8x2(halves(a), __NV_SATFINITE, __NV_E4M3);
+        code[i / 4] = __byte_perm(u, __nv_cvt_float2_to_fp8x2(halves(b), __NV_SATFINITE, __NV_E4M3), 0x5410);
       }
-      code[i / 4] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-    } else {
-      uint32_t u[2];
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const float x = f[i + 2 * e], y = f[i + 2 * e + 1];
-        u[e] = __nv_cvt_float2_to_fp8x2(make_float2(x * up, y * up), __NV_SATFINITE, __NV_E4M3);
-        differ |= u[e] ^ __nv_cvt_float2_to_fp8x2(make_float2(x * down, y * down), __NV_SATFINITE, __NV_E4M3);
-      }
-      code[i / 4] = __byte_perm(u[0], u[1], 0x5410);
     }
-  }
-  if (differ) {
+  } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
       uint32_t w = 0;

@@ -217,3 +217,30 @@ def test_refusals():
         kv_read(c, i32(0), -1)
     kv_append(c, x[:, :0], x[:, :0], i32(0))  # nothing to do
     assert kv_read(c, i32(0), 0)[0].shape == (2, 0, 3, 128)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 300.0, 1e30, 1e37, 1e-17, 1e-30])
+def test_codes_are_the_divisions(fmt, dtype, size):
+    """Every code of many vectors is the nearest of the fp32 quotient, bit for bit, zeros' signs included; short types
+    make many ties (a value half as large as the vector's largest is one of int8)."""
+    if dtype == torch.float16 and not 1e-3 <= size <= 300:
+        pytest.skip("outside fp16")
+    g = torch.Generator().manual_seed(41)
+    x = (torch.randn(1, 3000, 2, 256, generator=g) * size).to(dtype)
+    x[0, ::7, 0, 5] = -0.0
+    x[0, ::5, 1, 9] = 0.0
+    x[0, ::3, 0, 7] = x[0, ::3, 0].abs().amax(-1) / 2
+    x[0, ::4, 1, 8] = -x[0, ::4, 1].abs().amax(-1) / 4
+    cache = QuantizedKVCache.empty(1, 2, 3000, 256, fmt, "cuda:0")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+    kv_append(cache, x.to("cuda:0"), (-x).to("cuda:0"), zero)
+    m = 127.0 if fmt == "int8" else 448.0
+    for v, codes, scales in ((x, cache.k, cache.k_scale), (-x, cache.v, cache.v_scale)):
+        f = v.float().transpose(1, 2)
+        scale = f.abs().amax(-1) * torch.tensor(1 / m, dtype=torch.float32)
+        q = f / scale[..., None]
+        want = q.round().to(torch.int8) if fmt == "int8" else q.clamp(-448, 448).to(torch.float8_e4m3fn)
+        assert torch.equal(scales.cpu(), scale)
+        assert torch.equal(codes.cpu().view(torch.int8), want.view(torch.int8))
