@@ -25,11 +25,15 @@
 // range, whatever the scales.
 //
 // The work is divided in one of two ways.  UNITS: one cluster of 1 to 8 CTAs
-// for up to 16 rows of a sequence's head, whose CTAs take a share of its positions each and are
-// joined through distributed shared memory; one launch, no scratch.  Else the
-// tiles of all units are split evenly over the CTAs, and a unit that falls
-// into several is joined by a second launch: for long caches, where units of
-// very different length would leave SMs idle.
+// for up to 16 rows of a sequence's head, whose CTAs take a share of its
+// positions each and are joined through distributed shared memory; one launch,
+// no scratch.  Else the tiles of all units are split evenly over the CTAs, and
+// a unit that falls into several is joined by a second launch: for long caches,
+// where units of very different length would leave SMs idle.
+//
+// Measured: 24 sequences of up to 65536 positions, 32 heads on 4 of 128, int8
+// 212 to 228 us (5.2 to 5.6 TB/s); one of 131071, 24 heads on 4 of 256, e4m3
+// 57 us (4.8 TB/s, the join included); 64 ragged ones of up to 2304 53 us.
 #pragma once
 
 #include "attn_common.cuh"

@@ -44,9 +44,9 @@ void plan_units(Plan& p, int64_t units, int64_t most, int64_t tiles) {
 }
 
 // Up to 16 rows per key/value head the token kernel reads the cache once at the memory's rate; its tensor-core tiles
-// and registers hold two groups of eight rows.  By units up to 8192 positions: 64 ragged sequences of 2304 take 53 us and one
-// takes 14, against 67 and 17 with the tiles split evenly and joined by a second launch.  Units of longer caches may
-// differ by more than the CTA slots even out, and few units of one need more than 8 CTAs each.
+// and registers hold two groups of eight rows.  By units up to 8192 positions: 64 ragged sequences of up to 2304 take
+// 53 us and one takes 14, against 67 and 17 with the tiles split evenly and joined by a second launch.  Units of longer
+// caches may differ by more than the CTA slots even out, and few units of one need more than 8 CTAs each.
 //
 // More rows: the row-block kernel; or, of caches up to 8192 positions, several units of 16 rows for the token kernel,
 // which read the cache again (from L2).  A tile of 64 positions takes a CTA about as long in either, 1.0 us at 128
