@@ -9,8 +9,8 @@
 // back as NaN, and attention over it gives NaN, in the rows that see it only.
 //
 // Bound: HBM bytes (input + D + 4 a vector), or the launch for one token.
-// One warp per vector: the whole vector sits in the warp's registers (D / 32
-// values a lane), so nothing is read twice; a warp takes KV_EACH vectors, all
+// Eight values a lane, a vector of 256 in a warp's registers or two of 128, so
+// nothing is read twice; a warp takes KV_EACH times as many, all
 // loaded before the first is worked on.  Measured with 8 x 1999 tokens of 4
 // heads of 256, bf16: append 33 us (98 MB, 3.0 TB/s: instructions), read 15 us
 // of e4m3 (6.5 TB/s: HBM), 18 us of int8.
@@ -29,7 +29,7 @@ using namespace gsq;
 namespace {
 
 constexpr int KV_WARPS = 4;  // per CTA
-constexpr int KV_EACH = 4;   // vectors per warp
+constexpr int KV_EACH = 4;   // vectors per lane
 
 struct KvArgs {
   const void* src[2];     // k, v (append)
@@ -53,19 +53,15 @@ __device__ __forceinline__ KvSpan kv_span(const KvArgs& a, int b) {
   return {a.start[(int64_t)b * a.start_stride], a.counts ? min(a.counts[b], a.tokens) : a.tokens};
 }
 
-// N consecutive values of T at p, as one or two vector loads where VEC (p 16-byte aligned, or 8-byte for 8 bytes).
+// N consecutive values of T at p, as one or two vector loads where VEC (p 16-byte aligned).
 template <typename T, int N, bool VEC>
 __device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
   if constexpr (VEC) {
     constexpr int B = sizeof(T) * N;
-    static_assert(B == 8 || B % 16 == 0, "whole vector loads");
+    static_assert(B % 16 == 0, "whole vector loads");
     alignas(16) T e[N];
-    if constexpr (B == 8) {
-      *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
-    } else {
 #pragma unroll
-      for (int i = 0; i < B / 16; i++) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-    }
+    for (int i = 0; i < B / 16; i++) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
 #pragma unroll
     for (int i = 0; i < N; i++) f[i] = to_f32(e[i]);
   } else {
@@ -74,14 +70,15 @@ __device__ __forceinline__ void load_n(const T* p, float (&f)[N]) {
   }
 }
 
-// Codes (one byte each, in order) and scale of the warp's vector, N values a lane.
+// Codes (one byte each, in order) and scale of the vector that the lanes of `lanes` hold, N values each.
 template <int FMT, int N>
-__device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N / 4], float& scale) {
+__device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N / 4], float& scale,
+                                         uint32_t lanes = 0xffffffffu) {
   // the largest |x| by its bits, which for Inf and NaN are above every finite number's
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; i++) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
+  top = __reduce_max_sync(lanes, top);
   const float m = __uint_as_float(top);
   constexpr float M = FMT == KV_INT8 ? 127.f : 448.f;
   scale = __fmul_rn(m, 1.f / M);
@@ -93,7 +90,7 @@ __device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N
   // 2^-60 on only concerns quotients of code 0. (A product with the reciprocal alone, rounded both ways, and a division
   // where the codes differed, took 38 us where this takes 33: 39 % of bf16 vectors hold a tie of int8, such as a value
   // half as large as the largest.)
-  if (scale >= 0x1p-60f) {  // the same for the warp
+  if (scale >= 0x1p-60f) {  // the same for the vector's lanes
     const float y = __frcp_rn(scale);
     const float high = __uint_as_float(__float_as_uint(y) - (fmaf(-scale, y, 1.f) < 0.f ? 1u : 0u));
     const float low = fmaf(-scale, high, 1.f) * y;
@@ -134,82 +131,93 @@ __device__ __forceinline__ void quantise(const float (&f)[N], uint32_t (&code)[N
   }
 }
 
-template <int N>
-__device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t (&w)[N / 4]) {
-  if constexpr (N == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(p) = w[0];
-}
+// Where a lane's vectors of D values lie: vector `first` + i * PER_WARP, token t and head h, values from `at` on.
+template <int D>
+struct KvLane {
+  static constexpr int LANES = D / 8, PER_WARP = 32 / LANES;
+  unsigned first;
+  int t, h, at;
+  uint32_t lanes;  // that share its vectors
+
+  __device__ explicit KvLane(int heads) {
+    const int lane = threadIdx.x & 31;
+    first = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * (KV_EACH * PER_WARP) + lane / LANES;
+    t = first / (unsigned)heads;
+    h = first % (unsigned)heads;
+    at = lane % LANES * 8;
+    lanes = PER_WARP == 1 ? 0xffffffffu : 0xffffu << (lane / LANES * LANES);
+  }
+  __device__ void next(int heads) {
+    h += PER_WARP;
+    while (h >= heads) h -= heads, t++;
+  }
+};
 
 template <typename T, int FMT, int D, bool VEC>
 __global__ void __launch_bounds__(32 * KV_WARPS) kv_append_kernel(const KvArgs a) {
-  constexpr int N = D / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const unsigned first = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * KV_EACH;  // token and head
-  const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
-  float f[KV_EACH][N];
+  KvLane<D> lane(a.heads);
+  const int which = blockIdx.z, b = blockIdx.y;
+  float f[KV_EACH][8];
   int64_t row[KV_EACH];  // of codes and scales, or -1
-  int t = first / (unsigned)a.heads, h = first % (unsigned)a.heads;
   const KvSpan span = kv_span(a, b);
-  const T* src = static_cast<const T*>(a.src[which]) + b * a.sb[which] + lane * N;
+  const T* src = static_cast<const T*>(a.src[which]) + b * a.sb[which] + lane.at;
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
     row[i] = -1;
-    if (t < span.count) {
-      const int64_t p = (int64_t)span.start + t;
+    if (lane.t < span.count) {
+      const int64_t p = (int64_t)span.start + lane.t;
       if (p >= 0 && p < a.cap) {
-        row[i] = ((int64_t)b * a.heads + h) * a.cap + p;
-        load_n<T, N, VEC>(src + t * a.st[which] + h * a.sh[which], f[i]);
-      } else if (lane == 0 && a.err) {
+        row[i] = ((int64_t)b * a.heads + lane.h) * a.cap + p;
+        load_n<T, 8, VEC>(src + lane.t * a.st[which] + lane.h * a.sh[which], f[i]);
+      } else if (lane.at == 0 && a.err) {
         atomicExch(a.err, DEV_CACHE_POSITION);
       }
     }
-    if (++h == a.heads) h = 0, t++;
+    lane.next(a.heads);
   }
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
     if (row[i] < 0) continue;
-    uint32_t code[N / 4];
+    uint32_t code[2];
     float scale;
-    quantise<FMT, N>(f[i], code, scale);
-    store_codes<N>(a.codes[which] + row[i] * D + lane * N, code);
-    if (lane == 0) a.scale[which][row[i]] = scale;
+    quantise<FMT, 8>(f[i], code, scale, lane.lanes);
+    *reinterpret_cast<uint2*>(a.codes[which] + row[i] * D + lane.at) = make_uint2(code[0], code[1]);
+    if (lane.at == 0) a.scale[which][row[i]] = scale;
   }
 }
 
 // Positions outside the cache, and past a sequence's count, read as zeros.
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(32 * KV_WARPS) kv_read_kernel(const KvArgs a) {
-  constexpr int N = D / 32;
   pdl_launch_dependents();
   pdl_wait();
-  const unsigned first = (blockIdx.x * KV_WARPS + (threadIdx.x >> 5)) * KV_EACH, vectors = a.tokens * a.heads;
-  const int lane = threadIdx.x & 31, which = blockIdx.z, b = blockIdx.y;
-  uint32_t c[KV_EACH][N / 4];
+  KvLane<D> lane(a.heads);
+  const unsigned vectors = a.tokens * a.heads;
+  const int which = blockIdx.z, b = blockIdx.y;
+  uint32_t c[KV_EACH][2];
   float scale[KV_EACH];
-  int t = first / (unsigned)a.heads, h = first % (unsigned)a.heads;
   const KvSpan span = kv_span(a, b);
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
     scale[i] = 0.f;
-#pragma unroll
-    for (int e = 0; e < N / 4; e++) c[i][e] = 0u;
-    const int64_t p = (int64_t)span.start + t;
-    if (t < span.count && p >= 0 && p < a.cap) {
-      const int64_t row = ((int64_t)b * a.heads + h) * a.cap + p;
+    c[i][0] = c[i][1] = 0u;
+    const int64_t p = (int64_t)span.start + lane.t;
+    if (lane.t < span.count && p >= 0 && p < a.cap) {
+      const int64_t row = ((int64_t)b * a.heads + lane.h) * a.cap + p;
       scale[i] = a.scale[which][row];
-      const uint8_t* src = a.codes[which] + row * D + lane * N;
-      if constexpr (N == 8) *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(src);
-      else c[i][0] = *reinterpret_cast<const uint32_t*>(src);
+      *reinterpret_cast<uint2*>(c[i]) = *reinterpret_cast<const uint2*>(a.codes[which] + row * D + lane.at);
     }
-    if (++h == a.heads) h = 0, t++;
+    lane.next(a.heads);
   }
 #pragma unroll
   for (int i = 0; i < KV_EACH; i++) {
-    if (first + i >= vectors) break;
-    T* dst = static_cast<T*>(a.dst[which]) + ((int64_t)b * vectors + first + i) * D + lane * N;
+    const unsigned v = lane.first + i * KvLane<D>::PER_WARP;
+    if (v >= vectors) break;
+    T* dst = static_cast<T*>(a.dst[which]) + ((int64_t)b * vectors + v) * D + lane.at;
 #pragma unroll
-    for (int e = 0; e < N / 4; e++) {
+    for (int e = 0; e < 2; e++) {
       uint32_t lo, hi;
       codes_to_half2<FMT>(c[i][e], lo, hi);
       float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo));
@@ -301,7 +309,7 @@ __global__ void __launch_bounds__(32 * KV_WARPS) qkv_append_kernel(const QkvArgs
     float scale;
     quantise<FMT, N>(f, code, scale);
     const int64_t at = ((int64_t)b * a.nkv + h) * a.cap + p;
-    store_codes<N>(a.codes[which] + at * D + lane * N, code);
+    *reinterpret_cast<uint2*>(a.codes[which] + at * D + lane * N) = make_uint2(code[0], code[1]);
     if (lane == 0) a.scale[which][at] = scale;
   } else if (lane == 0 && a.err) {
     atomicExch(a.err, DEV_CACHE_POSITION);
@@ -342,6 +350,12 @@ cudaError_t read_launch(int dtype, dim3 grid, cudaStream_t st, const KvArgs& a) 
     case DT_F16: return launch_pdl(kv_read_kernel<__half, FMT, D>, grid, block, 0, st, a);
     default: return launch_pdl(kv_read_kernel<__nv_bfloat16, FMT, D>, grid, block, 0, st, a);
   }
+}
+
+// CTAs for `vectors` vectors of keys and of values in each sequence.
+dim3 kv_grid(int64_t vectors, int64_t batch, int64_t dim) {
+  const int64_t each = KV_WARPS * KV_EACH * (256 / dim);
+  return dim3((unsigned)((vectors + each - 1) / each), (unsigned)batch, 2);
 }
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -387,7 +401,7 @@ int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_
   KvArgs a = {};
   a.src[0] = k;
   a.src[1] = v;
-  // vector loads where every vector starts on a 16-byte boundary (two-byte values of 128-wide heads: 8 bytes a lane)
+  // vector loads where every vector starts on a 16-byte boundary
   bool vec = al16(k) && al16(v);
   for (int i = 0; i < 2; i++) {
     const int64_t* s = i ? v_strides : k_strides;
@@ -408,7 +422,7 @@ int gsq_kv_append(const void* k, const void* v, int dtype, int64_t batch, int64_
   a.heads = (int)heads;
   a.cap = cap;
   a.err = device_error_word();
-  const dim3 grid((unsigned)((tokens * heads + KV_WARPS * KV_EACH - 1) / (KV_WARPS * KV_EACH)), (unsigned)batch, 2);
+  const dim3 grid = kv_grid(tokens * heads, batch, dim);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = fmt == KV_INT8 ? (dim == 256 ? append_launch<KV_INT8, 256>(dtype, vec, grid, st, a)
                                                      : append_launch<KV_INT8, 128>(dtype, vec, grid, st, a))
@@ -441,7 +455,7 @@ int gsq_kv_read(int fmt, const void* k_codes, const void* v_codes, const float* 
   a.tokens = (int)tokens;
   a.heads = (int)heads;
   a.cap = cap;
-  const dim3 grid((unsigned)((tokens * heads + KV_WARPS * KV_EACH - 1) / (KV_WARPS * KV_EACH)), (unsigned)batch, 2);
+  const dim3 grid = kv_grid(tokens * heads, batch, dim);
   cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = fmt == KV_INT8 ? (dim == 256 ? read_launch<KV_INT8, 256>(dtype, grid, st, a)
                                                      : read_launch<KV_INT8, 128>(dtype, grid, st, a))
