@@ -8,7 +8,7 @@
 // positions takes 1024 cycles), else the bytes of the cache.  Each code is
 // read, made fp16 and stored to shared memory once per row block, and that
 // is what competes with the tensor core:
-//   - Q and P are TMEM operands, so the tensor core reads only K and V from
+//   - Q and P are TMEM operands, so that the tensor core reads only K and V from
 //     shared memory: per tile 64 KB written and 64 KB read, 1024 cycles of
 //     its 128 bytes a cycle, where Q in shared memory would add 64 KB;
 //   - K and V tiles have one layout (64 x 64 blocks of 128-byte rows, 128-byte
@@ -49,7 +49,7 @@ namespace gsq {
 
 constexpr int AR_M = 128, AR_TILE = 64, AR_HALF = AR_TILE / 2;
 constexpr int AR_GROUP = 4, AR_SOFTMAX = 2 * AR_GROUP, AR_DEQUANT = 8;  // warps
-constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four one issues products, one copies
+constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four: products, copies, scales
 
 template <int D>
 struct ArGeom {

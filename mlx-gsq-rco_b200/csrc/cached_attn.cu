@@ -52,9 +52,9 @@ void plan_units(Plan& p, int64_t units, int64_t most, int64_t tiles) {
 // which read the cache again (from L2).  A tile of 64 positions takes a CTA about as long in either, 1.0 us at 128
 // dimensions and 1.7 at 256.  In these terms a wave of the token kernel's CTAs costs 5 and its tiles; the row-block
 // kernel 8, 1 for every 32 rows (queries loaded, results stored), its tiles, and the joining launch 1 for every 1200
-// rows of parts.  Measured with 4 heads of 256 (us, token kernel and row blocks): one sequence, 42 rows, 1900
-// positions 18 and 21; 128 rows, 700 positions 16 and 25; 24 rows, 8000 positions 32 and 26; 8 sequences of 2000
-// positions, 24 rows 26 and 37, 96 rows 64 and 48.  Past 256 rows the row blocks are full.
+// rows of parts.  Measured with 4 heads of 256 (us, token kernel and row blocks): one sequence, 40 rows, 2000
+// positions 18 and 20; 128 rows, 700 positions 16 and 24; 24 rows, 8000 positions 32 and 25; 8 sequences of 2000
+// positions, 24 rows 26 and 34, 96 rows 64 and 44.  Past 256 rows the row blocks are full.
 Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, int64_t cap) {
   Plan p = {};
   const int64_t rows = n * (heads / kv), cached = batch * kv;  // heads in the cache
