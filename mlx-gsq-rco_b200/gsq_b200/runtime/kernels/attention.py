@@ -92,10 +92,12 @@ def cached_attention(q: torch.Tensor, cache, start: torch.Tensor, *, counts: tor
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous() or \
             out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape, dtype and device")
-    ws = q.new_empty(need // 2).data_ptr() if need else None  # this call's alone: the stream orders its next use
+    # this call's alone, held until its launches are queued: from then on the stream orders the memory's next use
+    ws = q.new_empty(need // 2) if need else None
     _lib.launch(dev, lib.gsq_cached_attention, q.data_ptr(), *args, *cache.pointers, cache.length, start.data_ptr(),
                 stride, None if counts is None else check_counts(counts, batch, dev), tree_ptr, tree_stride, gate_ptr,
-                gate_strides, cache.dim ** -0.5 if scale is None else float(scale), out.data_ptr(), ws, need)
+                gate_strides, cache.dim ** -0.5 if scale is None else float(scale), out.data_ptr(),
+                None if ws is None else ws.data_ptr(), need)
     return out
 
 
