@@ -492,6 +492,7 @@ class Qwen35:
         self.n_pos = 0  # host copy of the position (prefill bookkeeping)
         self._graph = None
         self._logits_control: dict | None = None
+        self._prompt_history = None  # that learns the token a prompt led to, once a decode step feeds it
         inv = cfg.rope_theta ** (-torch.arange(0, cfg.rotary_dim, 2, dtype=torch.float32) / cfg.rotary_dim)
         self._inv_freq = inv.to(self.dev)
 
@@ -528,6 +529,7 @@ class Qwen35:
         self.n_pos = 0
         self.batch = 1
         self._graph = None
+        self._prompt_history = None
 
     def fork(self, batch: int) -> None:
         """Batched decode from the current state: sequences 1..batch-1 become
@@ -680,10 +682,14 @@ class Qwen35:
         """Adjusts the logits of prefill, extend and every decode step before
         the next token is taken (``adjust_logits``, same arguments): row b of
         each tensor (up to max_batch rows, on the model's device) is for
-        sequence b. A ``history`` learns the prompt and the chosen tokens
-        (tokens given to ``decode_step`` are the caller's to record); the
-        tensors may be changed in place between steps, replays of a captured
-        graph included. Without arguments: plain logits again."""
+        sequence b. A ``history`` learns the prompt as it comes, the token that
+        a prompt leads to once a decode step feeds it (after a part of a longer
+        prompt none does), and the token that a decode step chooses at once.
+        Other tokens given to ``decode_step`` are the caller's to record; a
+        caller that chooses every token by other means leaves the history out
+        here and gives it to ``adjust_logits``. The tensors may be changed in place between steps,
+        replays of a captured graph included. Without arguments: plain logits
+        again."""
         given = dict(history=history, repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
                      bias_values=bias_values, allowed=allowed)
         if history is not None and history.rows < self.max_batch:
@@ -691,14 +697,14 @@ class Qwen35:
         self._logits_control = given if any(t is not None for t in given.values()) else None
         self._graph = None
 
-    def _adjusted(self, logits: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        """(logits, next tokens) of the first sequences' rows of logits."""
+    def _adjusted(self, logits: torch.Tensor, record: bool) -> tuple[torch.Tensor, torch.Tensor]:
+        """(logits, next tokens) of the first sequences' rows of logits; with ``record`` a history learns the tokens."""
         c, rows = self._logits_control, logits.shape[0]
         if c is None:
             return logits, torch.argmax(logits, dim=-1).to(torch.int32)
         rest = {k: t if t is None or (k == "allowed" and t.dim() == 1) else t[:rows]
                 for k, t in c.items() if k != "history"}
-        return adjust_logits(logits, history=c["history"], record=c["history"] is not None, **rest)
+        return adjust_logits(logits, history=c["history"], record=record and c["history"] is not None, **rest)
 
     def _prompt(self, ids: torch.Tensor) -> torch.Tensor:
         """Runs ids through sequence 0 from the current position; returns the last token's logits."""
@@ -710,9 +716,10 @@ class Qwen35:
         delta = self._layers(x, self.n_pos)
         last = x[T - 1:].clone()
         hf = rmsnorm(last, delta[T - 1:].contiguous(), self.out_norm, self.eps)
-        if self._logits_control is not None and self._logits_control["history"] is not None:
-            record_tokens(self._logits_control["history"], ids.to(torch.int32)[None], generated=False)
-        logits, token = self._adjusted(self.lm_head(hf))
+        self._prompt_history = None if self._logits_control is None else self._logits_control["history"]
+        if self._prompt_history is not None:
+            record_tokens(self._prompt_history, ids.to(torch.int32)[None], generated=False)
+        logits, token = self._adjusted(self.lm_head(hf), record=False)
         self.cur_id[:1].copy_(token)
         self.n_pos += T
         self.pos.fill_(self.n_pos)
@@ -745,6 +752,15 @@ class Qwen35:
             raise ValueError("prompt longer than the cache")
         return self._prompt(ids)
 
+    def _record_prompts_token(self, chosen: torch.Tensor | None = None) -> None:
+        """Before the first decode step after a prompt: its history learns the token it led to (``chosen``) as output,
+        for the sequences that are fed it."""
+        if self._prompt_history is not None:
+            fed = self.cur_id[:self.batch]
+            tokens = fed if chosen is None else torch.where(fed == chosen, fed, -1)
+            record_tokens(self._prompt_history, tokens[:, None])
+            self._prompt_history = None
+
     def _decode_body(self) -> torch.Tensor:
         cfg, B = self.cfg, self.batch
         ids = self.cur_id[:B]
@@ -753,7 +769,7 @@ class Qwen35:
         x = x.reshape(B, cfg.hidden_size)
         delta = self._layers(x, None)
         hf = rmsnorm(x, delta, self.out_norm, self.eps)
-        logits, tokens = self._adjusted(self.lm_head(hf))
+        logits, tokens = self._adjusted(self.lm_head(hf), record=True)
         ids.copy_(tokens)
         self.pos.add_(1)
         return logits
@@ -765,7 +781,10 @@ class Qwen35:
         (batch x vocab, fp32)."""
         if self.n_pos >= self.max_len:
             raise ValueError("cache full")
+        chosen = None
         if token is not None:
+            if self._prompt_history is not None:
+                chosen = self.cur_id[:self.batch].clone()
             if isinstance(token, int):
                 self.cur_id[:self.batch].fill_(int(token))
             else:
@@ -773,6 +792,7 @@ class Qwen35:
                 if t.numel() != self.batch:
                     raise ValueError(f"expected {self.batch} tokens")
                 self.cur_id[:self.batch].copy_(t.to(self.dev))
+        self._record_prompts_token(chosen)
         logits = self._decode_body()
         self.n_pos += 1
         return logits
@@ -807,6 +827,8 @@ class Qwen35:
             raise RuntimeError("capture_decode() first")
         if self.n_pos + n > self.max_len:
             raise ValueError("cache full")
+        if n > 0:
+            self._record_prompts_token()
         for _ in range(n):
             self._graph.replay()
         self.n_pos += n
