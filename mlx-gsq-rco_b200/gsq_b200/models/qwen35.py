@@ -51,6 +51,8 @@ from ..runtime.kernels import adjust_logits, cached_attention, packed_embedding,
 from ..runtime.kvcache import QuantizedKVCache
 from ..runtime.store import PackedWeight
 
+_CACHE_TOKENS = 65535  # of one gsq_qkv_append
+
 
 @dataclass(frozen=True)
 class Qwen35Config:
@@ -708,21 +710,24 @@ class Qwen35:
 
     def _prompt(self, ids: torch.Tensor) -> torch.Tensor:
         """Runs ids through sequence 0 from the current position; returns the last token's logits."""
-        cfg, T = self.cfg, ids.numel()
+        cfg = self.cfg
         ids = ids.reshape(-1).to(self.dev)
-        x = packed_embedding(ids, self.embed.data, qtype=self.embed.quantization_type,
-                             vocab_size=cfg.vocab_size, dimensions=cfg.hidden_size, dtype=torch.float32)
-        x = x.reshape(T, cfg.hidden_size).contiguous()
-        delta = self._layers(x, self.n_pos)
-        last = x[T - 1:].clone()
-        hf = rmsnorm(last, delta[T - 1:].contiguous(), self.out_norm, self.eps)
+        # an 8-bit cache is written by calls of so many tokens at most; the fp32 one is attended from position 0 only
+        parts = ids.split(_CACHE_TOKENS) if any("kv" in L for L in self.layers) else (ids,)
+        for part in parts:
+            T = part.numel()
+            x = packed_embedding(part, self.embed.data, qtype=self.embed.quantization_type,
+                                 vocab_size=cfg.vocab_size, dimensions=cfg.hidden_size, dtype=torch.float32)
+            x = x.reshape(T, cfg.hidden_size).contiguous()
+            delta = self._layers(x, self.n_pos)
+            self.n_pos += T
+            self.pos.fill_(self.n_pos)
+        hf = rmsnorm(x[T - 1:].clone(), delta[T - 1:].contiguous(), self.out_norm, self.eps)
         self._prompt_history = None if self._logits_control is None else self._logits_control["history"]
         if self._prompt_history is not None:
             record_tokens(self._prompt_history, ids.to(torch.int32)[None], generated=False)
         logits, token = self._adjusted(self.lm_head(hf), record=False)
         self.cur_id[:1].copy_(token)
-        self.n_pos += T
-        self.pos.fill_(self.n_pos)
         return logits[0]
 
     def prefill(self, ids: torch.Tensor) -> torch.Tensor:
