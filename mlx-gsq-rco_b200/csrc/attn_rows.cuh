@@ -303,9 +303,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
     do {
       const int r = run.at.mb * AR_M + row;  // row of the unit's head
       const int i = r / a.group;
-      // Q: the row in fp16, 16 dimensions in 8 columns; a half of it by each group. bf16: times a power of two that
-      // fits the largest of the warp's rows, so that one factor serves them all (what a row 2^27 times smaller loses
-      // is far below the rounding of its neighbours' scores, and its own are as much smaller). Padding counts as 0.
+      // Q: the row in fp16, 16 dimensions in 8 columns; a half of it by each group. bf16: times a power of two of the
+      // row's own (q_shift), whose inverse its thread multiplies the scores with. Padding counts as 0.
       const int r_load = i < run.at.span.count ? r : rows;
       int shift = 0;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -317,8 +316,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
 #pragma unroll
           for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(f[e]));
         }
-        amax = amax <= 3.4e38f ? amax : 0.f;  // a row with an infinity is lost by itself
-        shift = q_shift(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax))));
+        shift = q_shift(amax);
       }
       const float up = (a.scale < 0.f ? -1.f : 1.f) * exp2_int(shift);
       const float factor = fabsf(a.scale) * 1.4426950408889634f * exp2_int(-shift);  // fp16: with the keys' scales
