@@ -186,7 +186,8 @@ GSQ_API int gsq_qkv_append(const float* qkv, int64_t qkv_stride, int64_t batch, 
  * and those new tokens p = start + j, j < counts[b], whose bit j is set in
  * row i of the tree (int32 words [n, ceil(n / 32)] of sequence b at
  * tree + b * tree_stride, bit j % 32 of word j / 32; n <= 1024; stride 0: one
- * tree for all).  A row that sees nothing, and padding, gives zeros.
+ * tree for all).  A row that sees nothing, and padding, gives zeros.  Scales
+ * may have any size; only value scales above 2^57 ask for scores below 2^17.
  *   q     [batch, n, heads, dim] fp16 or bf16, strides in elements of the
  *         first three dimensions; rows 16-byte aligned
  *   gate  fp32 of the same shape with strides of its own, or NULL

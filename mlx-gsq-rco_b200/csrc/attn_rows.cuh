@@ -17,7 +17,10 @@
 //   - scales stay out of the codes: a position's key scale multiplies its
 //     score, and its value scale enters the weight as 2^(s + log2 vs - ref),
 //     with one exponential; the sum of weights takes the same value times
-//     1 / vs.
+//     1 / vs. From a tile with a scale outside 2^-40 .. 2^40 on, where that
+//     value may leave fp32's range, the run's sums come from the scores a
+//     second time, with exponentials of their own (the code for it costs the
+//     chunk below 1 %, in registers).
 // Roles (20 warps): two softmax warpgroups, one row a thread, that take the
 // two halves of every tile's columns; two that dequantise; one warp issues the
 // products, one thread the bulk copies of codes (a tile is one contiguous
@@ -48,6 +51,7 @@
 namespace gsq {
 
 constexpr int AR_M = 128, AR_TILE = 64, AR_HALF = AR_TILE / 2;
+constexpr int AR_SCALES = 3 * AR_HALF + 4;  // floats of half a tile's scales
 constexpr int AR_GROUP = 4, AR_SOFTMAX = 2 * AR_GROUP, AR_DEQUANT = 8;  // warps
 constexpr int AR_THREADS = 32 * (AR_SOFTMAX + AR_DEQUANT + 4);  // of the last four: products, copies, scales
 
@@ -57,8 +61,8 @@ struct ArGeom {
   static constexpr int STAGES = D == 256 ? 5 : 6;
   static constexpr int RAW = AR_TILE * D;       // its codes
   static constexpr int RAWS = 3;
-  static constexpr int SCALES = 2 * (6 * AR_HALF + 4) * 4;  // of two tiles, with a mask for each half
-  static constexpr int STATE = 6 * AR_M * 4;    // the two groups' maxima of two tiles, and their sums
+  static constexpr int SCALES = 4 * AR_SCALES * 4;  // of two tiles
+  static constexpr int STATE = 10 * AR_M * 4;    // the two groups' maxima of two tiles, their sums and what these are relative to
   static constexpr int SMEM = 1024 + STAGES * ITEM + RAWS * RAW + SCALES + STATE + 512;
   static constexpr int O = 0, Q = D, S = Q + D / 2;  // TMEM columns; S: two tiles
   static constexpr int COLS = 512;
@@ -207,27 +211,50 @@ __device__ __forceinline__ uint64_t ar_visible(const AttnArgs& a, int b, const S
   return m & below(s.len - p0);
 }
 
-// Scales of 32 positions, one a lane, as the softmax uses them: the key's times `factor`, log2 of the value's and its
-// inverse in linear terms, in 96 floats at `out`. Returns the positions (bits) whose value scale is 0.
-__device__ __forceinline__ uint32_t ar_scales(float k, float v, float factor, float* out) {
-  const int lane = threadIdx.x & 31;
-  // log2 of the values' scales, not below -100 (what is smaller vanishes beside any output). A vector of scale 0 has
-  // no part in the output, but in the sum of weights: it is weighted with the largest scale beside it, and that weight
-  // left out of P. NaN stays, with 1 / vs as 0, so that a row that does not see the position takes no harm.
-  float lv = v > 0.f ? fmaxf(log2_approx(v), -100.f) : -INFINITY;
-  const uint32_t zeros = __ballot_sync(0xffffffffu, v == 0.f);
-  if (zeros) {
-    float top = lv;
+// Whether a value scale is outside 2^-40 .. 2^40 (0 is not). Within, one reference serves both sums: a weight relative to
+// the largest of the scaled ones is within 2^80 of its size relative to the largest weight, so that those of 2^-32 and
+// more, which count in the sum, are 2^-112 and more, within fp32's range.
+__device__ __forceinline__ bool far_scale(float v) { return v > 0.f && (v < 0x1p-40f || v > 0x1p40f); }
+
+// Scales of a tile's positions p and p + 32, one a lane, as the softmax uses them: the key's times a factor, log2 of the
+// value's and its inverse in linear terms (not used where `wide`), and which of a half's value scales are 0 (bits).
+struct ArScales {
+  float key[2], log[2], inverse[2];
+  uint32_t zeros[2];
+
+  __device__ __forceinline__ void set(const float (&k)[2], const float (&v)[2], float factor, bool wide) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (v == 0.f) lv = top == -INFINITY ? -40.f : top;
+    for (int h = 0; h < 2; h++) {
+      // A vector of scale 0 has no part in the output, but in the sum of weights: where that is taken from the scaled
+      // weights it is weighted with the largest scale beside it, and that weight left out of P. NaN stays, with 1 / vs as
+      // 0, so that a row that does not see the position takes no harm.
+      float lv = v[h] > 0.f ? log2_approx(v[h]) : -INFINITY;
+      zeros[h] = __ballot_sync(0xffffffffu, v[h] == 0.f);
+      if (zeros[h] && !wide) {
+        float top = lv;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (v[h] == 0.f) lv = top == -INFINITY ? -40.f : top;
+      }
+      const bool nan = isnan(v[h]);
+      key[h] = k[h] * factor;
+      log[h] = nan ? v[h] : lv;
+      inverse[h] = nan ? 0.f : exp2_approx(-lv);
+    }
   }
-  const bool nan = isnan(v);
-  out[lane] = k * factor;
-  out[AR_HALF + lane] = nan ? v : lv;
-  out[2 * AR_HALF + lane] = nan ? 0.f : exp2_approx(-lv);
-  return zeros;
-}
+  // For each half 96 floats, its zeros and the flag.
+  __device__ __forceinline__ void store(float* out, bool wide) const {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float* to = out + h * AR_SCALES;
+      to[lane] = key[h];
+      to[AR_HALF + lane] = log[h];
+      to[2 * AR_HALF + lane] = inverse[h];
+      if (lane == 0) *reinterpret_cast<uint2*>(to + 3 * AR_HALF) = make_uint2(zeros[h], wide);
+    }
+  }
+};
 
 template <typename T, int FMT, int D>
 __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs a) {
@@ -235,10 +262,11 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);  // (an offset: the pointer stays a shared one)
   uint8_t* raw = smem + G::STAGES * G::ITEM;
-  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [tile & 1][half][ks | log2 vs | 1 / vs][32], masks
+  float* scales = reinterpret_cast<float*>(raw + G::RAWS * G::RAW);  // [tile & 1][half][ks | log2 vs | 1 / vs | zeros, wide]
   float* tops = scales + G::SCALES / 4;   // [tile & 1][group][128]: largest scores, to base 2
   float* sums = tops + 4 * AR_M;          // [group][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sums + 2 * AR_M);
+  float2* mores = reinterpret_cast<float2*>(sums + 2 * AR_M);  // [group][128]: the sum is relative to 2^(x + y)
+  uint64_t* bars = reinterpret_cast<uint64_t*>(mores + 2 * AR_M);
   uint64_t* full = bars;                  // [STAGES] count AR_DEQUANT
   uint64_t* empty = full + G::STAGES;     // [STAGES] commit
   uint64_t* s_full = empty + G::STAGES;   // [tile & 1] commit, and the tile's scales
@@ -344,14 +372,22 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       const int run0 = tile;  // the run's first tile
 
       float ref = -INFINITY, sum = 0.f;  // of the row; the sum of this group's half
+      bool wide = false;  // the run has met a scale outside 2^-40 .. 2^40: the sum is relative to its `mores`, else to 2^ref
       for (; tile < run0 + run.len; tile++) {
         const int p0 = (run.at.tile + tile - run0) * AR_TILE + group * AR_HALF;
         ok = warp_wait(&s_full[tile & 1], (uint32_t)((tile / 2) & 1), a.err);
         if (!ok) break;
         tc_fence_after();
-        const float* ks = scales + (tile & 1) * (6 * AR_HALF + 4) + group * 3 * AR_HALF;
-        const uint32_t zeros = reinterpret_cast<const uint32_t*>(scales)[(tile & 1) * (6 * AR_HALF + 4) + 6 * AR_HALF + group];
+        const float* ks = scales + ((tile & 1) * 2 + group) * AR_SCALES;
         const uint32_t scores = lanes + G::S + (tile & 1) * AR_TILE + group * AR_HALF;
+        // The run's first tile with a scale outside 2^-40 .. 2^40: from here on the sum follows the largest weight. (Both
+        // groups have met in this tile, so the other one has read the `mores` of the run before.)
+        auto turn = [&]() {
+          if (!wide && reinterpret_cast<const uint32_t*>(ks)[3 * AR_HALF + 1]) {
+            wide = true;
+            mores[group * AR_M + row] = ref == -INFINITY ? make_float2(0.f, -INFINITY) : make_float2(ref, 0.f);
+          }
+        };
         uint32_t s[AR_HALF];
         tmem_ld32(scores, s);
         tmem_wait_ld();
@@ -395,7 +431,8 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
         if (__any_sync(0xffffffffu, grow)) {
           const float next = grow ? top : ref;
           const float f = ref == next || ref == -INFINITY ? 1.f : exp2_approx(ref - next);  // no weight yet: 0, or NaN
-          sum *= f;
+          turn();
+          if (!wide) sum *= f;
           if (tile > run0) {
             // O holds this unit's tiles so far: wait for the last of them and rescale it, each group half its columns
             ok = warp_wait(&pv_done[(tile - 1) & 1], (uint32_t)(((tile - 1) / 2) & 1), a.err);
@@ -433,11 +470,44 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           w[e + 1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
         const float2 added = halves(add2(acc0, acc1));
+        const float before = sum;
         sum += added.x + added.y;
-        if (zeros) {
+        const uint2 rare = *reinterpret_cast<const uint2*>(ks + 3 * AR_HALF);  // positions of scale 0; far scales
+        if (rare.x | rare.y) {  // the same for all threads
 #pragma unroll
           for (int e = 0; e < AR_HALF / 2; e++)
-            w[e] &= (zeros >> 2 * e & 1 ? 0u : 0xffffu) | (zeros >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
+            w[e] &= (rare.x >> 2 * e & 1 ? 0u : 0xffffu) | (rare.x >> (2 * e + 1) & 1 ? 0u : 0xffff0000u);
+          turn();
+          if (wide) {
+            // the sum by itself, from the scores again: weights without their values' scales
+            const uint32_t see = (uint32_t)ar_visible(a, run.at.b, run.at.span, i, p0);
+            const float from = ref == -INFINITY ? 0.f : ref;
+            float2* more = mores + group * AR_M + row;
+            float at = more->y + (more->x - from);
+            sum = before;
+#pragma unroll 1
+            for (int c = 0; c < AR_HALF; c += 16) {
+              uint32_t z[16];
+              tmem_ld16(scores + c, z);
+              float next = at;
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                float y = __uint_as_float(z[e]);
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) y *= factor;
+                const float lv = ks[AR_HALF + c + e];  // t + lift as above, less lv; of scale 0 without it
+                y = lv == -INFINITY ? y * ks[c + e] + lift : fmaf(y, ks[c + e], lv) + lift - lv;
+                y = see >> (c + e) & 1 ? y : -INFINITY;
+                next = fmaxf(next, y);
+                z[e] = __float_as_uint(y);
+              }
+              if (at != next && at != -INFINITY) sum *= exp2_approx(at - next);
+              at = next;
+              const float base = at == -INFINITY ? 0.f : at;
+#pragma unroll
+              for (int e = 0; e < 16; e++) sum += exp2_approx(__uint_as_float(z[e]) - base);
+            }
+            *more = make_float2(from, at);
+          }
         }
         tmem_st16(scores, w);  // over the first half of the scores that they come from
         tmem_wait_st();
@@ -456,11 +526,23 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
            warp_wait(&pv_done[end & 1], (uint32_t)((end / 2) & 1), a.err);
       if (!ok) break;
       sum = sums[row] + sums[AR_M + row];
+      float more = 0.f;
+      if (wide) {  // relative to the same ref by now
+        const float2 m0 = mores[row], m1 = mores[AR_M + row];
+        more = fmaxf(m0.y, m1.y);
+        if (more == -INFINITY) {  // nothing seen
+          more = 0.f;
+        } else {
+          sum = shrunk(sums[row], m0.y - more) + shrunk(sums[AR_M + row], m1.y - more);
+          ref = m0.x + more;
+        }
+      }
       tc_fence_after();
       const int slot = 2 * blockIdx.x + (run.t == first ? 0 : 1);
       const bool live = r < rows;
       const bool none = sum == 0.f || i >= run.at.span.count;
-      const float inv = none ? 0.f : 1.f / sum;
+      // (root to be multiplied with twice: its square may be outside of fp32's range)
+      const float inv = none ? 0.f : 1.f / sum, root = exp2_approx(-0.5f * more);
       float* part = a.part + ((int64_t)slot * AR_M + row) * D;
 #pragma unroll 1
       for (int c = group * (D / 2); c < (group + 1) * (D / 2); c += 32) {
@@ -473,13 +555,15 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           for (int e = 0; e < 32; e += 8) {
             float f[8];
 #pragma unroll
-            for (int x = 0; x < 8; x++) f[x] = none ? 0.f : __uint_as_float(o[e + x]) * inv;
+            for (int x = 0; x < 8; x++) f[x] = none ? 0.f : __uint_as_float(o[e + x]) * inv * root * root;
             store_row8<T>(a, run.at.b, run.at.kh, r, c + e, f);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<uint4*>(part + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            *reinterpret_cast<float4*>(part + c + e) =
+                make_float4(__uint_as_float(o[e]) * root * root, __uint_as_float(o[e + 1]) * root * root,
+                            __uint_as_float(o[e + 2]) * root * root, __uint_as_float(o[e + 3]) * root * root);
         }
       }
       if (live && !run.whole && group == 0)
@@ -626,6 +710,7 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
           std::is_same<T, __half>::value ? fabsf(a.scale) * 1.4426950408889634f : 1.f;  // bf16: a row's own, later
       float k[2], v[2];
       int j = 0;
+      bool wide = false;  // the run has met a scale outside 2^-40 .. 2^40
       auto load = [&]() {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -638,20 +723,19 @@ __global__ void __launch_bounds__(AR_THREADS, 1) attn_rows_kernel(const AttnArgs
       };
       load();
       for (int t = 0; t < last - first; t++) {
+        wide = wide || __any_sync(0xffffffffu, far_scale(v[0]) || far_scale(v[1]));
+        ArScales made;  // before the wait: what follows it is on the softmax's path
+        made.set(k, v, factor, wide);
         if (t >= 2) {  // the softmax is through with tile t - 2
           ok = warp_wait(&pv_done[t & 1], (uint32_t)((t / 2 - 1) & 1), a.err);
           if (!ok) break;
         }
-        float* out = scales + (t & 1) * (6 * AR_HALF + 4);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const uint32_t zeros = ar_scales(k[h], v[h], factor, out + h * 3 * AR_HALF);
-          if (lane == 0) reinterpret_cast<uint32_t*>(out)[6 * AR_HALF + h] = zeros;
-        }
+        made.store(scales + (t & 1) * 2 * AR_SCALES, wide);
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_full[t & 1]);
         if (++j == run.len) {
           j = 0;
+          wide = false;
           if (!run.next(a)) break;
         }
         load();

@@ -22,7 +22,14 @@
 // of weights is of the unrounded ones, in fp32.  The values' scales differ by
 // position, so the rounded weight is 2^15 p vs / 2^ref with a reference per
 // row that follows s + log2(vs): no weight that matters leaves fp16's normal
-// range, whatever the scales.
+// range, whatever the scales.  The sum of weights is relative to 2^(ref + 36):
+// where ref comes from a scale up to 2^57, the weights that count in it, 2^-32
+// of the largest and more, are then 2^-126 and more; and where scores that do
+// not move ref have scales down to 2^-143 (below, a value is 0 in 16 bits), at
+// most 2^107 each.  Where a tile with a larger scale moves ref, the warp's sums
+// have references of their own from there on, in each thread (no exchanges);
+// their distance from ref is then that of two scores, which fp32 tells to 2^-7
+// for scores up to 2^17.
 //
 // The work is divided in one of two ways.  UNITS: one cluster of 1 to 8 CTAs
 // for up to 16 rows of a sequence's head, whose CTAs take a share of its
@@ -42,6 +49,10 @@ namespace gsq {
 
 constexpr int AT_WARPS = 4;  // of a CTA, two CTAs on an SM: one is read for while the other joins its warps
 constexpr int AT_TILE = 16 * AT_WARPS;
+// log2 of what the sums of weights are relative to, over what the sums of values are (but for 2^15); what brings these to
+// those; the scales that this does not serve
+constexpr float AT_GAP = 36.f, AT_OVER = 0x1p-51f, AT_HUGE = 0x1p57f;
+constexpr float AT_LOWEST = -3.402823466e38f;  // m of a row that has seen nothing
 
 template <int D, int NT>
 struct AtGeom {
@@ -112,11 +123,22 @@ __device__ __forceinline__ int q_shift(float amax) {
 }
 __device__ __forceinline__ float exp2_int(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
+// x 2^d, d <= 0, where 2^d may be below fp32's range and the product not.
+__device__ __forceinline__ float shrunk(float x, float d) {
+  const float r = exp2_approx(0.5f * d);
+  return x * r * r;
+}
+// Adds the weights of two scores to (at, sum).
+__device__ __forceinline__ void add_weights(float& at, float& sum, float s0, float s1) {
+  const float next = fmaxf(at, fmaxf(s0, s1));
+  sum = shrunk(sum, at - next) + exp2_approx(s0 - next) + exp2_approx(s1 - next);
+  at = next;
+}
 // Adds another part's (reference, sum) to (top, sum). No position seen: reference -inf, sum 0 (or NaN).
 __device__ __forceinline__ void add_stat(float& top, float& sum, float t2, float s2) {
   const float next = fmaxf(top, t2);
-  sum = (top == next || top == -INFINITY ? sum : sum * exp2_approx(top - next)) +
-        (t2 == next || t2 == -INFINITY ? s2 : s2 * exp2_approx(t2 - next));
+  sum = (top == next || top == -INFINITY ? sum : shrunk(sum, top - next)) +
+        (t2 == next || t2 == -INFINITY ? s2 : shrunk(s2, t2 - next));
   top = next;
 }
 // What a part's sums are multiplied with: to the common reference, 1 where it has seen nothing (its sums are 0, or NaN).
@@ -225,7 +247,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
   uint32_t qr[NT == 1 ? MT : 1][2];
   float factor[NT][2];  // of the scores of rows 8x + 2t, 8x + 2t + 1, to base 2
   int lim[NT][2];       // tree: prefix ends; causal: positions the row sees (relative to the prefix end)
-  float o[MT][NT][4], m[NT][2], l[NT][2];
+  float o[MT][NT][4], m[NT][2], l[NT][2];  // o relative to 2^(m - AT_GAP - 15), l to 2^m
+  float at[NT][2], own[NT][2];  // a thread's own reference and sum of weights
   uint4 raw[NT][2 * CH];  // q of the coming unit: row 8x + g, dimensions 64c + 16t ..
   auto fetch_q = [&]() {
 #pragma unroll
@@ -243,6 +266,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
     const bool whole = UNITS ? a.cluster == 1 : use.tile == 0 && tile + use.tiles <= last;
     const int slot = 2 * blockIdx.x + (tile == first ? 0 : 1);
     const int end = min(last, tile + use.tiles - use.tile);
+    bool wide = false;  // m may come from a scale above AT_HUGE: at and own instead of m and l
 #pragma unroll
     for (int x = 0; x < NT; x++) {
       float amax = 0.f;
@@ -284,7 +308,7 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
         const int r = 8 * x + 2 * t + c;  // this lane's columns of the score tile; their shift is held by lanes 4r'
         factor[x][c] = a.scale * 1.4426950408889634f * exp2_int(-__shfl_sync(0xffffffffu, shift, 4 * (2 * t + c)));
         lim[x][c] = (r0 + r) / a.group;
-        m[x][c] = -INFINITY;
+        m[x][c] = AT_LOWEST;
         l[x][c] = 0.f;
       }
     }
@@ -338,8 +362,11 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
       }
       // scores to base 2; s[x][e]: position p0 + g + 8 (e / 2), row 8x + 2t + e % 2
       const float ks0 = sc[g], ks1 = sc[g + 8];
-      const float lv0 = log2_approx(fmaxf(sc[16 + g], 1.4e-45f)) , lv1 = log2_approx(fmaxf(sc[24 + g], 1.4e-45f));
-      const float nan0 = sc[16 + g] - sc[16 + g], nan1 = sc[24 + g] - sc[24 + g];  // NaN scales stay NaN past fmaxf
+      // (of scale 0, whose vector has a part in the sum of weights only, as 2^-100: that sum stays finite)
+      const float lv0 = log2_approx(sc[16 + g] > 0.f ? sc[16 + g] : 0x1p-100f);
+      const float lv1 = log2_approx(sc[24 + g] > 0.f ? sc[24 + g] : 0x1p-100f);
+      const float nan0 = sc[16 + g] - sc[16 + g], nan1 = sc[24 + g] - sc[24 + g];  // NaN where the scale is
+      const float lr0 = lv0 + AT_GAP, lr1 = lv1 + AT_GAP, lift0 = 15.f + nan0, lift1 = 15.f + nan1;
       const bool edge = p0 + 16 > span.base || p0 + 16 > span.len;  // warp-uniform: some row may not see all of these
       uint32_t pb[NT][2];
 #pragma unroll
@@ -362,24 +389,43 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
             if (!see) s[x][e] = -INFINITY;
           }
         }
-        float lo[2];
-        // the reference of each row: the largest of s + log2(vs) (and s - 100, so that the sum of weights stays finite)
+        // the row's reference: the largest of u = s + log2(vs) + AT_GAP, rounded up to a whole number (it moves less often).
+        // Both weights come from u - m, so that they fit each other where s is so large that u has lost what was added.
+        float lo[2], u[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) u[e] = s[x][e] + (e < 2 ? lr0 : lr1);
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-          float r = fmaxf(fmaxf(s[x][c] + fmaxf(lv0, -100.f), s[x][2 + c] + fmaxf(lv1, -100.f)), m[x][c]);
+          float r = fmaxf(fmaxf(u[c], u[2 + c]), m[x][c]);
           r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 4));
           r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 8));
           r = fmaxf(r, __shfl_xor_sync(0xffffffffu, r, 16));
           lo[c] = r;
         }
-        const bool grew = lo[0] > m[x][0] || lo[1] > m[x][1];
+        const bool grew = lo[0] > m[x][0] || lo[1] > m[x][1] || wide;
         if (__any_sync(0xffffffffu, grew)) {
-          const float f0 = m[x][0] == -INFINITY ? 0.f : exp2_approx(m[x][0] - lo[0]);
-          const float f1 = m[x][1] == -INFINITY ? 0.f : exp2_approx(m[x][1] - lo[1]);
+          if (!wide && __any_sync(0xffffffffu, fmaxf(sc[16 + g], sc[24 + g]) > AT_HUGE)) {
+            wide = true;
+#pragma unroll
+            for (int y = 0; y < NT; y++)
+#pragma unroll
+              for (int c = 0; c < 2; c++) {
+                at[y][c] = m[y][c];
+                own[y][c] = l[y][c];
+              }
+          }
+          if (wide) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) add_weights(at[x][c], own[x][c], s[x][c], s[x][2 + c]);
+          }
+          lo[0] = ceilf(lo[0]);
+          lo[1] = ceilf(lo[1]);
+          const float r0 = exp2_approx(0.5f * (m[x][0] - lo[0])), f0 = r0 * r0;
+          const float r1 = exp2_approx(0.5f * (m[x][1] - lo[1])), f1 = r1 * r1;
+          l[x][0] = l[x][0] * r0 * r0;  // (f0 may be below fp32's range where this is not)
+          l[x][1] = l[x][1] * r1 * r1;
           m[x][0] = lo[0];
           m[x][1] = lo[1];
-          l[x][0] *= f0;
-          l[x][1] *= f1;
 #pragma unroll
           for (int j = 0; j < MT; j++) {
             o[j][x][0] *= f0;
@@ -391,10 +437,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float ref = m[x][e & 1] == -INFINITY ? 0.f : m[x][e & 1];
-          const float d = s[x][e] - ref;  // -inf where hidden
-          l[x][e & 1] += exp2_approx(d);
-          w[e] = s[x][e] == -INFINITY ? 0.f : exp2_approx(d + (e < 2 ? lv0 : lv1) + 15.f) + (e < 2 ? nan0 : nan1);
+          const float d = u[e] - m[x][e & 1];  // -inf where hidden
+          l[x][e & 1] += exp2_approx(d - (e < 2 ? lr0 : lr1));
+          w[e] = s[x][e] == -INFINITY ? 0.f : exp2_approx(d + (e < 2 ? lift0 : lift1));
         }
         const __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
         pb[x][0] = transpose8x8(*reinterpret_cast<const uint32_t*>(&h0));
@@ -448,6 +493,24 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
     for (int x = 0; x < NT; x++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
+        if (wide) {
+          // both sums relative to 2^row, the largest of the lanes' references, or where values are large to 2^(row + 80): fp32
+          // has a place for them there
+          float row = at[x][c];
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) row = fmaxf(row, __shfl_xor_sync(0xffffffffu, row, i));
+          const bool large = m[x][c] > row;
+          l[x][c] = shrunk(own[x][c], at[x][c] - row) * (large ? 0x1p-80f : 1.f);
+          row += large ? 80.f : 0.f;
+          const float r = exp2_approx(0.5f * (m[x][c] - row));  // (1 where both are AT_LOWEST, and o is 0)
+#pragma unroll
+          for (int j = 0; j < MT; j++) {
+            o[j][x][c] = o[j][x][c] * r * r;
+            o[j][x][c + 2] = o[j][x][c + 2] * r * r;
+          }
+          if (m[x][c] != AT_LOWEST) m[x][c] = row;
+        }
+        if (m[x][c] == AT_LOWEST) m[x][c] = -INFINITY;
 #pragma unroll
         for (int i = 4; i < 32; i <<= 1) l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], i);
         if (g == 0)
@@ -489,10 +552,10 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
 #pragma unroll
         for (int w = 0; w < AT_WARPS; w++) {
           const float2 s = *reinterpret_cast<const float2*>(stat + (w * G::ROWS + r) * 2);
-          sum += s.x == -INFINITY ? s.y : s.y * exp2_approx(s.x - top);
+          sum += s.x == -INFINITY ? s.y : shrunk(s.y, s.x - top);
         }
         const bool none = sum == 0.f || (r0 + r) / a.group >= span.count;
-        const float inv = none ? 0.f : 0x1p-15f / sum;
+        const float inv = none ? 0.f : 1.f / sum;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
           const int piece = warp + i * AT_WARPS, h = piece / 8;  // dimensions 16 piece ..
@@ -508,13 +571,13 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           if (whole) {
             const float f0 = a.gate ? inv * sigmoid(gate[x][c][i].x) : inv;
             const float f1 = a.gate ? inv * sigmoid(gate[x][c][i].y) : inv;
-            store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : v0 * f0, none ? 0.f : v1 * f1);
+            store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : v0 * AT_OVER * f0, none ? 0.f : v1 * AT_OVER * f1);
           } else if constexpr (UNITS) {
             *reinterpret_cast<float2*>(result(x) + (2 * tt + c) * D + d) = make_float2(v0, v1);
             if (piece == 0 && jj == 0) *reinterpret_cast<float2*>(unit_stat + r * 2) = make_float2(top, sum);
           } else {
             *reinterpret_cast<float2*>(a.part + ((int64_t)slot * G::ROWS + r) * D + d) =
-                make_float2(v0 * 0x1p-15f, v1 * 0x1p-15f);
+                make_float2(v0 * AT_OVER, v1 * AT_OVER);
             if (piece == 0 && jj == 0)
               *reinterpret_cast<float2*>(a.stat + ((int64_t)slot * G::ROWS + r) * 2) = make_float2(top, sum);
           }
@@ -548,9 +611,9 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
           y = fmaf(v[k].y, f, y);
         }
         const bool none = sum == 0.f || (r0 + r) / a.group >= span.count;
-        const float inv = none ? 0.f : 0x1p-15f / sum;
+        const float inv = none ? 0.f : 1.f / sum;
         const float f0 = a.gate ? inv * sigmoid(gate2.x) : inv, f1 = a.gate ? inv * sigmoid(gate2.y) : inv;
-        store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : x * f0, none ? 0.f : y * f1);
+        store_row2<T>(a, b, kh, r0 + r, d, none ? 0.f : x * AT_OVER * f0, none ? 0.f : y * AT_OVER * f1);
       }
       cluster_sync_all();  // no CTA leaves while another may read its shared memory
       return;
