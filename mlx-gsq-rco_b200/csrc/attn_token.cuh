@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
             if (!see) s[x][e] = -INFINITY;
           }
         }
-        // the row's reference: the largest of u = s + log2(vs) + AT_GAP, rounded up to a whole number (it moves less often).
+        // the row's reference: the largest of u = s + log2(vs) + AT_GAP (itself, so that the largest weight, 2^15, needs no
+        // rounding to fp16: rounded up to a whole number it moves less often, but the error of the outputs grows by a third).
         // Both weights come from u - m, so that they fit each other where s is so large that u has lost what was added.
         float lo[2], u[4];
 #pragma unroll
@@ -418,8 +419,6 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
 #pragma unroll
             for (int c = 0; c < 2; c++) add_weights(at[x][c], own[x][c], s[x][c], s[x][2 + c]);
           }
-          lo[0] = ceilf(lo[0]);
-          lo[1] = ceilf(lo[1]);
           const float r0 = exp2_approx(0.5f * (m[x][0] - lo[0])), f0 = r0 * r0;
           const float r1 = exp2_approx(0.5f * (m[x][1] - lo[1])), f1 = r1 * r1;
           l[x][0] = l[x][0] * r0 * r0;  // (f0 may be below fp32's range where this is not)
