@@ -19,8 +19,8 @@
 //     with one exponential; the sum of weights takes the same value times
 //     1 / vs. From a tile with a scale outside 2^-40 .. 2^40 on, where that
 //     value may leave fp32's range, the run's sums come from the scores a
-//     second time, with exponentials of their own (the code for it costs the
-//     chunk below 1 %, in registers).
+//     second time, with exponentials of their own (that code costs the chunk
+//     below 1.3 % of its time, in registers).
 // Roles (20 warps): two softmax warpgroups, one row a thread, that take the
 // two halves of every tile's columns; two that dequantise; one warp issues the
 // products, one thread the bulk copies of codes (a tile is one contiguous
@@ -33,12 +33,12 @@
 // instruction caches: with whole tiles in turn a fifth of its time went into
 // instruction misses.
 // Measured (777 rows of 6 heads on each of 4, after 23224 positions of 256):
-// 566 us, 796 TFLOP/s, 48 % of the tensor core's measured rate; about 2300
+// 577 us, 782 TFLOP/s, 47 % of the tensor core's measured rate; about 2300
 // cycles a tile, of which the softmax warps are busy 2000 (their instructions
 // depend on one another, and two of them share an issue slot with dequantising
-// warps).  With all rows seeing all positions 476 us; there, products issued
-// by one lane with values of its own took 562, and scales prepared by each
-// softmax warp for itself 542.
+// warps).  Before the code for far scales, with all rows seeing all positions,
+// 476 us; there, products issued by one lane with values of its own took 562,
+// and scales prepared by each softmax warp for itself 542.
 // The reference is followed lazily: O is rescaled only when it grows by more
 // than 2^8, which weights of up to 2^14 in fp16 leave room for.
 // Weights are rounded to fp16 (2^-11 each); their sum is of the unrounded

@@ -39,8 +39,8 @@
 // where units of very different length would leave SMs idle.
 //
 // Measured: 24 sequences of up to 65536 positions, 32 heads on 4 of 128, int8
-// 212 to 228 us (5.2 to 5.6 TB/s); one of 131071, 24 heads on 4 of 256, e4m3
-// 57 us (4.8 TB/s, the join included); 64 ragged ones of up to 2304 53 us.
+// 228 us (5.2 TB/s); one of 131071, 24 heads on 4 of 256, e4m3 57 us (4.8 TB/s,
+// the join included); 64 ragged ones of up to 2304 54 us.
 #pragma once
 
 #include "attn_common.cuh"
@@ -493,8 +493,8 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         if (wide) {
-          // both sums relative to 2^row, the largest of the lanes' references, or where values are large to 2^(row + 80): fp32
-          // has a place for them there
+          // both sums relative to 2^row, the largest of the lanes' references, or where values are large to 2^(row + 80):
+          // fp32 has a place for them there
           float row = at[x][c];
 #pragma unroll
           for (int i = 4; i < 32; i <<= 1) row = fmaxf(row, __shfl_xor_sync(0xffffffffu, row, i));

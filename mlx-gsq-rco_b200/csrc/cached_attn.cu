@@ -36,7 +36,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Token kernel by units of up to 16 rows: as many CTAs for each unit, up to 8, as fill `most` slots; twice as many where
 // a CTA would still have more than 64 tiles, since units of unlike length then even out (64 sequences, 4 heads of 256:
 // up to 8000 positions 154 us and with twice as many CTAs 101, all of 8000 169 and 175; up to 2304 positions, 36 tiles,
-// 49 and 42, but all of 2304 54 and 63).
+// 49 and 42, but all of 2304 54 and 63; of an earlier state of the kernel, to be compared with each other).
 void plan_units(Plan& p, int64_t units, int64_t most, int64_t tiles) {
   p.cluster = 1;
   while (p.cluster < 8 && units * p.cluster * (tiles > 64 * p.cluster ? 1 : 2) <= most) p.cluster *= 2;
@@ -52,9 +52,9 @@ void plan_units(Plan& p, int64_t units, int64_t most, int64_t tiles) {
 // which read the cache again (from L2).  A tile of 64 positions takes a CTA about as long in either, 1.0 us at 128
 // dimensions and 1.7 at 256.  In these terms a wave of the token kernel's CTAs costs 5 and its tiles; the row-block
 // kernel 8, 1 for every 32 rows (queries loaded, results stored), its tiles, and the joining launch 1 for every 1200
-// rows of parts.  Measured with 4 heads of 256 (us, token kernel and row blocks): one sequence, 40 rows, 2000
-// positions 18 and 20; 128 rows, 700 positions 16 and 24; 24 rows, 8000 positions 32 and 25; 8 sequences of 2000
-// positions, 24 rows 26 and 34, 96 rows 64 and 44.  Past 256 rows the row blocks are full.
+// rows of parts.  Fitted to measurements with 4 heads of 256, such as (us, token kernel and row blocks): one sequence,
+// 40 rows, 2000 positions 18 and 20; 128 rows, 700 positions 16 and 24; 24 rows, 8000 positions 32 and 25; 8 sequences
+// of 2000 positions, 24 rows 26 and 34, 96 rows 64 and 44.  Past 256 rows the row blocks are full.
 Plan plan_of(int64_t batch, int64_t n, int64_t heads, int64_t kv, int64_t dim, int64_t cap) {
   Plan p = {};
   const int64_t rows = n * (heads / kv), cached = batch * kv;  // heads in the cache

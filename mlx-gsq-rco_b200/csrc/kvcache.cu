@@ -12,8 +12,8 @@
 // Eight values a lane, a vector of 256 in a warp's registers or two of 128, so
 // nothing is read twice; a warp takes KV_EACH times as many, all
 // loaded before the first is worked on.  Measured with 8 x 1999 tokens of 4
-// heads of 256, bf16: append 33 us (98 MB, 3.0 TB/s: instructions), read 15 us
-// of e4m3 (6.5 TB/s: HBM), 18 us of int8.
+// heads of 256, bf16: append 33 us (98 MB, 3.0 TB/s: instructions, and waits
+// for loads), read 15 us of e4m3 (6.5 TB/s: HBM), 18 us of int8.
 #include <cuda_fp8.h>
 
 #include <cstdio>
