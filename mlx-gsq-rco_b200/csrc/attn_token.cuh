@@ -362,11 +362,13 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
       }
       // scores to base 2; s[x][e]: position p0 + g + 8 (e / 2), row 8x + 2t + e % 2
       const float ks0 = sc[g], ks1 = sc[g + 8];
-      // (of scale 0, whose vector has a part in the sum of weights only, as 2^-100: that sum stays finite)
+      // (of scale 0, whose vector has a part in the sum of weights only, as 2^-100, so that that sum stays finite, and with
+      // no weight in the other, whatever its codes)
       const float lv0 = log2_approx(sc[16 + g] > 0.f ? sc[16 + g] : 0x1p-100f);
       const float lv1 = log2_approx(sc[24 + g] > 0.f ? sc[24 + g] : 0x1p-100f);
       const float nan0 = sc[16 + g] - sc[16 + g], nan1 = sc[24 + g] - sc[24 + g];  // NaN where the scale is
-      const float lr0 = lv0 + AT_GAP, lr1 = lv1 + AT_GAP, lift0 = 15.f + nan0, lift1 = 15.f + nan1;
+      const float lr0 = lv0 + AT_GAP, lift0 = (sc[16 + g] > 0.f ? 15.f : -INFINITY) + nan0;
+      const float lr1 = lv1 + AT_GAP, lift1 = (sc[24 + g] > 0.f ? 15.f : -INFINITY) + nan1;
       const bool edge = p0 + 16 > span.base || p0 + 16 > span.len;  // warp-uniform: some row may not see all of these
       uint32_t pb[NT][2];
 #pragma unroll
@@ -411,8 +413,11 @@ __global__ void __launch_bounds__(32 * AT_WARPS, AtGeom<D, NT>::CTAS) attn_token
             for (int y = 0; y < NT; y++)
 #pragma unroll
               for (int c = 0; c < 2; c++) {
-                at[y][c] = m[y][c];
-                own[y][c] = l[y][c];
+                // (brought to 1 .. 2: beside m it may be 2^-100 times smaller)
+                const int power = min((int)(__float_as_uint(l[y][c]) >> 23 & 255), 253) - 127;
+                const bool some = l[y][c] > 0.f;
+                at[y][c] = some ? m[y][c] + (float)max(power, -126) : AT_LOWEST;
+                own[y][c] = some ? l[y][c] * exp2_int(-max(power, -126)) : l[y][c];
               }
           }
           if (wide) {

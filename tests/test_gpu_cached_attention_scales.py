@@ -77,13 +77,26 @@ def test_all_values_of_one_size(n, group, cap, power, fmt):
 
 @pytest.mark.parametrize("dim", [128, 256])
 @pytest.mark.parametrize("n,group,cap", SHAPES)
-@pytest.mark.parametrize("low,high", [(-148, 0), (0, -148), (-100, 118), (118, -100), (-60, 20), (20, -60)])
+@pytest.mark.parametrize("low,high", [(-148, 0), (0, -148), (-100, 118), (118, -100), (-60, 20), (20, -60), (-146, 60),
+                                      (50, 110)])
 def test_sizes_along_the_cache(n, group, cap, low, high, dim):
     """Rising: a row's last positions decide; falling: its first. The sum of weights has all of them alike."""
     cache = filled(1, 2, cap, dim, "int8", 64)
     cache.v_scale.copy_(torch.exp2(torch.linspace(low, high, cap, device=DEV)).expand_as(cache.v_scale))
     cache.v_scale[0, 0, 5::37] = 0
     compare(cache, n, group, cap, 65, gate=True)
+
+
+@pytest.mark.parametrize("n,group,cap", SHAPES)
+@pytest.mark.parametrize("power", [-130, -60, 0, 90])
+@pytest.mark.parametrize("share", [2, 1])
+def test_scales_of_zero_over_any_codes(n, group, cap, power, share):
+    """Every other vector's scale is 0, or all are: zero vectors, whatever their codes are."""
+    cache = filled(1, 1, cap, 128, "int8", 76)
+    cache.v_scale.fill_(2.0 ** power)
+    cache.v_scale[..., ::share] = 0
+    want = compare(cache, n, group, cap, 77)
+    assert share == 2 or not want.any()
 
 
 @pytest.mark.parametrize("n,group,cap", SHAPES)
@@ -95,6 +108,15 @@ def test_small_and_large_side_by_side(n, group, cap, every):
     small = (at % every != 0) if every <= 2 else (at // (every // 2)) % 2 == 0
     cache.v_scale[..., small] *= 2.0 ** -90
     compare(cache, n, group, cap, 67)
+
+
+@pytest.mark.parametrize("n,group,cap", SHAPES)
+@pytest.mark.parametrize("low,high", [(-130, 60), (-10, 60), (50, 115), (56, 100)])
+def test_any_size_anywhere(n, group, cap, low, high):
+    cache = filled(1, 1, cap, 128, "fp8", 78)
+    g = torch.Generator(device=DEV).manual_seed(79)
+    cache.v_scale.copy_(torch.exp2(low + (high - low) * torch.rand(cache.v_scale.shape, generator=g, device=DEV)))
+    compare(cache, n, group, cap, 80)
 
 
 @pytest.mark.parametrize("n,group", [(7, 2), (60, 6)])
