@@ -226,15 +226,16 @@ struct ArScales {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       // A vector of scale 0 has no part in the output, but in the sum of weights: where that is taken from the scaled
-      // weights it is weighted with the largest scale beside it, and that weight left out of P. NaN stays, with 1 / vs as
+      // weights it is weighted with the smallest scale beside it (a larger one would move the
+      // reference of rows that do not see its vector), and that weight left out of P. NaN stays, with 1 / vs as
       // 0, so that a row that does not see the position takes no harm.
       float lv = v[h] > 0.f ? log2_approx(v[h]) : -INFINITY;
       zeros[h] = __ballot_sync(0xffffffffu, v[h] == 0.f);
       if (zeros[h] && !wide) {
-        float top = lv;
+        float low = v[h] > 0.f ? lv : INFINITY;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (v[h] == 0.f) lv = top == -INFINITY ? -40.f : top;
+        for (int o = 16; o; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        if (v[h] == 0.f) lv = low == INFINITY ? -40.f : low;
       }
       const bool nan = isnan(v[h]);
       key[h] = k[h] * factor;

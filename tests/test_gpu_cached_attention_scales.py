@@ -194,3 +194,17 @@ def test_scores_so_large_that_a_scale_is_lost_beside_them(n, group, cap, power, 
     top = got[large].abs().amax(-1) * 2.0 ** -power
     # codes of a vector reach 127; a mean of vectors of equal score has codes of order 10 at least
     assert (top <= 127 * 1.01).all() and (top >= 5).all()
+
+
+@pytest.mark.parametrize("n,group,cap", SHAPES)
+def test_a_zero_vector_beside_a_large_one_that_a_row_does_not_see(n, group, cap):
+    if n == 1:
+        cap += 1
+    cache = filled(1, 1, cap, 128, "int8", 81)
+    cache.v_scale.fill_(2.0 ** -10)
+    cache.v_scale[..., -3] = 0
+    cache.v_scale[..., -1] = 2.0 ** 30
+    q = queries(1, n, group, 128, torch.bfloat16, 82)
+    start = cap - max(n, 2)
+    want, bound = wide_formula(q, cache, visible(1, n, cap, [start], None, None))
+    check(cached_attention(q, cache, i32(start)), want, bound)
